@@ -81,7 +81,7 @@ def draw(rng):
     seqs = min(64, int(math.exp(rng.uniform(0, math.log(rows + 1)))))
     if op == "preference":
         seqs = max(2, seqs - seqs % 2)
-    tokens = max(1, rows // seqs)
+    tokens = max(1, min(8192, rows // seqs))
     packed = op == "preference" and rng.random() < 0.5
     case = _case("", op, dtype, seqs, tokens, vocab, prompt=rng.choice([0.0, 0.125, 0.25]),
                  shifted=not packed and rng.random() < 0.4, packed=packed,
@@ -149,7 +149,8 @@ def prepare(case, seed):
         s = _sequence_sums(logp.double(), st)
         if case["average"]:
             s = s / _sequence_sums((st["targets"] >= 0).double(), st).clamp(min=1)
-        noise = 3.0 * torch.randn(s.shape, generator=gen, device=dev)
+        # policy and reference drift apart by about 0.1 a token, independently, besides a constant
+        noise = (0.3 if case["average"] else 1.0 + 0.1 * math.sqrt(T)) * torch.randn(s.shape, generator=gen, device=dev)
         st["ref_logprobs"] = (s + noise).float() if case["ref"] else None
     return st
 
