@@ -353,6 +353,78 @@ MOTEOPT_API int moteopt_selftest_grad_divide(const float* a, float d, float* out
 MOTEOPT_API int moteopt_selftest_wait_timeout(int mode, double limit_seconds, int* counter, int* status,
                                               unsigned long long* elapsed_ns, moteopt_stream_t stream);
 
+/* ---- losses on logits, for post-training (the reference trains on such losses in mote/train/dpo.py, kto.py and
+ *      rlvr.py, with the clip and AdamW of this library's kind behind them: dpo.py:217, kto.py:151, rlvr.py:308).
+ *
+ * The logits are [seqs][tokens][vocab], fp32 or bf16, the last axis contiguous and the others with strides (in elements),
+ * so a shifted view needs no copy; packed sequences are seqs = 1. `targets` are int64. For a position with logits z,
+ * x = z / temperature and target y: lse = log sum_j exp x_j, logp = x_y - lse. A position whose target is negative does
+ * not count: its logits are not read, its logp and lse are 0, its gradient is 0. A target >= vocab gives NaN. -inf logits
+ * have probability 0. Gradients are written contiguous, [seqs][tokens][vocab], in the logits' type, each rounded once;
+ * the sums behind them are fp32 within a thread and fp64 above, in a fixed order, so the same call gives the same bits.
+ * At most 2^27 - 1 positions. */
+typedef struct moteopt_logits {
+  const void* data;
+  int dtype;                    /* MOTEOPT_DTYPE_* */
+  int64_t seqs, tokens, vocab;
+  int64_t seq_stride, token_stride;
+} moteopt_logits;
+
+/* One value per position (targets: int64; everything else: fp32), with strides in elements; a stride of 0 broadcasts. */
+typedef struct moteopt_positions {
+  const void* data;
+  int64_t seq_stride, token_stride;
+} moteopt_positions;
+
+/* logprobs, lse: [seqs * tokens] fp32, contiguous; lse may be NULL. One launch. */
+MOTEOPT_API int moteopt_token_logprobs(const moteopt_logits* logits, const moteopt_positions* targets, double temperature,
+                                       float* logprobs, float* lse, moteopt_stream_t stream);
+/* grad_logits = grad_logprobs ([j == y] - exp(x_j - lse)) / temperature from the logprobs and lse that
+ * moteopt_token_logprobs gave for these logits. A position whose grad_logprobs is 0 is not read and gets 0. */
+MOTEOPT_API int moteopt_token_logprobs_backward(const moteopt_logits* logits, const moteopt_positions* targets,
+                                                double temperature, const moteopt_positions* logprobs,
+                                                const moteopt_positions* lse, const moteopt_positions* grad_logprobs,
+                                                void* grad_logits, moteopt_stream_t stream);
+
+/* The clipped policy loss with a KL term. Per counted position, with w its weight (1 without weights; a position of
+ * weight 0 does not count): r = exp(logp - old), loss -= w min(r A, clip(r, 1 - clip_low, 1 + clip_high) A), and
+ * loss += w kl_coef k with k = exp(d) - d - 1, d = ref - logp; all divided by the divisor. */
+typedef struct moteopt_policy {
+  moteopt_positions advantages, old_logprobs;
+  moteopt_positions ref_logprobs;   /* data NULL: no KL term (kl_coef must be 0) */
+  moteopt_positions weights;        /* data NULL: 1 */
+  double clip_low, clip_high, kl_coef;
+  double divisor;                   /* not 0 */
+  const float* divisor_device;      /* or, when non-NULL, the divisor as a DEVICE fp32 scalar */
+} moteopt_policy;
+/* sums (device, 4 floats) = [loss, sum of w, sum of w k / divisor, sum of w over the positions whose ratio was clipped];
+ * logprobs [seqs * tokens]; grad_logits NULL: no gradient. */
+MOTEOPT_API size_t moteopt_policy_loss_workspace_size(const moteopt_logits* logits);
+MOTEOPT_API int moteopt_policy_loss(const moteopt_logits* logits, const moteopt_positions* targets,
+                                    const moteopt_policy* policy, double temperature, float* sums, float* logprobs,
+                                    void* grad_logits, void* workspace, size_t workspace_bytes, moteopt_stream_t stream);
+
+/* The paired preference loss over `sequences` sequences, the first half chosen, the second half rejected, in order:
+ * s = the sum of a sequence's logp (the mean with `average`; 0 for a sequence without a counted position),
+ * u = beta ((s_i - ref_i) - (s_j - ref_j)), j = i + sequences / 2,
+ * loss = sum over i of (-(1 - label_smoothing) log sigmoid(u) - label_smoothing log sigmoid(-u)) / divisor. */
+typedef struct moteopt_preference {
+  int64_t sequences;
+  const int32_t* cu_seqlens;        /* NULL: sequence q is logits' seq q. Else (logits->seqs == 1) device, sequences + 1
+                                       ascending row offsets; rows outside [first, last) do not count */
+  const float* ref_logprobs;        /* device [sequences], or NULL: 0 */
+  double beta, label_smoothing;
+  int average;
+  double divisor;                   /* not 0 */
+  const float* divisor_device;      /* or, when non-NULL, the divisor as a DEVICE fp32 scalar */
+} moteopt_preference;
+/* loss: 1 float; rewards [sequences] = beta (s - ref); logprobs [sequences] = s; grad_logits NULL: no gradient. */
+MOTEOPT_API size_t moteopt_preference_loss_workspace_size(const moteopt_logits* logits, int64_t sequences);
+MOTEOPT_API int moteopt_preference_loss(const moteopt_logits* logits, const moteopt_positions* targets,
+                                        const moteopt_preference* preference, double temperature, float* loss,
+                                        float* rewards, float* logprobs, void* grad_logits, void* workspace,
+                                        size_t workspace_bytes, moteopt_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

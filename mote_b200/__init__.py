@@ -4,6 +4,7 @@ The public names load the CUDA library (libmoteopt.so) on first use; `mote_b200.
 `mote_b200.build` work without it.
 
     from mote_b200 import Muon, AdamW, MultiOpt, build_optimizer, split_muon_params, clip_grad_norm_, newton_schulz
+    from mote_b200 import token_logprobs, token_logprobs_backward, policy_loss, preference_loss
 """
 
 _LAZY = {
@@ -12,6 +13,8 @@ _LAZY = {
     "clip_grad_norm_": "ops", "newton_schulz": "ops",
     "optimizer_step": "functional", "MuonItem": "functional", "AdamWItem": "functional",
     "CapturedStep": "functional", "moe_update_bias": "functional",
+    "token_logprobs": "losses", "token_logprobs_backward": "losses", "policy_loss": "losses",
+    "preference_loss": "losses",
 }
 
 

@@ -38,6 +38,9 @@ EXPORTS = (
     "moteopt_newton_schulz_workspace_size_variant", "moteopt_newton_schulz_variant",
     "moteopt_grad_sumsq_tensors", "moteopt_peer_reduce_workspace_size", "moteopt_peer_reduce_sumsq",
     "moteopt_clip_coef_from_tensor_sums", "moteopt_selftest_grad_divide",
+    "moteopt_token_logprobs", "moteopt_token_logprobs_backward",
+    "moteopt_policy_loss_workspace_size", "moteopt_policy_loss",
+    "moteopt_preference_loss_workspace_size", "moteopt_preference_loss",
 )
 MAX_PEERS = 8
 
@@ -80,6 +83,27 @@ class MoeBias(C.Structure):
 class PeerPiece(C.Structure):
     _fields_ = [("dst", C.c_void_p), ("src", C.c_void_p * MAX_PEERS), ("numel", C.c_int64), ("dtype", C.c_int),
                 ("tensor", C.c_int)]
+
+
+class Logits(C.Structure):
+    _fields_ = [("data", C.c_void_p), ("dtype", C.c_int), ("seqs", C.c_int64), ("tokens", C.c_int64),
+                ("vocab", C.c_int64), ("seq_stride", C.c_int64), ("token_stride", C.c_int64)]
+
+
+class Positions(C.Structure):
+    _fields_ = [("data", C.c_void_p), ("seq_stride", C.c_int64), ("token_stride", C.c_int64)]
+
+
+class Policy(C.Structure):
+    _fields_ = [("advantages", Positions), ("old_logprobs", Positions), ("ref_logprobs", Positions),
+                ("weights", Positions), ("clip_low", C.c_double), ("clip_high", C.c_double), ("kl_coef", C.c_double),
+                ("divisor", C.c_double), ("divisor_device", C.c_void_p)]
+
+
+class Preference(C.Structure):
+    _fields_ = [("sequences", C.c_int64), ("cu_seqlens", C.c_void_p), ("ref_logprobs", C.c_void_p), ("beta", C.c_double),
+                ("label_smoothing", C.c_double), ("average", C.c_int), ("divisor", C.c_double),
+                ("divisor_device", C.c_void_p)]
 
 
 class MoteoptError(RuntimeError):
@@ -146,6 +170,15 @@ def _load() -> C.CDLL:
         "moteopt_peer_reduce_workspace_size": (sz, [C.POINTER(PeerPiece), i32]),
         "moteopt_peer_reduce_sumsq": (i32, [C.POINTER(PeerPiece), i32, i32, i32, dbl, vp, vp, sz, vp]),
         "moteopt_clip_coef_from_tensor_sums": (i32, [vp, i32, i32, i32, dbl, vp, vp]),
+        "moteopt_token_logprobs": (i32, [C.POINTER(Logits), C.POINTER(Positions), dbl, vp, vp, vp]),
+        "moteopt_token_logprobs_backward": (i32, [C.POINTER(Logits), C.POINTER(Positions), dbl, C.POINTER(Positions),
+                                                  C.POINTER(Positions), C.POINTER(Positions), vp, vp]),
+        "moteopt_policy_loss_workspace_size": (sz, [C.POINTER(Logits)]),
+        "moteopt_policy_loss": (i32, [C.POINTER(Logits), C.POINTER(Positions), C.POINTER(Policy), dbl, vp, vp, vp, vp, sz,
+                                      vp]),
+        "moteopt_preference_loss_workspace_size": (sz, [C.POINTER(Logits), i64]),
+        "moteopt_preference_loss": (i32, [C.POINTER(Logits), C.POINTER(Positions), C.POINTER(Preference), dbl, vp, vp, vp,
+                                          vp, vp, sz, vp]),
     }
     for name, (res, args) in sig.items():
         f = getattr(lib, name)

@@ -1,0 +1,457 @@
+// C-ABI entry points of the losses on logits (include/moteopt.h): argument checks, the choice of kernels and the launches.
+// Included by moteopt.cu, whose error and launch macros it uses. No device memory is allocated here, nothing synchronises.
+#pragma once
+
+namespace {
+
+using namespace moteopt::loss;
+
+// Rows of up to this many bytes take the warp-per-rows kernels, longer ones a block each.
+constexpr int64_t kShortBytes = kTileBytes - 16;
+
+int64_t esize(int dtype) { return dtype == MOTEOPT_DTYPE_BF16 ? 2 : 4; }
+
+bool positions_fit(const moteopt_logits* z) {
+  return z->tokens == 0 || z->seqs <= ((int64_t{1} << 27) - 1) / z->tokens;
+}
+
+int check_logits(const char* who, const moteopt_logits* z, const moteopt_positions* y, Rows* R, double temperature) {
+  const std::string w(who);
+  if (!z || !y) return fail(MOTEOPT_ERR_INVALID, w + ": null logits or targets");
+  if (z->dtype != MOTEOPT_DTYPE_F32 && z->dtype != MOTEOPT_DTYPE_BF16)
+    return fail(MOTEOPT_ERR_INVALID, w + ": logits must be fp32 or bf16");
+  if (z->seqs < 0 || z->tokens < 0 || z->vocab < 1) return fail(MOTEOPT_ERR_INVALID, w + ": bad logits shape");
+  if (z->vocab >= (int64_t{1} << 31)) return fail(MOTEOPT_ERR_LIMIT, w + ": a vocabulary of 2^31 or more");
+  if (!positions_fit(z)) return fail(MOTEOPT_ERR_LIMIT, w + ": 2^27 positions or more");
+  if (!(temperature > 0.0) || !std::isfinite(temperature) || !std::isfinite(1.0 / temperature))
+    return fail(MOTEOPT_ERR_INVALID, w + ": the temperature must be positive and finite");
+  const int64_t n = z->seqs * z->tokens;
+  if (n > 0 && (!z->data || !y->data)) return fail(MOTEOPT_ERR_INVALID, w + ": null logits or targets");
+  if (reinterpret_cast<uint64_t>(z->data) % esize(z->dtype) != 0 || reinterpret_cast<uint64_t>(y->data) % 8 != 0)
+    return fail(MOTEOPT_ERR_INVALID, w + ": logits or targets are not aligned to their elements");
+  std::memset(R, 0, sizeof(*R));
+  R->z = static_cast<const char*>(z->data);
+  R->y = static_cast<const int64_t*>(y->data);
+  R->z_seq = z->seq_stride;
+  R->z_tok = z->token_stride;
+  R->y_seq = y->seq_stride;
+  R->y_tok = y->token_stride;
+  R->n = static_cast<uint32_t>(n);
+  R->tokens = static_cast<uint32_t>(z->tokens);
+  R->vocab = static_cast<uint32_t>(z->vocab);
+  R->inv_t = 1.0 / temperature;
+  const double c = kLog2e * R->inv_t;
+  float hi = static_cast<float>(c);
+  if (static_cast<double>(hi) >= c) hi = std::nextafter(hi, 0.f);
+  R->c_hi = hi;
+  R->c_lo = static_cast<float>(c - static_cast<double>(hi));
+  if (!(R->c_lo > 0.f) || !std::isfinite(hi)) return fail(MOTEOPT_ERR_INVALID, w + ": the temperature is out of range");
+  return MOTEOPT_OK;
+}
+
+Per per_of(const moteopt_positions& p) { return Per{static_cast<const float*>(p.data), p.seq_stride, p.token_stride}; }
+
+// A launch behind another one of the same call: its blocks may be placed before that one has ended (they wait for it
+// themselves). The first launch of a call (`first`) is an ordinary one.
+template <typename Args>
+int launch_after(void (*kernel)(Args), const Args& A, unsigned grid, unsigned block, cudaStream_t st, const char* what,
+                 bool first = false) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid, 1, 1);
+  cfg.blockDim = dim3(block, 1, 1);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = first ? 0 : 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, A);
+  if (e != cudaSuccess) return fail(MOTEOPT_ERR_CUDA, std::string(what) + ": " + cudaGetErrorString(e));
+  g_launches.fetch_add(1, std::memory_order_relaxed);
+  return MOTEOPT_OK;
+}
+
+template <typename Args>
+int launch_cluster(void (*kernel)(Args), const Args& A, unsigned rows, unsigned cl, unsigned block, cudaStream_t st,
+                   const char* what) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(rows * cl, 1, 1);
+  cfg.blockDim = dim3(block, 1, 1);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = cl;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = cl > 1 ? 1 : 0;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, A);
+  if (e != cudaSuccess) return fail(MOTEOPT_ERR_CUDA, std::string(what) + ": " + cudaGetErrorString(e));
+  g_launches.fetch_add(1, std::memory_order_relaxed);
+  return MOTEOPT_OK;
+}
+
+bool short_rows(int dtype, int64_t vocab) { return vocab * esize(dtype) <= kShortBytes; }
+
+// The warps' share of short rows: as many rows as fit kTileBytes, at most kTileRows.
+void tile_shape(int dtype, int64_t vocab, int* per_warp, uint32_t* pitch) {
+  *pitch = static_cast<uint32_t>((vocab * esize(dtype) + 16 - esize(dtype) + 15) / 16 * 16);
+  *per_warp = std::max(1, std::min(kTileRows, static_cast<int>(kTileBytes / *pitch)));
+}
+
+template <typename T, bool kPolicy>
+int launch_tile_t(const TileArgs& A, cudaStream_t st) {
+  const int64_t tiles = cdiv(A.R.n, A.per_warp);
+  const size_t smem = static_cast<size_t>(kTileWarps) * A.per_warp * A.pitch;
+  tile_kernel<T, kPolicy><<<static_cast<unsigned>(cdiv(tiles, kTileWarps)), kTileWarps * 32, smem, st>>>(A);
+  MO_LAUNCHED("loss tile_kernel");
+  return MOTEOPT_OK;
+}
+int launch_tile(int dtype, const TileArgs& A, bool policy, cudaStream_t st) {
+  if (dtype == MOTEOPT_DTYPE_BF16)
+    return policy ? launch_tile_t<__nv_bfloat16, true>(A, st) : launch_tile_t<__nv_bfloat16, false>(A, st);
+  return policy ? launch_tile_t<float, true>(A, st) : launch_tile_t<float, false>(A, st);
+}
+
+// Blocks per row of the long forward pass: enough for two blocks on every SM, each with at least 1024 vectors.
+int row_cluster(const Rows& R, int dtype, int sms) {
+  const int64_t vecs = R.vocab * esize(dtype) / 16;
+  int cl = 1;
+  while (cl < kMaxCluster && static_cast<int64_t>(R.n) * cl * 2 <= 2 * sms && vecs / (cl * 2) >= 1024) cl *= 2;
+  return cl;
+}
+int launch_rows(int dtype, RowArgs A, int sms, cudaStream_t st) {
+  A.cl = row_cluster(A.R, dtype, sms);
+  return dtype == MOTEOPT_DTYPE_BF16
+             ? launch_cluster(row_kernel<__nv_bfloat16>, A, A.R.n, A.cl, kRowThreads, st, "loss row_kernel")
+             : launch_cluster(row_kernel<float>, A, A.R.n, A.cl, kRowThreads, st, "loss row_kernel");
+}
+
+// logp, lse (or logp64, coef = 0) of every row
+int launch_forward(int dtype, const Rows& R, float* logp, float* lse, double* logp64, float* coef, int sms, cudaStream_t st) {
+  if (short_rows(dtype, R.vocab)) {
+    TileArgs A;
+    std::memset(&A, 0, sizeof(A));
+    A.R = R;
+    A.logp = logp;
+    A.lse = lse;
+    A.logp64 = logp64;
+    A.coef = coef;
+    tile_shape(dtype, R.vocab, &A.per_warp, &A.pitch);
+    return launch_tile(dtype, A, false, st);
+  }
+  RowArgs A;
+  std::memset(&A, 0, sizeof(A));
+  A.R = R;
+  A.logp = logp;
+  A.lse = lse;
+  A.logp64 = logp64;
+  A.coef = coef;
+  return launch_rows(dtype, A, sms, st);
+}
+
+int launch_gradient(int dtype, GradArgs A, cudaStream_t st, bool first = false) {
+  const int64_t vecs = A.R.vocab * esize(dtype) / 16;
+  if (vecs < 128) {
+    const unsigned grid = static_cast<unsigned>(cdiv(A.R.n, kGradThreads / 32));
+    return dtype == MOTEOPT_DTYPE_BF16
+               ? launch_after(grad_short_kernel<__nv_bfloat16>, A, grid, kGradThreads, st, "loss grad_short_kernel", first)
+               : launch_after(grad_short_kernel<float>, A, grid, kGradThreads, st, "loss grad_short_kernel", first);
+  }
+  A.pieces = static_cast<uint32_t>(cdiv(vecs, kGradThreads * kGradVecs));
+  if (static_cast<int64_t>(A.R.n) * A.pieces >= (int64_t{1} << 31))
+    return fail(MOTEOPT_ERR_LIMIT, "loss gradient: too many logits for one call");
+  const unsigned grid = A.R.n * A.pieces;
+  return dtype == MOTEOPT_DTYPE_BF16
+             ? launch_after(grad_kernel<__nv_bfloat16>, A, grid, kGradThreads, st, "loss grad_kernel", first)
+             : launch_after(grad_kernel<float>, A, grid, kGradThreads, st, "loss grad_kernel", first);
+}
+
+// The held policy kernel's shape: threads and blocks per row that hold a row's vectors at 32 logits a thread; 0 where 16
+// blocks of 512 threads do not.
+struct HeldShape {
+  int threads, cl;
+};
+HeldShape held_shape(int dtype, int64_t vocab) {
+  const int64_t per = 32 * esize(dtype) / 16;   // vectors a thread
+  const int64_t vecs = vocab * esize(dtype) / 16;
+  if (vecs <= 256 * per) return {256, 1};
+  for (int cl = 1; cl <= kMaxCluster; cl *= 2)
+    if (cdiv(vecs, cl) <= 512 * per) return {512, cl};
+  return {0, 0};
+}
+
+constexpr int kSumShare = 4096;   // partials one block adds up
+constexpr int kSumBlocks = 128;
+
+struct PolicyLayout {
+  size_t partials, sums, logp64, lse, coef, bytes;
+  bool short_, held;
+};
+PolicyLayout policy_layout(int dtype, int64_t n, int64_t vocab) {
+  PolicyLayout L;
+  L.short_ = short_rows(dtype, vocab);
+  L.held = !L.short_ && held_shape(dtype, vocab).cl > 0;
+  int per = 1;
+  uint32_t pitch = 0;
+  if (L.short_) tile_shape(dtype, vocab, &per, &pitch);
+  L.partials = kHeaderBytes;
+  const int64_t parts = L.short_ ? cdiv(n, per) : n;
+  L.sums = align_up(L.partials + 32 * static_cast<size_t>(parts), 256);
+  L.logp64 = L.sums + 32 * kSumBlocks;
+  const bool kept = !L.short_ && !L.held;
+  L.lse = align_up(L.logp64 + (kept ? 8 * static_cast<size_t>(n) : 0), 256);
+  L.coef = align_up(L.lse + (kept ? 4 * static_cast<size_t>(n) : 0), 256);
+  L.bytes = align_up(L.coef + (kept ? 4 * static_cast<size_t>(n) : 0), 256);
+  return L;
+}
+
+int launch_sums(const double* partials, int64_t n, double* mid, float* out, cudaStream_t st) {
+  SumArgs A = {partials, static_cast<uint32_t>(n), mid, out};
+  if (n > kSumShare) {
+    const unsigned blocks = static_cast<unsigned>(std::min<int64_t>(kSumBlocks, cdiv(n, kSumShare / 4)));
+    MO_TRY(launch_after(sum_kernel, A, blocks, kSumThreads, st, "loss sum_kernel"));
+    A.partials = mid;
+    A.n = blocks;
+  }
+  return launch_after(sum_kernel, A, 1, kSumThreads, st, "loss sum_kernel");
+}
+
+struct PreferenceLayout {
+  size_t logp64, lse, coef, pairs, bytes;
+};
+PreferenceLayout preference_layout(int64_t n, int64_t pairs) {
+  PreferenceLayout L;
+  L.logp64 = kHeaderBytes;
+  L.lse = align_up(L.logp64 + 8 * static_cast<size_t>(n), 256);
+  L.coef = align_up(L.lse + 4 * static_cast<size_t>(n), 256);
+  L.pairs = align_up(L.coef + 4 * static_cast<size_t>(n), 256);
+  L.bytes = align_up(L.pairs + 8 * static_cast<size_t>(pairs), 256);
+  return L;
+}
+
+int check_divisor(const char* who, double divisor, const float* divisor_device) {
+  if (!divisor_device && (!(divisor != 0.0) || !std::isfinite(divisor)))
+    return fail(MOTEOPT_ERR_INVALID, std::string(who) + ": the divisor must be finite and not 0");
+  return MOTEOPT_OK;
+}
+
+// the clusters of 16 blocks that the longest rows take are beyond the portable size
+int loss_setup(int* sms) {
+  MO_TRY(device_setup(sms));
+  static std::atomic<unsigned long long> ready{0};   // a bit per device
+  int dev = 0;
+  MO_CUDA(cudaGetDevice(&dev));
+  if (ready.load(std::memory_order_acquire) >> dev & 1) return MOTEOPT_OK;
+  const void* wide[] = {reinterpret_cast<const void*>(row_kernel<__nv_bfloat16>),
+                        reinterpret_cast<const void*>(row_kernel<float>),
+                        reinterpret_cast<const void*>(held_kernel<__nv_bfloat16, 512>),
+                        reinterpret_cast<const void*>(held_kernel<float, 512>)};
+  for (const void* k : wide) MO_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+  ready.fetch_or(1ull << dev, std::memory_order_release);
+  return MOTEOPT_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int moteopt_token_logprobs(const moteopt_logits* logits, const moteopt_positions* targets, double temperature,
+                           float* logprobs, float* lse, moteopt_stream_t stream) {
+  Rows R;
+  MO_TRY(check_logits("moteopt_token_logprobs", logits, targets, &R, temperature));
+  if (R.n == 0) return MOTEOPT_OK;
+  if (!logprobs) return fail(MOTEOPT_ERR_INVALID, "moteopt_token_logprobs: null output");
+  int sms = 0;
+  MO_TRY(loss_setup(&sms));
+  return launch_forward(logits->dtype, R, logprobs, lse, nullptr, nullptr, sms, reinterpret_cast<cudaStream_t>(stream));
+}
+
+int moteopt_token_logprobs_backward(const moteopt_logits* logits, const moteopt_positions* targets, double temperature,
+                                    const moteopt_positions* logprobs, const moteopt_positions* lse,
+                                    const moteopt_positions* grad_logprobs, void* grad_logits, moteopt_stream_t stream) {
+  GradArgs A;
+  std::memset(&A, 0, sizeof(A));
+  MO_TRY(check_logits("moteopt_token_logprobs_backward", logits, targets, &A.R, temperature));
+  if (A.R.n == 0) return MOTEOPT_OK;
+  if (!logprobs || !lse || !grad_logprobs || !logprobs->data || !lse->data || !grad_logprobs->data || !grad_logits)
+    return fail(MOTEOPT_ERR_INVALID, "moteopt_token_logprobs_backward: null pointer");
+  int sms = 0;
+  MO_TRY(loss_setup(&sms));
+  A.logp = per_of(*logprobs);
+  A.lse = per_of(*lse);
+  A.coef = per_of(*grad_logprobs);
+  A.grad = grad_logits;
+  return launch_gradient(logits->dtype, A, reinterpret_cast<cudaStream_t>(stream), true);
+}
+
+size_t moteopt_policy_loss_workspace_size(const moteopt_logits* logits) {
+  if (!logits || logits->seqs < 0 || logits->tokens < 0 || logits->vocab < 1 ||
+      (logits->dtype != MOTEOPT_DTYPE_F32 && logits->dtype != MOTEOPT_DTYPE_BF16) || !positions_fit(logits))
+    return 0;
+  return policy_layout(logits->dtype, logits->seqs * logits->tokens, logits->vocab).bytes;
+}
+
+int moteopt_policy_loss(const moteopt_logits* logits, const moteopt_positions* targets, const moteopt_policy* policy,
+                        double temperature, float* sums, float* logprobs, void* grad_logits, void* workspace,
+                        size_t workspace_bytes, moteopt_stream_t stream) {
+  const char* const who = "moteopt_policy_loss";
+  Rows R;
+  MO_TRY(check_logits(who, logits, targets, &R, temperature));
+  if (!policy || !sums) return fail(MOTEOPT_ERR_INVALID, "moteopt_policy_loss: null pointer");
+  MO_TRY(check_divisor(who, policy->divisor, policy->divisor_device));
+  if (!(policy->clip_low >= 0.0) || !(policy->clip_high >= 0.0) || !std::isfinite(policy->kl_coef))
+    return fail(MOTEOPT_ERR_INVALID, "moteopt_policy_loss: the clips must not be negative, the KL coefficient finite");
+  if (R.n > 0 && (!logprobs || !policy->advantages.data || !policy->old_logprobs.data))
+    return fail(MOTEOPT_ERR_INVALID, "moteopt_policy_loss: null pointer");
+  if (policy->kl_coef != 0.0 && R.n > 0 && !policy->ref_logprobs.data)
+    return fail(MOTEOPT_ERR_INVALID, "moteopt_policy_loss: a KL coefficient without reference log-probabilities");
+  const PolicyLayout L = policy_layout(logits->dtype, R.n, R.vocab);
+  MO_TRY(check_ws(workspace, workspace_bytes, L.bytes));
+  int sms = 0;
+  MO_TRY(loss_setup(&sms));
+  const cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  if (R.n == 0) {
+    MO_CUDA(cudaMemsetAsync(sums, 0, 4 * sizeof(float), st));
+    return MOTEOPT_OK;
+  }
+  char* const ws = static_cast<char*>(workspace);
+  Policy P;
+  std::memset(&P, 0, sizeof(P));
+  P.adv = per_of(policy->advantages);
+  P.old_lp = per_of(policy->old_logprobs);
+  P.ref_lp = per_of(policy->ref_logprobs);
+  P.weight = per_of(policy->weights);
+  P.clip_lo = 1.0 - policy->clip_low;
+  P.clip_hi = 1.0 + policy->clip_high;
+  P.kl = policy->kl_coef;
+  P.inv_div = policy->divisor_device ? 0.0 : 1.0 / policy->divisor;
+  P.div = policy->divisor_device;
+  double* const partials = reinterpret_cast<double*>(ws + L.partials);
+  double* const mid = reinterpret_cast<double*>(ws + L.sums);
+  if (L.short_) {
+    TileArgs A;
+    std::memset(&A, 0, sizeof(A));
+    A.R = R;
+    A.P = P;
+    A.logp = logprobs;
+    A.grad = grad_logits;
+    A.partials = partials;
+    tile_shape(logits->dtype, R.vocab, &A.per_warp, &A.pitch);
+    MO_TRY(launch_tile(logits->dtype, A, true, st));
+    return launch_sums(partials, cdiv(R.n, A.per_warp), mid, sums, st);
+  }
+  if (L.held) {
+    HeldArgs A;
+    std::memset(&A, 0, sizeof(A));
+    A.R = R;
+    A.P = P;
+    A.logp = logprobs;
+    A.grad = grad_logits;
+    A.partials = partials;
+    const HeldShape s = held_shape(logits->dtype, R.vocab);
+    A.cl = s.cl;
+    const bool bf = logits->dtype == MOTEOPT_DTYPE_BF16;
+    auto* const k = s.threads == 256 ? (bf ? held_kernel<__nv_bfloat16, 256> : held_kernel<float, 256>)
+                                     : (bf ? held_kernel<__nv_bfloat16, 512> : held_kernel<float, 512>);
+    MO_TRY(launch_cluster(k, A, R.n, s.cl, s.threads, st, "loss held_kernel"));
+    return launch_sums(partials, R.n, mid, sums, st);
+  }
+  double* const logp64 = reinterpret_cast<double*>(ws + L.logp64);
+  float* const lse = reinterpret_cast<float*>(ws + L.lse);
+  float* const coef = reinterpret_cast<float*>(ws + L.coef);
+  MO_TRY(launch_forward(logits->dtype, R, nullptr, lse, logp64, coef, sms, st));
+  PolicyRowsArgs B;
+  std::memset(&B, 0, sizeof(B));
+  B.R = R;
+  B.P = P;
+  B.logp64 = logp64;
+  B.logp = logprobs;
+  B.coef = coef;
+  B.partials = partials;
+  const unsigned blocks = static_cast<unsigned>(cdiv(R.n, 256));
+  MO_TRY(launch_after(policy_rows_kernel, B, blocks, 256, st, "loss policy_rows_kernel"));
+  MO_TRY(launch_sums(partials, blocks, mid, sums, st));
+  if (!grad_logits) return MOTEOPT_OK;
+  GradArgs G;
+  std::memset(&G, 0, sizeof(G));
+  G.R = R;
+  G.logp64 = logp64;
+  G.lse_row = lse;
+  G.coef_row = coef;
+  G.grad = grad_logits;
+  return launch_gradient(logits->dtype, G, st);
+}
+
+size_t moteopt_preference_loss_workspace_size(const moteopt_logits* logits, int64_t sequences) {
+  if (!logits || logits->seqs < 0 || logits->tokens < 0 || sequences < 0 || !positions_fit(logits)) return 0;
+  return preference_layout(logits->seqs * logits->tokens, sequences / 2).bytes;
+}
+
+int moteopt_preference_loss(const moteopt_logits* logits, const moteopt_positions* targets,
+                            const moteopt_preference* preference, double temperature, float* loss, float* rewards,
+                            float* logprobs, void* grad_logits, void* workspace, size_t workspace_bytes,
+                            moteopt_stream_t stream) {
+  const char* const who = "moteopt_preference_loss";
+  Rows R;
+  MO_TRY(check_logits(who, logits, targets, &R, temperature));
+  if (!preference || !loss) return fail(MOTEOPT_ERR_INVALID, "moteopt_preference_loss: null pointer");
+  const moteopt_preference& p = *preference;
+  MO_TRY(check_divisor(who, p.divisor, p.divisor_device));
+  if (p.sequences < 0 || p.sequences % 2 != 0 || p.sequences >= (int64_t{1} << 27))
+    return fail(MOTEOPT_ERR_INVALID, "moteopt_preference_loss: the sequences are pairs: an even number of them");
+  if (p.cu_seqlens ? logits->seqs != 1 : p.sequences != logits->seqs)
+    return fail(MOTEOPT_ERR_INVALID, "moteopt_preference_loss: sequences do not match the logits");
+  if (!std::isfinite(p.beta) || !(p.label_smoothing >= 0.0 && p.label_smoothing <= 1.0))
+    return fail(MOTEOPT_ERR_INVALID, "moteopt_preference_loss: beta must be finite, label_smoothing in [0, 1]");
+  if (p.sequences > 0 && (!rewards || !logprobs)) return fail(MOTEOPT_ERR_INVALID, "moteopt_preference_loss: null pointer");
+  const PreferenceLayout L = preference_layout(R.n, p.sequences / 2);
+  MO_TRY(check_ws(workspace, workspace_bytes, L.bytes));
+  int sms = 0;
+  MO_TRY(loss_setup(&sms));
+  const cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  if (p.sequences == 0) {
+    MO_CUDA(cudaMemsetAsync(loss, 0, sizeof(float), st));
+    if (grad_logits && R.n > 0)
+      MO_CUDA(cudaMemsetAsync(grad_logits, 0, static_cast<size_t>(R.n) * R.vocab * esize(logits->dtype), st));
+    return MOTEOPT_OK;
+  }
+  char* const ws = static_cast<char*>(workspace);
+  double* const logp64 = reinterpret_cast<double*>(ws + L.logp64);
+  float* const lse = reinterpret_cast<float*>(ws + L.lse);
+  float* const coef = reinterpret_cast<float*>(ws + L.coef);
+  double* const pair_loss = reinterpret_cast<double*>(ws + L.pairs);
+  R.cu = p.cu_seqlens;
+  R.n_seqs = static_cast<int>(p.sequences);
+  if (R.n > 0) MO_TRY(launch_forward(logits->dtype, R, nullptr, lse, logp64, coef, sms, st));
+  PairArgs A;
+  std::memset(&A, 0, sizeof(A));
+  A.R = R;
+  A.pairs = static_cast<int>(p.sequences / 2);
+  A.ref = p.ref_logprobs;
+  A.beta = p.beta;
+  A.eps = p.label_smoothing;
+  A.inv_div = p.divisor_device ? 0.0 : 1.0 / p.divisor;
+  A.div = p.divisor_device;
+  A.average = p.average;
+  A.logp64 = logp64;
+  A.coef = grad_logits ? coef : nullptr;
+  A.pair_loss = pair_loss;
+  A.rewards = rewards;
+  A.seq_logp = logprobs;
+  MO_TRY(launch_after(pair_kernel, A, static_cast<unsigned>(A.pairs), kPairThreads, st, "loss pair_kernel", R.n == 0));
+  GradArgs G;
+  std::memset(&G, 0, sizeof(G));
+  G.R = R;
+  G.logp64 = logp64;
+  G.lse_row = lse;
+  G.coef_row = coef;
+  G.grad = grad_logits;
+  G.pair_loss = pair_loss;
+  G.pairs = A.pairs;
+  G.loss = loss;
+  if (!grad_logits || R.n == 0) return launch_after(pair_sum_kernel, G, 1, 32, st, "loss pair_sum_kernel");
+  return launch_gradient(logits->dtype, G, st);
+}
+
+}  // extern "C"

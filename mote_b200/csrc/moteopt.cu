@@ -14,6 +14,7 @@
 #include <vector>
 
 #include "moteopt.h"
+#include "loss_kernels.cuh"
 #include "mt_kernels.cuh"
 #include "ns_gemm.cuh"
 
@@ -2200,3 +2201,5 @@ int moteopt_selftest_wait_timeout(int mode, double limit_seconds, int* counter, 
 }
 
 }  // extern "C"
+
+#include "loss_api.cuh"   // the losses on logits
