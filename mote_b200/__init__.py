@@ -23,7 +23,8 @@ def __getattr__(name):
     if mod is None:
         raise AttributeError(name)
     import importlib
-    return getattr(importlib.import_module(f"{__name__}.{mod}"), name)
+    value = globals()[name] = getattr(importlib.import_module(f"{__name__}.{mod}"), name)   # found directly from now on
+    return value
 
 
 __all__ = sorted(_LAZY)

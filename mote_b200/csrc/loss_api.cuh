@@ -7,7 +7,10 @@ namespace {
 using namespace moteopt::loss;
 
 // Rows of up to this many bytes take the warp-per-rows kernels, longer ones a block each.
-constexpr int64_t kShortBytes = kTileBytes - 16;
+constexpr int64_t kShortBytes = kTileBytes - 32;
+
+constexpr int64_t kSliceBytes = 72 * 1024, kSliceMost = 220 * 1024, kSliceLeast = 8 * 1024;
+constexpr int64_t kRowMost = kMaxCluster * (kSliceMost - 64);   // bytes of the longest row
 
 int64_t esize(int dtype) { return dtype == MOTEOPT_DTYPE_BF16 ? 2 : 4; }
 
@@ -21,7 +24,8 @@ int check_logits(const char* who, const moteopt_logits* z, const moteopt_positio
   if (z->dtype != MOTEOPT_DTYPE_F32 && z->dtype != MOTEOPT_DTYPE_BF16)
     return fail(MOTEOPT_ERR_INVALID, w + ": logits must be fp32 or bf16");
   if (z->seqs < 0 || z->tokens < 0 || z->vocab < 1) return fail(MOTEOPT_ERR_INVALID, w + ": bad logits shape");
-  if (z->vocab >= (int64_t{1} << 31)) return fail(MOTEOPT_ERR_LIMIT, w + ": a vocabulary of 2^31 or more");
+  if (z->vocab > kRowMost / esize(z->dtype))
+    return fail(MOTEOPT_ERR_LIMIT, w + ": a row of logits may take " + std::to_string(kRowMost) + " bytes");
   if (!positions_fit(z)) return fail(MOTEOPT_ERR_LIMIT, w + ": 2^27 positions or more");
   if (!(temperature > 0.0) || !std::isfinite(temperature) || !std::isfinite(1.0 / temperature))
     return fail(MOTEOPT_ERR_INVALID, w + ": the temperature must be positive and finite");
@@ -39,6 +43,7 @@ int check_logits(const char* who, const moteopt_logits* z, const moteopt_positio
   R->n = static_cast<uint32_t>(n);
   R->tokens = static_cast<uint32_t>(z->tokens);
   R->vocab = static_cast<uint32_t>(z->vocab);
+  R->t = temperature;
   R->inv_t = 1.0 / temperature;
   const double c = kLog2e * R->inv_t;
   float hi = static_cast<float>(c);
@@ -54,11 +59,12 @@ Per per_of(const moteopt_positions& p) { return Per{static_cast<const float*>(p.
 // A launch behind another one of the same call: its blocks may be placed before that one has ended (they wait for it
 // themselves). The first launch of a call (`first`) is an ordinary one.
 template <typename Args>
-int launch_after(void (*kernel)(Args), const Args& A, unsigned grid, unsigned block, cudaStream_t st, const char* what,
-                 bool first = false) {
+int launch_after(void (*kernel)(Args), const Args& A, unsigned grid, unsigned block, size_t smem, cudaStream_t st,
+                 const char* what, bool first = false) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(grid, 1, 1);
   cfg.blockDim = dim3(block, 1, 1);
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -72,11 +78,12 @@ int launch_after(void (*kernel)(Args), const Args& A, unsigned grid, unsigned bl
 }
 
 template <typename Args>
-int launch_cluster(void (*kernel)(Args), const Args& A, unsigned rows, unsigned cl, unsigned block, cudaStream_t st,
-                   const char* what) {
+int launch_cluster(void (*kernel)(Args), const Args& A, unsigned rows, unsigned cl, unsigned block, size_t smem,
+                   cudaStream_t st, const char* what) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(rows * cl, 1, 1);
   cfg.blockDim = dim3(block, 1, 1);
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -93,38 +100,53 @@ int launch_cluster(void (*kernel)(Args), const Args& A, unsigned rows, unsigned 
 
 bool short_rows(int dtype, int64_t vocab) { return vocab * esize(dtype) <= kShortBytes; }
 
-// The warps' share of short rows: as many rows as fit kTileBytes, at most kTileRows.
-void tile_shape(int dtype, int64_t vocab, int* per_warp, uint32_t* pitch) {
-  *pitch = static_cast<uint32_t>((vocab * esize(dtype) + 16 - esize(dtype) + 15) / 16 * 16);
-  *per_warp = std::max(1, std::min(kTileRows, static_cast<int>(kTileBytes / *pitch)));
+// The warps' share of short rows: as many rows as fit kTileBytes, at most kTileRows, and fewer while that would leave an SM
+// less than 16 warps (a warp takes its rows one after the other).
+void tile_shape(int64_t rows, int dtype, int64_t vocab, int sms, int* per_warp, uint32_t* pitch) {
+  *pitch = static_cast<uint32_t>(((vocab * esize(dtype) + 16 - esize(dtype) + 15) / 16 + 1) * 16);
+  const int64_t most = std::min<int64_t>(kTileRows, kTileBytes / *pitch);
+  *per_warp = static_cast<int>(std::max<int64_t>(1, std::min(most, rows / (16 * sms))));
 }
 
-template <typename T, bool kPolicy>
-int launch_tile_t(const TileArgs& A, cudaStream_t st) {
-  const int64_t tiles = cdiv(A.R.n, A.per_warp);
+// Lanes per row: 8, and the whole warp where a row has more than 16 lines for each of them.
+constexpr uint32_t kNarrowPitch = 8 * 16 * 16;
+template <Mode kMode>
+int launch_tile(int dtype, TileArgs A, int sms, cudaStream_t st, bool after = false) {
+  tile_shape(A.R.n, dtype, A.R.vocab, sms, &A.per_warp, &A.pitch);
+  const bool bf = dtype == MOTEOPT_DTYPE_BF16, narrow = A.pitch <= kNarrowPitch;
+  auto* const k = narrow ? (bf ? tile_kernel<__nv_bfloat16, 8, kMode> : tile_kernel<float, 8, kMode>)
+                         : (bf ? tile_kernel<__nv_bfloat16, 32, kMode> : tile_kernel<float, 32, kMode>);
   const size_t smem = static_cast<size_t>(kTileWarps) * A.per_warp * A.pitch;
-  tile_kernel<T, kPolicy><<<static_cast<unsigned>(cdiv(tiles, kTileWarps)), kTileWarps * 32, smem, st>>>(A);
-  MO_LAUNCHED("loss tile_kernel");
-  return MOTEOPT_OK;
-}
-int launch_tile(int dtype, const TileArgs& A, bool policy, cudaStream_t st) {
-  if (dtype == MOTEOPT_DTYPE_BF16)
-    return policy ? launch_tile_t<__nv_bfloat16, true>(A, st) : launch_tile_t<__nv_bfloat16, false>(A, st);
-  return policy ? launch_tile_t<float, true>(A, st) : launch_tile_t<float, false>(A, st);
+  const int64_t blocks = cdiv(cdiv(A.R.n, A.per_warp), kTileWarps);
+  return launch_after(k, A, static_cast<unsigned>(blocks), kTileWarps * 32, smem, st, "loss tile_kernel", !after);
 }
 
-// Blocks per row of the long forward pass: enough for two blocks on every SM, each with at least 1024 vectors.
-int row_cluster(const Rows& R, int dtype, int sms) {
-  const int64_t vecs = R.vocab * esize(dtype) / 16;
-  int cl = 1;
-  while (cl < kMaxCluster && static_cast<int64_t>(R.n) * cl * 2 <= 2 * sms && vecs / (cl * 2) >= 1024) cl *= 2;
-  return cl;
+// Long rows: blocks per row and bytes of shared memory each. A slice of up to kSliceBytes leaves three blocks an SM; a
+// row that 16 such slices do not hold takes larger ones, one block an SM. Where there are too few rows for the
+// GPU they are cut further, down to kSliceLeast.
+struct SliceShape {
+  int threads, cl;
+  size_t smem;
+};
+SliceShape slice_shape(int64_t rows, int64_t vocab, int dtype, int sms) {
+  const int64_t bytes = vocab * esize(dtype);
+  SliceShape s = {256, 1, 0};
+  const auto smem = [&](int cl) { return (cdiv(bytes / 16, cl) + 4) * 16; };   // 3 lines beside the share, 1 to read over
+  while (s.cl < kMaxCluster && smem(s.cl) > kSliceBytes) s.cl *= 2;
+  while (s.cl < kMaxCluster && rows * s.cl * 2 <= 2 * sms && smem(s.cl * 2) >= kSliceLeast) s.cl *= 2;
+  s.smem = static_cast<size_t>(smem(s.cl));
+  if (s.smem <= kSliceBytes / 4) s.threads = 128;
+  return s;
 }
-int launch_rows(int dtype, RowArgs A, int sms, cudaStream_t st) {
-  A.cl = row_cluster(A.R, dtype, sms);
-  return dtype == MOTEOPT_DTYPE_BF16
-             ? launch_cluster(row_kernel<__nv_bfloat16>, A, A.R.n, A.cl, kRowThreads, st, "loss row_kernel")
-             : launch_cluster(row_kernel<float>, A, A.R.n, A.cl, kRowThreads, st, "loss row_kernel");
+
+template <bool kPolicy>
+int launch_slices(int dtype, SliceArgs A, int sms, cudaStream_t st) {
+  const SliceShape s = slice_shape(A.R.n, A.R.vocab, dtype, sms);
+  const bool bf = dtype == MOTEOPT_DTYPE_BF16;
+  A.cl = s.cl;
+  auto* const k = s.threads == 128 ? (bf ? slice_kernel<__nv_bfloat16, 128, kPolicy> : slice_kernel<float, 128, kPolicy>)
+                                   : (bf ? slice_kernel<__nv_bfloat16, 256, kPolicy> : slice_kernel<float, 256, kPolicy>);
+  return launch_cluster(k, A, A.R.n, s.cl, s.threads, s.smem, st, "loss slice_kernel");
 }
 
 // logp, lse (or logp64, coef = 0) of every row
@@ -137,72 +159,52 @@ int launch_forward(int dtype, const Rows& R, float* logp, float* lse, double* lo
     A.lse = lse;
     A.logp64 = logp64;
     A.coef = coef;
-    tile_shape(dtype, R.vocab, &A.per_warp, &A.pitch);
-    return launch_tile(dtype, A, false, st);
+    return launch_tile<kForward>(dtype, A, sms, st);
   }
-  RowArgs A;
+  SliceArgs A;
   std::memset(&A, 0, sizeof(A));
   A.R = R;
   A.logp = logp;
   A.lse = lse;
   A.logp64 = logp64;
   A.coef = coef;
-  return launch_rows(dtype, A, sms, st);
+  return launch_slices<false>(dtype, A, sms, st);
 }
 
-int launch_gradient(int dtype, GradArgs A, cudaStream_t st, bool first = false) {
-  const int64_t vecs = A.R.vocab * esize(dtype) / 16;
-  if (vecs < 128) {
-    const unsigned grid = static_cast<unsigned>(cdiv(A.R.n, kGradThreads / 32));
-    return dtype == MOTEOPT_DTYPE_BF16
-               ? launch_after(grad_short_kernel<__nv_bfloat16>, A, grid, kGradThreads, st, "loss grad_short_kernel", first)
-               : launch_after(grad_short_kernel<float>, A, grid, kGradThreads, st, "loss grad_short_kernel", first);
+int launch_gradient(int dtype, const Rows& R, const Kept& K, void* grad, int sms, cudaStream_t st, bool after) {
+  if (short_rows(dtype, R.vocab)) {
+    TileArgs A;
+    std::memset(&A, 0, sizeof(A));
+    A.R = R;
+    A.K = K;
+    A.grad = grad;
+    return launch_tile<kGradient>(dtype, A, sms, st, after);
   }
-  A.pieces = static_cast<uint32_t>(cdiv(vecs, kGradThreads * kGradVecs));
-  if (static_cast<int64_t>(A.R.n) * A.pieces >= (int64_t{1} << 31))
+  GradArgs A;
+  std::memset(&A, 0, sizeof(A));
+  A.R = R;
+  A.K = K;
+  A.grad = grad;
+  A.pieces = static_cast<uint32_t>(cdiv(R.vocab * esize(dtype) / 16, kGradThreads * kGradVecs));
+  if (static_cast<int64_t>(R.n) * A.pieces >= (int64_t{1} << 31))
     return fail(MOTEOPT_ERR_LIMIT, "loss gradient: too many logits for one call");
-  const unsigned grid = A.R.n * A.pieces;
+  const unsigned grid = R.n * A.pieces;
   return dtype == MOTEOPT_DTYPE_BF16
-             ? launch_after(grad_kernel<__nv_bfloat16>, A, grid, kGradThreads, st, "loss grad_kernel", first)
-             : launch_after(grad_kernel<float>, A, grid, kGradThreads, st, "loss grad_kernel", first);
-}
-
-// The held policy kernel's shape: threads and blocks per row that hold a row's vectors at 32 logits a thread; 0 where 16
-// blocks of 512 threads do not.
-struct HeldShape {
-  int threads, cl;
-};
-HeldShape held_shape(int dtype, int64_t vocab) {
-  const int64_t per = 32 * esize(dtype) / 16;   // vectors a thread
-  const int64_t vecs = vocab * esize(dtype) / 16;
-  if (vecs <= 256 * per) return {256, 1};
-  for (int cl = 1; cl <= kMaxCluster; cl *= 2)
-    if (cdiv(vecs, cl) <= 512 * per) return {512, cl};
-  return {0, 0};
+             ? launch_after(grad_kernel<__nv_bfloat16>, A, grid, kGradThreads, 0, st, "loss grad_kernel", !after)
+             : launch_after(grad_kernel<float>, A, grid, kGradThreads, 0, st, "loss grad_kernel", !after);
 }
 
 constexpr int kSumShare = 4096;   // partials one block adds up
 constexpr int kSumBlocks = 128;
 
 struct PolicyLayout {
-  size_t partials, sums, logp64, lse, coef, bytes;
-  bool short_, held;
+  size_t partials, sums, bytes;
 };
-PolicyLayout policy_layout(int dtype, int64_t n, int64_t vocab) {
+PolicyLayout policy_layout(int64_t n) {
   PolicyLayout L;
-  L.short_ = short_rows(dtype, vocab);
-  L.held = !L.short_ && held_shape(dtype, vocab).cl > 0;
-  int per = 1;
-  uint32_t pitch = 0;
-  if (L.short_) tile_shape(dtype, vocab, &per, &pitch);
   L.partials = kHeaderBytes;
-  const int64_t parts = L.short_ ? cdiv(n, per) : n;
-  L.sums = align_up(L.partials + 32 * static_cast<size_t>(parts), 256);
-  L.logp64 = L.sums + 32 * kSumBlocks;
-  const bool kept = !L.short_ && !L.held;
-  L.lse = align_up(L.logp64 + (kept ? 8 * static_cast<size_t>(n) : 0), 256);
-  L.coef = align_up(L.lse + (kept ? 4 * static_cast<size_t>(n) : 0), 256);
-  L.bytes = align_up(L.coef + (kept ? 4 * static_cast<size_t>(n) : 0), 256);
+  L.sums = align_up(L.partials + 32 * static_cast<size_t>(n), 256);   // at most one row of partials a position
+  L.bytes = L.sums + 32 * kSumBlocks;
   return L;
 }
 
@@ -210,11 +212,11 @@ int launch_sums(const double* partials, int64_t n, double* mid, float* out, cuda
   SumArgs A = {partials, static_cast<uint32_t>(n), mid, out};
   if (n > kSumShare) {
     const unsigned blocks = static_cast<unsigned>(std::min<int64_t>(kSumBlocks, cdiv(n, kSumShare / 4)));
-    MO_TRY(launch_after(sum_kernel, A, blocks, kSumThreads, st, "loss sum_kernel"));
+    MO_TRY(launch_after(sum_kernel, A, blocks, kSumThreads, 0, st, "loss sum_kernel"));
     A.partials = mid;
     A.n = blocks;
   }
-  return launch_after(sum_kernel, A, 1, kSumThreads, st, "loss sum_kernel");
+  return launch_after(sum_kernel, A, 1, kSumThreads, 0, st, "loss sum_kernel");
 }
 
 struct PreferenceLayout {
@@ -236,18 +238,26 @@ int check_divisor(const char* who, double divisor, const float* divisor_device) 
   return MOTEOPT_OK;
 }
 
-// the clusters of 16 blocks that the longest rows take are beyond the portable size
+// the slices' shared memory and their clusters of 16 blocks are beyond the default limits
 int loss_setup(int* sms) {
   MO_TRY(device_setup(sms));
   static std::atomic<unsigned long long> ready{0};   // a bit per device
   int dev = 0;
   MO_CUDA(cudaGetDevice(&dev));
   if (ready.load(std::memory_order_acquire) >> dev & 1) return MOTEOPT_OK;
-  const void* wide[] = {reinterpret_cast<const void*>(row_kernel<__nv_bfloat16>),
-                        reinterpret_cast<const void*>(row_kernel<float>),
-                        reinterpret_cast<const void*>(held_kernel<__nv_bfloat16, 512>),
-                        reinterpret_cast<const void*>(held_kernel<float, 512>)};
-  for (const void* k : wide) MO_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+  const void* const kernels[] = {
+      reinterpret_cast<const void*>(slice_kernel<__nv_bfloat16, 128, false>),
+      reinterpret_cast<const void*>(slice_kernel<__nv_bfloat16, 128, true>),
+      reinterpret_cast<const void*>(slice_kernel<__nv_bfloat16, 256, false>),
+      reinterpret_cast<const void*>(slice_kernel<__nv_bfloat16, 256, true>),
+      reinterpret_cast<const void*>(slice_kernel<float, 128, false>),
+      reinterpret_cast<const void*>(slice_kernel<float, 128, true>),
+      reinterpret_cast<const void*>(slice_kernel<float, 256, false>),
+      reinterpret_cast<const void*>(slice_kernel<float, 256, true>)};
+  for (const void* k : kernels) {
+    MO_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    MO_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kSliceMost)));
+  }
   ready.fetch_or(1ull << dev, std::memory_order_release);
   return MOTEOPT_OK;
 }
@@ -270,26 +280,26 @@ int moteopt_token_logprobs(const moteopt_logits* logits, const moteopt_positions
 int moteopt_token_logprobs_backward(const moteopt_logits* logits, const moteopt_positions* targets, double temperature,
                                     const moteopt_positions* logprobs, const moteopt_positions* lse,
                                     const moteopt_positions* grad_logprobs, void* grad_logits, moteopt_stream_t stream) {
-  GradArgs A;
-  std::memset(&A, 0, sizeof(A));
-  MO_TRY(check_logits("moteopt_token_logprobs_backward", logits, targets, &A.R, temperature));
-  if (A.R.n == 0) return MOTEOPT_OK;
+  Rows R;
+  MO_TRY(check_logits("moteopt_token_logprobs_backward", logits, targets, &R, temperature));
+  if (R.n == 0) return MOTEOPT_OK;
   if (!logprobs || !lse || !grad_logprobs || !logprobs->data || !lse->data || !grad_logprobs->data || !grad_logits)
     return fail(MOTEOPT_ERR_INVALID, "moteopt_token_logprobs_backward: null pointer");
   int sms = 0;
   MO_TRY(loss_setup(&sms));
-  A.logp = per_of(*logprobs);
-  A.lse = per_of(*lse);
-  A.coef = per_of(*grad_logprobs);
-  A.grad = grad_logits;
-  return launch_gradient(logits->dtype, A, reinterpret_cast<cudaStream_t>(stream), true);
+  Kept K;
+  std::memset(&K, 0, sizeof(K));
+  K.logp = per_of(*logprobs);
+  K.lse = per_of(*lse);
+  K.coef = per_of(*grad_logprobs);
+  return launch_gradient(logits->dtype, R, K, grad_logits, sms, reinterpret_cast<cudaStream_t>(stream), false);
 }
 
 size_t moteopt_policy_loss_workspace_size(const moteopt_logits* logits) {
   if (!logits || logits->seqs < 0 || logits->tokens < 0 || logits->vocab < 1 ||
       (logits->dtype != MOTEOPT_DTYPE_F32 && logits->dtype != MOTEOPT_DTYPE_BF16) || !positions_fit(logits))
     return 0;
-  return policy_layout(logits->dtype, logits->seqs * logits->tokens, logits->vocab).bytes;
+  return policy_layout(logits->seqs * logits->tokens).bytes;
 }
 
 int moteopt_policy_loss(const moteopt_logits* logits, const moteopt_positions* targets, const moteopt_policy* policy,
@@ -306,7 +316,7 @@ int moteopt_policy_loss(const moteopt_logits* logits, const moteopt_positions* t
     return fail(MOTEOPT_ERR_INVALID, "moteopt_policy_loss: null pointer");
   if (policy->kl_coef != 0.0 && R.n > 0 && !policy->ref_logprobs.data)
     return fail(MOTEOPT_ERR_INVALID, "moteopt_policy_loss: a KL coefficient without reference log-probabilities");
-  const PolicyLayout L = policy_layout(logits->dtype, R.n, R.vocab);
+  const PolicyLayout L = policy_layout(R.n);
   MO_TRY(check_ws(workspace, workspace_bytes, L.bytes));
   int sms = 0;
   MO_TRY(loss_setup(&sms));
@@ -329,7 +339,7 @@ int moteopt_policy_loss(const moteopt_logits* logits, const moteopt_positions* t
   P.div = policy->divisor_device;
   double* const partials = reinterpret_cast<double*>(ws + L.partials);
   double* const mid = reinterpret_cast<double*>(ws + L.sums);
-  if (L.short_) {
+  if (short_rows(logits->dtype, R.vocab)) {
     TileArgs A;
     std::memset(&A, 0, sizeof(A));
     A.R = R;
@@ -337,50 +347,19 @@ int moteopt_policy_loss(const moteopt_logits* logits, const moteopt_positions* t
     A.logp = logprobs;
     A.grad = grad_logits;
     A.partials = partials;
-    tile_shape(logits->dtype, R.vocab, &A.per_warp, &A.pitch);
-    MO_TRY(launch_tile(logits->dtype, A, true, st));
+    MO_TRY(launch_tile<kPolicyLoss>(logits->dtype, A, sms, st));
+    tile_shape(R.n, logits->dtype, R.vocab, sms, &A.per_warp, &A.pitch);
     return launch_sums(partials, cdiv(R.n, A.per_warp), mid, sums, st);
   }
-  if (L.held) {
-    HeldArgs A;
-    std::memset(&A, 0, sizeof(A));
-    A.R = R;
-    A.P = P;
-    A.logp = logprobs;
-    A.grad = grad_logits;
-    A.partials = partials;
-    const HeldShape s = held_shape(logits->dtype, R.vocab);
-    A.cl = s.cl;
-    const bool bf = logits->dtype == MOTEOPT_DTYPE_BF16;
-    auto* const k = s.threads == 256 ? (bf ? held_kernel<__nv_bfloat16, 256> : held_kernel<float, 256>)
-                                     : (bf ? held_kernel<__nv_bfloat16, 512> : held_kernel<float, 512>);
-    MO_TRY(launch_cluster(k, A, R.n, s.cl, s.threads, st, "loss held_kernel"));
-    return launch_sums(partials, R.n, mid, sums, st);
-  }
-  double* const logp64 = reinterpret_cast<double*>(ws + L.logp64);
-  float* const lse = reinterpret_cast<float*>(ws + L.lse);
-  float* const coef = reinterpret_cast<float*>(ws + L.coef);
-  MO_TRY(launch_forward(logits->dtype, R, nullptr, lse, logp64, coef, sms, st));
-  PolicyRowsArgs B;
-  std::memset(&B, 0, sizeof(B));
-  B.R = R;
-  B.P = P;
-  B.logp64 = logp64;
-  B.logp = logprobs;
-  B.coef = coef;
-  B.partials = partials;
-  const unsigned blocks = static_cast<unsigned>(cdiv(R.n, 256));
-  MO_TRY(launch_after(policy_rows_kernel, B, blocks, 256, st, "loss policy_rows_kernel"));
-  MO_TRY(launch_sums(partials, blocks, mid, sums, st));
-  if (!grad_logits) return MOTEOPT_OK;
-  GradArgs G;
-  std::memset(&G, 0, sizeof(G));
-  G.R = R;
-  G.logp64 = logp64;
-  G.lse_row = lse;
-  G.coef_row = coef;
-  G.grad = grad_logits;
-  return launch_gradient(logits->dtype, G, st);
+  SliceArgs A;
+  std::memset(&A, 0, sizeof(A));
+  A.R = R;
+  A.P = P;
+  A.logp = logprobs;
+  A.grad = grad_logits;
+  A.partials = partials;
+  MO_TRY(launch_slices<true>(logits->dtype, A, sms, st));
+  return launch_sums(partials, R.n, mid, sums, st);
 }
 
 size_t moteopt_preference_loss_workspace_size(const moteopt_logits* logits, int64_t sequences) {
@@ -439,19 +418,17 @@ int moteopt_preference_loss(const moteopt_logits* logits, const moteopt_position
   A.pair_loss = pair_loss;
   A.rewards = rewards;
   A.seq_logp = logprobs;
-  MO_TRY(launch_after(pair_kernel, A, static_cast<unsigned>(A.pairs), kPairThreads, st, "loss pair_kernel", R.n == 0));
-  GradArgs G;
-  std::memset(&G, 0, sizeof(G));
-  G.R = R;
-  G.logp64 = logp64;
-  G.lse_row = lse;
-  G.coef_row = coef;
-  G.grad = grad_logits;
-  G.pair_loss = pair_loss;
-  G.pairs = A.pairs;
-  G.loss = loss;
-  if (!grad_logits || R.n == 0) return launch_after(pair_sum_kernel, G, 1, 32, st, "loss pair_sum_kernel");
-  return launch_gradient(logits->dtype, G, st);
+  MO_TRY(launch_after(pair_kernel, A, static_cast<unsigned>(A.pairs), kPairThreads, 0, st, "loss pair_kernel", R.n == 0));
+  Kept K;
+  std::memset(&K, 0, sizeof(K));
+  K.logp64 = logp64;
+  K.lse_row = lse;
+  K.coef_row = coef;
+  K.pair_loss = pair_loss;
+  K.pairs = A.pairs;
+  K.loss = loss;
+  if (!grad_logits || R.n == 0) return launch_after(pair_sum_kernel, K, 1, 32, 0, st, "loss pair_sum_kernel");
+  return launch_gradient(logits->dtype, R, K, grad_logits, sms, st, true);
 }
 
 }  // extern "C"

@@ -45,7 +45,7 @@ struct Rows {
   const int32_t* cu;      // packed: n_seqs + 1 row offsets, or null. Rows outside [cu[0], cu[n_seqs]) do not count
   int n_seqs;
   float c_hi, c_lo;       // log2(e) / T as two floats, c_lo > 0 (see ex2_of)
-  double inv_t;
+  double t, inv_t;        // T and 1 / T
 };
 
 struct Per {              // fp32 values per position, broadcast where a stride is 0
@@ -95,12 +95,11 @@ __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
 struct Ex {               // the constants of one row's exponentials, two at a time
   uint64_t neg_m, hi, lo;
   __device__ Ex(float m, float c_hi, float c_lo) : neg_m(pack2(-m, -m)), hi(pack2(c_hi, c_hi)), lo(pack2(c_lo, c_lo)) {}
-  __device__ __forceinline__ void two(float z0, float z1, float& e0, float& e1) const {
-    const uint64_t d = add2(pack2(z0, z1), neg_m);
+  __device__ __forceinline__ uint64_t two(uint64_t z) const {
+    const uint64_t d = add2(z, neg_m);
     float t0, t1;
     unpack2(fma2(d, hi, mul2(d, lo)), t0, t1);
-    e0 = ex2(t0);
-    e1 = ex2(t1);
+    return pack2(ex2(t0), ex2(t1));
   }
 };
 __device__ __forceinline__ float ex_one(float z, float m, float c_hi, float c_lo) {
@@ -174,6 +173,38 @@ __device__ __forceinline__ double warp_sum(double v) {
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void pdl_go() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
+// A line's 16 bytes as pairs of fp32: 4 of bf16, 2 of fp32
+template <typename T>
+struct Pairs;
+template <>
+struct Pairs<__nv_bfloat16> {
+  static constexpr int kN = 4;
+  uint64_t p[4];
+  __device__ __forceinline__ explicit Pairs(const uint4& v)
+      : p{pack2(lo_bf16(v.x), hi_bf16(v.x)), pack2(lo_bf16(v.y), hi_bf16(v.y)), pack2(lo_bf16(v.z), hi_bf16(v.z)),
+          pack2(lo_bf16(v.w), hi_bf16(v.w))} {}
+  __device__ __forceinline__ uint4 line() const {   // rounded once
+    float a[8];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) unpack2(p[u], a[2 * u], a[2 * u + 1]);
+    return make_uint4(to_bf16x2(a[0], a[1]), to_bf16x2(a[2], a[3]), to_bf16x2(a[4], a[5]), to_bf16x2(a[6], a[7]));
+  }
+};
+template <>
+struct Pairs<float> {
+  static constexpr int kN = 2;
+  uint64_t p[2];
+  __device__ __forceinline__ explicit Pairs(const uint4& v)
+      : p{pack2(bits(v.x), bits(v.y)), pack2(bits(v.z), bits(v.w))} {}
+  static __device__ __forceinline__ float bits(uint32_t w) { return __uint_as_float(w); }
+  __device__ __forceinline__ uint4 line() const {
+    float a[4];
+    unpack2(p[0], a[0], a[1]);
+    unpack2(p[1], a[2], a[3]);
+    return make_uint4(__float_as_uint(a[0]), __float_as_uint(a[1]), __float_as_uint(a[2]), __float_as_uint(a[3]));
+  }
+};
+
 // (largest logit, sum) of a part of a row
 struct Part {
   float m, s;
@@ -237,203 +268,6 @@ __device__ __forceinline__ bool in_packed(const Rows& R, uint32_t row) {
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
-// Short rows: a warp takes `per_warp` rows. Their 16-byte lines come into shared memory by cp.async (a line may hold up to
-// 15 bytes beside the row: the same aligned line, so nothing beyond the allocation), which lifts every alignment and stride
-// question and keeps all of a warp's rows in flight at once. Then per row the maximum and the sum over the warp's lanes; then
-// one lane per row for the row's values in 64 bits (they would cost a warp more than the whole row if every lane formed them
-// for one row); then, for the gradient, the exponentials again from shared memory.
-constexpr int kTileWarps = 4;
-constexpr int kTileRows = 16;          // most rows of a warp
-constexpr int kTileBytes = 9216;       // most bytes of a warp's rows: 6 blocks of 4 warps in an SM's shared memory
-
-struct TileArgs {
-  Rows R;
-  int per_warp;
-  uint32_t pitch;                      // bytes of a row's lines in shared memory
-  float* logp;                         // [n], or null
-  float* lse;                          // [n], or null
-  double* logp64;                      // [n] with coef [n] (preference), or null
-  float* coef;
-  Policy P;
-  void* grad;                          // [n][vocab], or null
-  double* partials;                    // [warps][4] (policy)
-};
-
-template <typename T, bool kPolicy>
-__global__ void __launch_bounds__(kTileWarps * 32) tile_kernel(const __grid_constant__ TileArgs A) {
-  extern __shared__ __align__(16) unsigned char sm[];
-  using W = Word<T>;
-  const Rows& R = A.R;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t tile = blockIdx.x * kTileWarps + warp;
-  const uint32_t first = tile * static_cast<uint32_t>(A.per_warp);
-  pdl_go();
-  if (first >= R.n) return;
-  const int rows = static_cast<int>(min(static_cast<uint32_t>(A.per_warp), R.n - first));
-  unsigned char* const base = sm + static_cast<size_t>(warp) * A.per_warp * A.pitch;
-
-  // lane r: its row
-  uint32_t seq = 0, tok = 0, y = 0;
-  int64_t y64 = -1;
-  uint64_t addr = 0;
-  float wt = 1.f;
-  if (lane < rows) {
-    const uint32_t row = first + lane;
-    seq = row / R.tokens;
-    tok = row - seq * R.tokens;
-    y64 = in_packed(R, row) ? R.y[seq * R.y_seq + tok * R.y_tok] : -1;
-    addr = reinterpret_cast<uint64_t>(R.z) + (seq * R.z_seq + tok * R.z_tok) * sizeof(T);
-    if (kPolicy && A.P.weight.p) wt = A.P.weight.at(seq, tok);
-  }
-  const bool live = y64 >= 0 && wt != 0.f;
-  const bool has_y = live && y64 < static_cast<int64_t>(R.vocab);
-  if (has_y) y = static_cast<uint32_t>(y64);
-  const unsigned live_rows = __ballot_sync(0xffffffffu, live);
-  for (int r = 0; r < rows; ++r) {
-    if (!(live_rows >> r & 1)) continue;
-    const uint64_t a = __shfl_sync(0xffffffffu, addr, r);
-    const uint32_t lines = (static_cast<uint32_t>(a & 15) + R.vocab * static_cast<uint32_t>(sizeof(T)) + 15) / 16;
-    MO_CHECK(lines * 16 <= A.pitch);
-    const uint32_t dst = smem_u32(base + static_cast<size_t>(r) * A.pitch);
-    for (uint32_t v = lane; v < lines; v += 32)
-      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + v * 16), "l"((a & ~15ull) + v * 16) : "memory");
-  }
-  asm volatile("cp.async.commit_group;" ::: "memory");
-  float adv = 0.f, old_lp = 0.f, ref_lp = 0.f;
-  if (kPolicy && live) {
-    adv = A.P.adv.at(seq, tok);
-    old_lp = A.P.old_lp.at(seq, tok);
-    if (A.P.ref_lp.p) ref_lp = A.P.ref_lp.at(seq, tok);
-  }
-  asm volatile("cp.async.wait_group 0;" ::: "memory");
-  __syncwarp();
-
-  // lane r: takes the target out of its row, and what lies beside the row in its first and last word
-  const uint32_t skew = static_cast<uint32_t>(addr & 15) / sizeof(T);   // elements in front of the row
-  const uint32_t w_begin = skew / W::kPer, w_end = (skew + R.vocab + W::kPer - 1) / W::kPer;
-  uint32_t* const mine = reinterpret_cast<uint32_t*>(base + static_cast<size_t>(lane) * A.pitch);
-  float zy = NAN;
-  if (live) {
-    if (W::kPer == 2) {
-      if (skew & 1) mine[w_begin] = W::drop(mine[w_begin], 0);
-      if ((skew + R.vocab) & 1) mine[w_end - 1] = W::drop(mine[w_end - 1], 1);
-    }
-    if (has_y) {
-      const uint32_t e = skew + y, w = e / W::kPer;
-      zy = W::kPer == 2 ? ((e & 1) ? hi_bf16(mine[w]) : lo_bf16(mine[w])) : __uint_as_float(mine[w]);
-      mine[w] = W::drop(mine[w], e % W::kPer);
-    }
-  }
-  __syncwarp();
-
-  float m_mine = kNegInf, s_mine = 0.f;
-  for (int r = 0; r < rows; ++r) {
-    if (!(live_rows >> r & 1)) continue;
-    const uint32_t b = __shfl_sync(0xffffffffu, w_begin, r), e = __shfl_sync(0xffffffffu, w_end, r);
-    const uint32_t* row = reinterpret_cast<const uint32_t*>(base + static_cast<size_t>(r) * A.pitch);
-    uint32_t top = W::kEmpty;
-#pragma unroll 4
-    for (uint32_t w = b + lane; w < e; w += 32) top = W::max(top, row[w]);
-    const float m = warp_max(W::top(top));
-    const float mm = m == kNegInf ? 0.f : m;
-    const Ex ex(mm, R.c_hi, R.c_lo);
-    float s = 0.f, s2 = 0.f;
-#pragma unroll 4
-    for (uint32_t w = b + lane; w < e; w += 32) {
-      const uint32_t v = row[w];
-      if (W::kPer == 2) {
-        float e0, e1;
-        ex.two(lo_bf16(v), hi_bf16(v), e0, e1);
-        s += e0;
-        s2 += e1;
-      } else {
-        s += ex_one(__uint_as_float(v), mm, R.c_hi, R.c_lo);
-      }
-    }
-    s = warp_sum(s + s2);
-    if (lane == r) {
-      m_mine = m;
-      s_mine = s;
-    }
-  }
-
-  // lane r: the row's values
-  RowStat st = {0.0, 0.0, 0.f, 0.f};
-  double part[4] = {0.0, 0.0, 0.0, 0.0};
-  float g = 0.f;
-  if (live) {
-    st = row_stat(zy, m_mine, s_mine, R.inv_t);
-    if (kPolicy) {
-      const RowLoss L = policy_row_loss(st.logp, A.P, old_lp, ref_lp, A.P.ref_lp.p != nullptr, adv);
-      const double w = wt, inv = A.P.div ? 1.0 / static_cast<double>(*A.P.div) : A.P.inv_div;
-      part[0] = w * L.loss * inv;
-      part[1] = w;
-      part[2] = w * L.kl * inv;
-      part[3] = L.clipped ? w : 0.0;
-      g = static_cast<float>(w * L.slope * inv * R.inv_t);
-    }
-  }
-  if (lane < rows) {
-    const uint32_t row = first + lane;
-    if (A.logp) A.logp[row] = static_cast<float>(st.logp);
-    if (A.lse) A.lse[row] = static_cast<float>(st.lse);
-    if (A.logp64) {
-      A.logp64[row] = st.logp;
-      A.coef[row] = 0.f;
-    }
-  }
-  if (!kPolicy) return;
-#pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    const double v = warp_sum(part[k]);
-    if (lane == k) A.partials[static_cast<size_t>(tile) * 4 + k] = v;
-  }
-  if (A.grad == nullptr) return;
-
-  const float gf = -g * st.f;
-  for (int r = 0; r < rows; ++r) {
-    T* const out = static_cast<T*>(A.grad) + static_cast<size_t>(first + r) * R.vocab;
-    const bool on = live_rows >> r & 1;
-    const uint32_t b = __shfl_sync(0xffffffffu, w_begin, r), e = __shfl_sync(0xffffffffu, w_end, r);
-    const uint32_t sk = __shfl_sync(0xffffffffu, skew, r);
-    const float k = __shfl_sync(0xffffffffu, gf, r);
-    const float m = __shfl_sync(0xffffffffu, m_mine, r);
-    const uint32_t* row = reinterpret_cast<const uint32_t*>(base + static_cast<size_t>(r) * A.pitch);
-    if (!on) {
-      for (uint32_t j = lane; j < R.vocab; j += 32) store_one(out + j, 0.f);
-      continue;
-    }
-    const float mm = m == kNegInf ? 0.f : m;
-    if (W::kPer == 2) {
-      const Ex ex(mm, R.c_hi, R.c_lo);
-      // the output's pairs fall on 4 bytes where its row's alignment has the parity of the input's
-      const bool wide = ((reinterpret_cast<uint64_t>(out) >> 1) & 1) == (sk & 1);
-      T* const o = out - static_cast<int>(sk);
-#pragma unroll 4
-      for (uint32_t w = b + lane; w < e; w += 32) {
-        float e0, e1;
-        const uint32_t v = row[w];
-        ex.two(lo_bf16(v), hi_bf16(v), e0, e1);
-        const uint32_t d = to_bf16x2(e0 * k, e1 * k);
-        const bool in0 = 2 * w >= sk, in1 = 2 * w + 1 < sk + R.vocab;
-        if (wide && in0 && in1) {
-          *reinterpret_cast<uint32_t*>(o + 2 * w) = d;
-        } else {
-          if (in0) *reinterpret_cast<uint16_t*>(o + 2 * w) = static_cast<uint16_t>(d);
-          if (in1) *reinterpret_cast<uint16_t*>(o + 2 * w + 1) = static_cast<uint16_t>(d >> 16);
-        }
-      }
-    } else {
-#pragma unroll 4
-      for (uint32_t w = b + lane; w < e; w += 32)
-        store_one(out + (w - b), ex_one(__uint_as_float(row[w]), mm, R.c_hi, R.c_lo) * k);
-    }
-  }
-  __syncwarp();   // the targets' elements, written as 0 above
-  if (has_y) store_one(static_cast<T*>(A.grad) + static_cast<size_t>(first + lane) * R.vocab + y, g * st.rest);
-}
-
-// ---------------------------------------------------------------------------------------------------------------------
 // A row in vectors of 16 bytes: `head` elements up to the first aligned one, then `vecs` vectors, then `tail` elements
 template <typename T>
 struct Split {
@@ -467,12 +301,40 @@ __device__ __forceinline__ uint32_t vec_max(uint32_t top, const uint4& v) {
   return W::max(W::max(W::max(top, v.x), W::max(v.y, v.z)), v.w);
 }
 
+// `n` elements of a line from `from` stay, the others become -inf
+template <typename T>
+__device__ __forceinline__ void keep(uint4& v, uint32_t from, uint32_t n) {
+#pragma unroll
+  for (uint32_t i = 0; i < 16 / sizeof(T); ++i)
+    if (i < from || i >= from + n) drop_target<T>(v, i);
+}
+// 16 bytes from byte `by` (1 to 15) of two lines (uniform over a row)
+__device__ __forceinline__ uint4 shift_lines(const uint4& a, const uint4& b, uint32_t by) {
+  uint32_t w[5];
+  switch (by >> 2) {
+    case 0: w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w, w[4] = b.x; break;
+    case 1: w[0] = a.y, w[1] = a.z, w[2] = a.w, w[3] = b.x, w[4] = b.y; break;
+    case 2: w[0] = a.z, w[1] = a.w, w[2] = b.x, w[3] = b.y, w[4] = b.z; break;
+    default: w[0] = a.w, w[1] = b.x, w[2] = b.y, w[3] = b.z, w[4] = b.w; break;
+  }
+  const uint32_t sh = (by & 3u) * 8;
+  return make_uint4(__funnelshift_r(w[0], w[1], sh), __funnelshift_r(w[1], w[2], sh), __funnelshift_r(w[2], w[3], sh),
+                    __funnelshift_r(w[3], w[4], sh));
+}
+// 16 bytes of shared memory from any element
+__device__ __forceinline__ uint4 load_shifted(const unsigned char* p, uint32_t off) {
+  const uint4* const l = reinterpret_cast<const uint4*>(p + (off & ~15u));
+  const uint32_t by = off & 15u;
+  return by ? shift_lines(l[0], l[1], by) : l[0];
+}
+
 __device__ __forceinline__ uint32_t cluster_rank() {
   uint32_t r;
   asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
   return r;
 }
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_arrive_relaxed() { asm volatile("barrier.cluster.arrive.relaxed.aligned;"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 __device__ __forceinline__ void store_remote(void* local, uint32_t rank, float a, float b) {   // 8 bytes in rank's copy
   uint32_t dst;
@@ -495,9 +357,13 @@ __device__ __forceinline__ Part row_join(Part p, int cl, uint32_t rank, float in
   b = warp_join(b, inv_t);
   if (cl > 1) {
     cluster_wait();   // every block of the cluster runs (arrived at its start)
-    if (warp == 0 && lane < cl) store_remote(sh_block + rank, lane, b.m, b.s);
-    __syncwarp();
-    cluster_arrive();
+    if (warp == 0) {   // the only writes to be seen by other blocks
+      if (lane < cl) store_remote(sh_block + rank, lane, b.m, b.s);
+      __syncwarp();
+      cluster_arrive();
+    } else {
+      cluster_arrive_relaxed();
+    }
     cluster_wait();
     b = lane < cl ? sh_block[lane] : Part{kNegInf, 0.f};
     b = warp_join(b, inv_t);
@@ -506,132 +372,290 @@ __device__ __forceinline__ Part row_join(Part p, int cl, uint32_t rank, float in
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
-// Long rows, forward only: a row per block (or per cluster of blocks where there are few rows), read once in vectors with a
-// running maximum and sum per thread.
-struct RowArgs {
-  Rows R;
-  int cl;               // blocks per row
-  float* logp;
-  float* lse;
-  double* logp64;
-  float* coef;
+// The gradient from kept row values: d_j = g ([j == y] - exp(x_j - lse)) / T with one coefficient g per row. Rows with g = 0
+// are written as zeros.
+struct Kept {
+  Per logp, lse, coef;       // per position ...
+  const double* logp64;      // ... or by row: the preference loss's own [n] arrays
+  const float* lse_row;
+  const float* coef_row;
+  const double* pair_loss;   // preference: the first block adds up the pairs' losses
+  int pairs;
+  float* loss;
 };
-constexpr int kRowThreads = 256;
-
-template <typename T>
-__global__ void __launch_bounds__(kRowThreads) row_kernel(const __grid_constant__ RowArgs A) {
-  constexpr int kUnroll = 4;
-  using W = Word<T>;
-  __shared__ Part sh_warp[kRowThreads / 32], sh_block[kMaxCluster];
-  const Rows& R = A.R;
-  const uint32_t rank = A.cl > 1 ? cluster_rank() : 0;
-  const uint32_t row = blockIdx.x / A.cl;
-  MO_CHECK(row < R.n && rank < static_cast<uint32_t>(A.cl));
-  pdl_go();
-  const uint32_t seq = row / R.tokens, tok = row - seq * R.tokens;
-  const int64_t y64 = in_packed(R, row) ? R.y[seq * R.y_seq + tok * R.y_tok] : -1;
-  if (y64 < 0) {   // the whole cluster
-    if (rank == 0 && threadIdx.x == 0) {
-      if (A.logp) A.logp[row] = 0.f;
-      if (A.lse) A.lse[row] = 0.f;
-      if (A.logp64) {
-        A.logp64[row] = 0.0;
-        A.coef[row] = 0.f;
-      }
-    }
-    return;
-  }
-  if (A.cl > 1) cluster_arrive();
-  const T* const z = reinterpret_cast<const T*>(R.z) + (seq * R.z_seq + tok * R.z_tok);
-  const bool has_y = y64 < static_cast<int64_t>(R.vocab);
-  const uint32_t y = has_y ? static_cast<uint32_t>(y64) : 0xffffffffu;
-  const Split<T> sp(z, R.vocab);
-  const float zy = has_y ? load_one(z + y) : NAN;
-  const float inv_t = static_cast<float>(R.inv_t);
-  const uint32_t yv = has_y && y >= sp.head ? (y - sp.head) / sp.kPer : 0xffffffffu, ye = (y - sp.head) % sp.kPer;
-  const uint32_t share = (sp.vecs + A.cl - 1) / A.cl, begin = rank * share, end = min(begin + share, sp.vecs);
-  const uint4* const zv = reinterpret_cast<const uint4*>(z + sp.head);
-  Part p = {kNegInf, 0.f};
-  if (rank == 0 && threadIdx.x < sp.head + sp.tail) {
-    const uint32_t j = sp.edge(threadIdx.x);
-    if (j != y) {
-      p.m = load_one(z + j);
-      p.s = p.m == kNegInf ? 0.f : ex_one(p.m, p.m, R.c_hi, R.c_lo);   // 1, or NaN
-    }
-  }
-  for (uint32_t i = begin + threadIdx.x; i < end; i += kRowThreads * kUnroll) {
-    uint4 v[kUnroll];
-#pragma unroll
-    for (int k = 0; k < kUnroll; ++k) {
-      const uint32_t at = i + k * kRowThreads;
-      v[k] = make_uint4(W::kEmpty, W::kEmpty, W::kEmpty, W::kEmpty);
-      if (at < end) v[k] = load_vec(zv + at);
-    }
-    uint32_t top = W::kEmpty;
-#pragma unroll
-    for (int k = 0; k < kUnroll; ++k) {
-      if (i + k * kRowThreads == yv) drop_target<T>(v[k], ye);
-      top = vec_max<T>(top, v[k]);
-    }
-    const float t = W::top(top);
-    if (t > p.m) {
-      p.s *= rescale(p.m, t, inv_t);
-      p.m = t;
-    }
-    const float mm = p.m == kNegInf ? 0.f : p.m;
-    const Ex ex(mm, R.c_hi, R.c_lo);
-    float s0 = 0.f, s1 = 0.f;
-#pragma unroll
-    for (int k = 0; k < kUnroll; ++k) {
-      const uint32_t q[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
-      float e0, e1;
-      if (W::kPer == 2) {
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          ex.two(lo_bf16(q[u]), hi_bf16(q[u]), e0, e1);
-          s0 += e0;
-          s1 += e1;
-        }
-      } else {
-#pragma unroll
-        for (int u = 0; u < 4; u += 2) {
-          ex.two(__uint_as_float(q[u]), __uint_as_float(q[u + 1]), e0, e1);
-          s0 += e0;
-          s1 += e1;
-        }
-      }
-    }
-    p.s += s0 + s1;
-  }
-  p = row_join<kRowThreads>(p, A.cl, rank, inv_t, sh_warp, sh_block);
-  if (rank == 0 && threadIdx.x == 0) {
-    const RowStat st = row_stat(zy, p.m, p.s, R.inv_t);
-    if (A.logp) A.logp[row] = static_cast<float>(st.logp);
-    if (A.lse) A.lse[row] = static_cast<float>(st.lse);
-    if (A.logp64) {
-      A.logp64[row] = st.logp;
-      A.coef[row] = 0.f;
-    }
-  }
+// exp(x_j - lse) = 2^((z_j - m) c) (1 + d) with m = lse T rounded to fp32 and d = m / T - lse, at most 2^-24 lse
+struct KeptRow {
+  float m, f, gy;   // d_j = 2^((z_j - m) c) f, gy at the target
+};
+__device__ __forceinline__ float kept_coef(const Kept& K, uint32_t row, uint32_t seq, uint32_t tok) {
+  return K.coef_row ? K.coef_row[row] : K.coef.at(seq, tok);
+}
+__device__ __forceinline__ KeptRow kept_row(const Kept& K, const Rows& R, uint32_t row, uint32_t seq, uint32_t tok, float coef) {
+  const double lse = K.lse_row ? K.lse_row[row] : K.lse.at(seq, tok);
+  const float lp = K.logp64 ? static_cast<float>(K.logp64[row]) : K.logp.at(seq, tok);
+  const float g = static_cast<float>(coef * R.inv_t);
+  KeptRow r;
+  r.m = static_cast<float>(lse * R.t);
+  r.f = -g * static_cast<float>(1.0 + (r.m * R.inv_t - lse));
+  r.gy = -expm1f(lp) * g;
+  return r;
+}
+__device__ __forceinline__ void sum_pairs(const Kept& K) {   // one warp, in a fixed order
+  const int lane = threadIdx.x & 31;
+  double v = 0.0;
+  for (int i = lane; i < K.pairs; i += 32) v += K.pair_loss[i];
+  v = warp_sum(v);
+  if (lane == 0) *K.loss = static_cast<float>(v);
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
-// Long rows, the policy loss and its gradient in one pass: a row's exponentials stay in the registers of one block, or of a
-// cluster of blocks (32 a thread), relative to each thread's own maximum; when the row's sum is known each thread scales
-// them by one factor. Each logit is read once, exponentiated once, and its gradient written once.
-struct HeldArgs {
+// Short rows: a warp takes `per_warp` rows. Their 16-byte lines come into shared memory by cp.async (a line may hold up to
+// 15 bytes beside the row: the same aligned line, so nothing beyond the allocation), which lifts every alignment and stride
+// question and keeps all of a warp's rows in flight at once. kG lanes work on a row in lines of 16 bytes, 32 / kG rows at a
+// time: the quarter of a warp that shared memory serves at once reads 128 bytes in a row whatever the rows' pitch, and the
+// maximum and the sum take 3 shuffles for four rows. One lane per row forms the row's values in 64 bits (they would cost a
+// warp more than the whole row if it formed them for one row at a time). Then, for the gradient, the exponentials again from
+// shared memory, by the lines of the output.
+constexpr int kTileWarps = 4;
+constexpr int kTileRows = 16;          // most rows of a warp
+constexpr int kTileBytes = 9216;       // most bytes of a warp's rows: 6 blocks of 4 warps in an SM's shared memory
+enum Mode { kForward, kPolicyLoss, kGradient };
+
+struct TileArgs {
   Rows R;
-  int cl;
-  float* logp;
+  int per_warp;
+  uint32_t pitch;                      // bytes of a row's lines in shared memory, and 16 to read over
+  float* logp;                         // [n], or null
+  float* lse;                          // [n], or null
+  double* logp64;                      // [n] with coef [n] (preference), or null
+  float* coef;
   Policy P;
-  void* grad;
-  double* partials;     // [n][4]
+  void* grad;                          // [n][vocab], or null
+  double* partials;                    // [warps][4] (policy)
+  Kept K;                              // (gradient)
 };
 
-template <typename T, int kThreads>
-__global__ void __launch_bounds__(kThreads) held_kernel(const __grid_constant__ HeldArgs A) {
+template <int kG>
+__device__ __forceinline__ float group_max(float v) {
+  if (kG == 32) return warp_max(v);
+#pragma unroll
+  for (int o = kG / 2; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
+}
+template <int kG>
+__device__ __forceinline__ float group_sum(float v) {
+#pragma unroll
+  for (int o = kG / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+template <typename T, int kG, Mode kMode>
+__global__ void __launch_bounds__(kTileWarps * 32) tile_kernel(const __grid_constant__ TileArgs A) {
+  extern __shared__ __align__(16) unsigned char sm[];
   using W = Word<T>;
-  constexpr int kPer = 16 / sizeof(T), kVecs = 32 / kPer;
+  constexpr uint32_t kPer = 16 / sizeof(T);
+  constexpr int kAtOnce = 32 / kG;
+  const Rows& R = A.R;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gl = lane % kG, group = lane / kG;
+  const uint32_t tile = blockIdx.x * kTileWarps + warp;
+  const uint32_t first = tile * static_cast<uint32_t>(A.per_warp);
+  if (kMode != kGradient) pdl_go();
+  if (first >= R.n) return;
+  const int rows = static_cast<int>(min(static_cast<uint32_t>(A.per_warp), R.n - first));
+  unsigned char* const base = sm + static_cast<size_t>(warp) * A.per_warp * A.pitch;
+
+  // lane r: its row
+  uint32_t seq = 0, tok = 0, y = 0;
+  int64_t y64 = -1;
+  uint64_t addr = 0;
+  float wt = 1.f;
+  if (lane < rows) {
+    const uint32_t row = first + lane;
+    seq = row / R.tokens;
+    tok = row - seq * R.tokens;
+    y64 = in_packed(R, row) ? R.y[seq * R.y_seq + tok * R.y_tok] : -1;
+    addr = reinterpret_cast<uint64_t>(R.z) + (seq * R.z_seq + tok * R.z_tok) * sizeof(T);
+    if (kMode == kPolicyLoss && A.P.weight.p) wt = A.P.weight.at(seq, tok);
+  }
+  bool live = y64 >= 0 && wt != 0.f;
+  const bool has_y = live && y64 < static_cast<int64_t>(R.vocab);
+  if (has_y) y = static_cast<uint32_t>(y64);
+  const uint32_t skew = static_cast<uint32_t>(addr & 15) / sizeof(T);   // elements in front of the row in its first line
+  const uint32_t lines = (skew + R.vocab + kPer - 1) / kPer;
+  unsigned live_rows = __ballot_sync(0xffffffffu, live);
+  for (int r = 0; r < rows; ++r) {
+    const uint64_t a = __shfl_sync(0xffffffffu, addr, r) & ~15ull;
+    const uint32_t nl = __shfl_sync(0xffffffffu, lines, r);
+    if (!(live_rows >> r & 1)) continue;
+    MO_CHECK((nl + 1) * 16 <= A.pitch);
+    const uint32_t dst = smem_u32(base + static_cast<size_t>(r) * A.pitch);
+    for (uint32_t v = lane; v < nl; v += 32)
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + v * 16), "l"(a + v * 16) : "memory");
+  }
+  asm volatile("cp.async.commit_group;" ::: "memory");
+  float adv = 0.f, old_lp = 0.f, ref_lp = 0.f;
+  if (kMode == kPolicyLoss && live) {
+    adv = A.P.adv.at(seq, tok);
+    old_lp = A.P.old_lp.at(seq, tok);
+    if (A.P.ref_lp.p) ref_lp = A.P.ref_lp.at(seq, tok);
+  }
+  // lane r: the row's values; d_j = 2^((z_j - m) c) f, gy at the target
+  float m_mine = kNegInf, s_mine = 0.f, f = 0.f, gy = 0.f;
+  if (kMode == kGradient) {
+    pdl_wait();   // the rows are inputs; their coefficients may come from the launch before
+    if (A.K.pair_loss && tile == 0) sum_pairs(A.K);
+    float coef = 0.f;
+    if (live) coef = kept_coef(A.K, first + lane, seq, tok);
+    live = live && coef != 0.f;
+    live_rows = __ballot_sync(0xffffffffu, live);
+    if (live) {
+      const KeptRow k = kept_row(A.K, R, first + lane, seq, tok, coef);
+      m_mine = k.m;
+      f = k.f;
+      gy = k.gy;
+    }
+  }
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+  __syncwarp();
+
+  // lane r: takes the target out of its row, and what lies beside the row in its first and last line
+  uint4* const mine = reinterpret_cast<uint4*>(base + static_cast<size_t>(lane) * A.pitch);
+  float zy = NAN;
+  if (live) {
+    if (has_y) {
+      const uint32_t at = skew + y;
+      zy = load_one(reinterpret_cast<const T*>(mine) + at);
+      reinterpret_cast<T*>(mine)[at] = static_cast<T>(kNegInf);
+    }
+    if (kMode != kGradient) {
+      if (skew != 0) keep<T>(mine[0], skew, kPer);
+      keep<T>(mine[lines - 1], 0, skew + R.vocab - (lines - 1) * kPer);
+    }
+  }
+  __syncwarp();
+
+  if (kMode != kGradient) {
+    for (int r0 = 0; r0 < rows; r0 += kAtOnce) {
+      const int r = r0 + group;
+      uint32_t nl = __shfl_sync(0xffffffffu, lines, r & 31);
+      if (r >= rows || !(live_rows >> r & 1)) nl = 0;
+      const uint4* const row = reinterpret_cast<const uint4*>(base + static_cast<size_t>(r) * A.pitch);
+      uint32_t top = W::kEmpty;
+#pragma unroll 4
+      for (uint32_t l = gl; l < nl; l += kG) top = vec_max<T>(top, row[l]);
+      const float m = group_max<kG>(W::top(top));
+      const Ex ex(m == kNegInf ? 0.f : m, R.c_hi, R.c_lo);
+      uint64_t acc = 0;
+#pragma unroll 4
+      for (uint32_t l = gl; l < nl; l += kG) {
+        const Pairs<T> q(row[l]);
+#pragma unroll
+        for (int u = 0; u < Pairs<T>::kN; ++u) acc = add2(acc, ex.two(q.p[u]));
+      }
+      float s0, s1;
+      unpack2(acc, s0, s1);
+      const float s = group_sum<kG>(s0 + s1);
+      const int from = ((lane - r0) & (kAtOnce - 1)) * kG;
+      const float mr = __shfl_sync(0xffffffffu, m, from), sr = __shfl_sync(0xffffffffu, s, from);
+      if (lane >= r0 && lane < r0 + kAtOnce) {
+        m_mine = mr;
+        s_mine = sr;
+      }
+    }
+    RowStat st = {0.0, 0.0, 0.f, 0.f};
+    double part[4] = {0.0, 0.0, 0.0, 0.0};
+    if (live) {
+      st = row_stat(zy, m_mine, s_mine, R.inv_t);
+      if (kMode == kPolicyLoss) {
+        const RowLoss L = policy_row_loss(st.logp, A.P, old_lp, ref_lp, A.P.ref_lp.p != nullptr, adv);
+        const double w = wt, inv = A.P.div ? 1.0 / static_cast<double>(*A.P.div) : A.P.inv_div;
+        part[0] = w * L.loss * inv;
+        part[1] = w;
+        part[2] = w * L.kl * inv;
+        part[3] = L.clipped ? w : 0.0;
+        const float g = static_cast<float>(w * L.slope * inv * R.inv_t);
+        f = -g * st.f;
+        gy = g * st.rest;
+      }
+    }
+    if (lane < rows) {
+      const uint32_t row = first + lane;
+      if (A.logp) A.logp[row] = static_cast<float>(st.logp);
+      if (A.lse) A.lse[row] = static_cast<float>(st.lse);
+      if (A.logp64) {
+        A.logp64[row] = st.logp;
+        A.coef[row] = 0.f;
+      }
+    }
+    if (kMode == kForward) return;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const double v = warp_sum(part[k]);
+      if (lane == k) A.partials[static_cast<size_t>(tile) * 4 + k] = v;
+    }
+    if (A.grad == nullptr) return;
+    if (m_mine == kNegInf) m_mine = 0.f;
+  }
+
+  for (int r0 = 0; r0 < rows; r0 += kAtOnce) {
+    const int r = r0 + group;
+    const float m = __shfl_sync(0xffffffffu, m_mine, r & 31), k = __shfl_sync(0xffffffffu, f, r & 31);
+    const uint32_t sk = __shfl_sync(0xffffffffu, skew, r & 31);
+    if (r >= rows) continue;
+    T* const out = static_cast<T*>(A.grad) + static_cast<size_t>(first + r) * R.vocab;
+    const Split<T> so(out, R.vocab);
+    uint4* const ov = reinterpret_cast<uint4*>(out + so.head);
+    const unsigned char* const row = base + static_cast<size_t>(r) * A.pitch;
+    if (!(live_rows >> r & 1)) {
+      for (uint32_t l = gl; l < so.vecs; l += kG) ov[l] = make_uint4(0, 0, 0, 0);
+      for (uint32_t i = gl; i < so.head + so.tail; i += kG) store_one(out + so.edge(i), 0.f);
+      continue;
+    }
+    const Ex ex(m, R.c_hi, R.c_lo);
+    const uint64_t k2 = pack2(k, k);
+    const uint32_t shift = (sk + so.head) * sizeof(T);
+#pragma unroll 2
+    for (uint32_t l = gl; l < so.vecs; l += kG) {
+      Pairs<T> q(load_shifted(row, l * 16 + shift));
+#pragma unroll
+      for (int u = 0; u < Pairs<T>::kN; ++u) q.p[u] = mul2(ex.two(q.p[u]), k2);
+      ov[l] = q.line();
+    }
+    for (uint32_t i = gl; i < so.head + so.tail; i += kG) {
+      const uint32_t j = so.edge(i);
+      store_one(out + j, ex_one(load_one(reinterpret_cast<const T*>(row) + sk + j), m, R.c_hi, R.c_lo) * k);
+    }
+  }
+  __syncwarp();   // the targets' elements, written as 0 above
+  if (live && has_y) store_one(static_cast<T*>(A.grad) + static_cast<size_t>(first + lane) * R.vocab + y, gy);
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+// Long rows: a row per block, or per cluster of blocks that take a slice each. A slice's 16-byte lines come into shared
+// memory at once by cp.async, so a block has all its bytes in flight and several blocks of an SM are at different stages:
+// each row is read once, however often the kernel goes over it. Every thread masks, maximises and sums the lines that it
+// loaded itself; the blocks' parts meet in distributed shared memory; for the policy loss one thread forms the row's values
+// in 64 bits, and all go over the slice again for the gradient, by the lines of the output.
+//
+// Exponentials again instead of kept ones: 32 fp32 exponentials a thread in registers left two blocks of 512 threads an SM, whose
+// chain of load, cluster exchange and row values then stands between them (8192 rows of 131072: 1497 us).
+struct SliceArgs {
+  Rows R;
+  int cl;               // blocks per row
+  float* logp;          // [n], or null
+  float* lse;           // [n], or null
+  double* logp64;       // [n] with coef [n] (preference), or null
+  float* coef;
+  Policy P;
+  void* grad;           // [n][vocab], or null
+  double* partials;     // [n][4] (policy)
+};
+
+template <typename T, int kThreads, bool kPolicy>
+__global__ void __launch_bounds__(kThreads, 1024 / kThreads) slice_kernel(const __grid_constant__ SliceArgs A) {
+  extern __shared__ __align__(16) unsigned char sm[];
+  using W = Word<T>;
+  constexpr uint32_t kPer = 16 / sizeof(T);
   __shared__ Part sh_warp[kThreads / 32], sh_block[kMaxCluster];
   __shared__ float sh_g[2];
   __shared__ float sh_in[4];   // the row's target logit, advantage, old and reference log-probability
@@ -641,385 +665,215 @@ __global__ void __launch_bounds__(kThreads) held_kernel(const __grid_constant__ 
   MO_CHECK(row < R.n && rank < static_cast<uint32_t>(A.cl));
   pdl_go();
   const uint32_t seq = row / R.tokens, tok = row - seq * R.tokens;
-  const int64_t y64 = R.y[seq * R.y_seq + tok * R.y_tok];
   const T* const z = reinterpret_cast<const T*>(R.z) + (seq * R.z_seq + tok * R.z_tok);
   T* const out = static_cast<T*>(A.grad) + static_cast<size_t>(row) * R.vocab;
-  const Split<T> sp(z, R.vocab);
-  const Split<T> so(out, R.vocab);
-  const uint32_t share = (sp.vecs + A.cl - 1) / A.cl, begin = rank * share, end = min(begin + share, sp.vecs);
-  MO_CHECK(share <= static_cast<uint32_t>(kThreads * kVecs));
-  const bool wide = so.head == sp.head;   // both rows start at the same place of a 16-byte line
-  const bool edge = rank == 0 && threadIdx.x < sp.head + sp.tail;
-  const uint32_t je = sp.edge(threadIdx.x);
-  if (y64 < 0 || (A.P.weight.p && A.P.weight.at(seq, tok) == 0.f)) {   // the whole cluster
-    if (rank == 0 && threadIdx.x < 4) {
-      A.partials[static_cast<size_t>(row) * 4 + threadIdx.x] = 0.0;
-      if (threadIdx.x == 0) A.logp[row] = 0.f;
+  // the slice [e0, e1) is cut at the output's lines where there is a gradient, at the input's otherwise
+  const Split<T> so(kPolicy && A.grad ? out : z, R.vocab);
+  const uint32_t share = (so.vecs + A.cl - 1) / A.cl;
+  const uint32_t v0 = min(rank * share, so.vecs), v1 = min(v0 + share, so.vecs);
+  const bool last = rank == static_cast<uint32_t>(A.cl) - 1;
+  const uint32_t e0 = rank == 0 ? 0 : so.head + v0 * kPer, e1 = last ? R.vocab : so.head + v1 * kPer;
+  // this thread's element beside the output's lines, if any
+  uint32_t je = 0xffffffffu;
+  if (rank == 0 && threadIdx.x < so.head) je = threadIdx.x;
+  if (last && threadIdx.x >= 32 && threadIdx.x < 32 + so.tail) je = so.head + so.vecs * kPer + threadIdx.x - 32;
+
+  int64_t y64 = in_packed(R, row) ? R.y[seq * R.y_seq + tok * R.y_tok] : -1;
+  if (kPolicy && A.P.weight.p && A.P.weight.at(seq, tok) == 0.f) y64 = -1;
+  if (y64 < 0) {   // the whole cluster
+    if (rank == 0 && threadIdx.x == 0) {
+      if (A.logp) A.logp[row] = 0.f;
+      if (A.lse) A.lse[row] = 0.f;
+      if (A.logp64) {
+        A.logp64[row] = 0.0;
+        A.coef[row] = 0.f;
+      }
     }
-    if (A.grad) {
-      if (wide) {
-        if (edge) store_one(out + je, 0.f);
-        for (uint32_t i = begin + threadIdx.x; i < end; i += kThreads)
-          reinterpret_cast<uint4*>(out + sp.head)[i] = make_uint4(0, 0, 0, 0);
-      } else {
-        for (uint32_t j = rank * kThreads + threadIdx.x; j < R.vocab; j += kThreads * A.cl) store_one(out + j, 0.f);
+    if (kPolicy) {
+      if (rank == 0 && threadIdx.x < 4) A.partials[static_cast<size_t>(row) * 4 + threadIdx.x] = 0.0;
+      if (A.grad) {
+        if (je != 0xffffffffu) store_one(out + je, 0.f);
+        for (uint32_t i = v0 + threadIdx.x; i < v1; i += kThreads)
+          reinterpret_cast<uint4*>(out + so.head)[i] = make_uint4(0, 0, 0, 0);
       }
     }
     return;
   }
-  if (A.cl > 1) cluster_arrive();
+  if (A.cl > 1) cluster_arrive_relaxed();
+
+  const uint64_t a0 = reinterpret_cast<uint64_t>(z + e0);
+  const uint32_t skew = static_cast<uint32_t>(a0 & 15) / sizeof(T);             // elements in front of e0 in line 0
+  const uint32_t lines = e1 > e0 ? (skew + (e1 - e0) + kPer - 1) / kPer : 0;
+  MO_CHECK(lines <= share + 3);
+  const uint32_t dst = smem_u32(sm);
+  const float inv_t = static_cast<float>(R.inv_t);
+  for (uint32_t i = threadIdx.x; i < lines; i += kThreads)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + i * 16), "l"((a0 & ~15ull) + i * 16ull) : "memory");
+  asm volatile("cp.async.commit_group;" ::: "memory");
   const bool has_y = y64 < static_cast<int64_t>(R.vocab);
   const uint32_t y = has_y ? static_cast<uint32_t>(y64) : 0xffffffffu;
-  const uint32_t yv = has_y && y >= sp.head ? (y - sp.head) / kPer : 0xffffffffu, ye = (y - sp.head) % kPer;
-  const uint4* const zv = reinterpret_cast<const uint4*>(z + sp.head);
-  uint4 v[kVecs];
-#pragma unroll
-  for (int k = 0; k < kVecs; ++k) {
-    const uint32_t at = begin + threadIdx.x + k * kThreads;
-    v[k] = make_uint4(W::kEmpty, W::kEmpty, W::kEmpty, W::kEmpty);
-    if (at < end) v[k] = load_vec(zv + at);
-  }
-  float xe = kNegInf;
-  if (edge && je != y) xe = load_one(z + je);
   if (threadIdx.x < 4) {   // read by thread 0 behind row_join's barrier
-    const Per& per = threadIdx.x == 1 ? A.P.adv : threadIdx.x == 2 ? A.P.old_lp : A.P.ref_lp;
     float x = NAN;
     if (threadIdx.x == 0) {
       if (has_y) x = load_one(z + y);
-    } else if (per.p) {
-      x = per.at(seq, tok);
+    } else if (kPolicy) {
+      const Per& per = threadIdx.x == 1 ? A.P.adv : threadIdx.x == 2 ? A.P.old_lp : A.P.ref_lp;
+      if (per.p) x = per.at(seq, tok);
     }
     sh_in[threadIdx.x] = x;
   }
-  uint32_t top = W::kEmpty;
-#pragma unroll
-  for (int k = 0; k < kVecs; ++k) {
-    if (begin + threadIdx.x + k * kThreads == yv) drop_target<T>(v[k], ye);
-    top = vec_max<T>(top, v[k]);
-  }
-  const float m = fmaxf(W::top(top), xe), mm = m == kNegInf ? 0.f : m;
-  const Ex ex(mm, R.c_hi, R.c_lo);
-  float e[32], s0 = 0.f, s1 = 0.f;
-#pragma unroll
-  for (int k = 0; k < kVecs; ++k) {
-    const uint32_t q[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
-    if (W::kPer == 2) {
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        ex.two(lo_bf16(q[u]), hi_bf16(q[u]), e[k * 8 + 2 * u], e[k * 8 + 2 * u + 1]);
-        s0 += e[k * 8 + 2 * u];
-        s1 += e[k * 8 + 2 * u + 1];
-      }
-    } else {
-#pragma unroll
-      for (int u = 0; u < 4; u += 2) {
-        ex.two(__uint_as_float(q[u]), __uint_as_float(q[u + 1]), e[k * 4 + u], e[k * 4 + u + 1]);
-        s0 += e[k * 4 + u];
-        s1 += e[k * 4 + u + 1];
-      }
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+
+  // a thread's own lines: what lies beside the slice in the first and the last one, and the target, become -inf
+  uint4* const line = reinterpret_cast<uint4*>(sm);
+  const uint32_t len = e1 - e0, ty = y - e0 < len ? skew + (y - e0) : 0xffffffffu;
+  if (threadIdx.x == 0 && skew != 0 && lines > 0) keep<T>(line[0], skew, kPer);
+  if (lines > 0 && threadIdx.x == (lines - 1) % kThreads) keep<T>(line[lines - 1], 0, skew + len - (lines - 1) * kPer);
+  if (ty != 0xffffffffu && threadIdx.x == ty / kPer % kThreads) drop_target<T>(line[ty / kPer], ty % kPer);
+  float m = kNegInf;
+  uint64_t acc = 0;
+  for (uint32_t i = threadIdx.x; i < lines; i += 2 * kThreads) {   // two lines at a time under a running maximum
+    const uint4 va = line[i];
+    uint4 vb = make_uint4(W::kEmpty, W::kEmpty, W::kEmpty, W::kEmpty);
+    if (i + kThreads < lines) vb = line[i + kThreads];
+    const float top = W::top(vec_max<T>(vec_max<T>(W::kEmpty, va), vb));
+    if (top > m) {
+      const float by = rescale(m, top, inv_t);
+      acc = mul2(acc, pack2(by, by));
+      m = top;
     }
+    const Ex ex(m == kNegInf ? 0.f : m, R.c_hi, R.c_lo);
+    const Pairs<T> qa(va), qb(vb);
+#pragma unroll
+    for (int u = 0; u < Pairs<T>::kN; ++u) acc = add2(acc, add2(ex.two(qa.p[u]), ex.two(qb.p[u])));
   }
-  const float ee = ex_one(xe, mm, R.c_hi, R.c_lo);
-  const float inv_t = static_cast<float>(R.inv_t);
-  const Part p = row_join<kThreads>(Part{m, s0 + s1 + ee}, A.cl, rank, inv_t, sh_warp, sh_block);
-  if (threadIdx.x == 0) {
+  float s0, s1;
+  unpack2(acc, s0, s1);
+  const Part p = row_join<kThreads>(Part{m, s0 + s1}, A.cl, rank, inv_t, sh_warp, sh_block);
+  if (threadIdx.x == 0 && (kPolicy || rank == 0)) {
     const RowStat st = row_stat(sh_in[0], p.m, p.s, R.inv_t);
-    const RowLoss L = policy_row_loss(st.logp, A.P, sh_in[2], sh_in[3], A.P.ref_lp.p != nullptr, sh_in[1]);
-    const double w = A.P.weight.p ? A.P.weight.at(seq, tok) : 1.f;
-    const double inv = A.P.div ? 1.0 / static_cast<double>(*A.P.div) : A.P.inv_div;
-    const float g = static_cast<float>(w * L.slope * inv * R.inv_t);
-    sh_g[0] = -g * st.f;
-    sh_g[1] = g * st.rest;
+    if (kPolicy) {
+      const RowLoss L = policy_row_loss(st.logp, A.P, sh_in[2], sh_in[3], A.P.ref_lp.p != nullptr, sh_in[1]);
+      const double w = A.P.weight.p ? A.P.weight.at(seq, tok) : 1.f;
+      const double inv = A.P.div ? 1.0 / static_cast<double>(*A.P.div) : A.P.inv_div;
+      const float g = static_cast<float>(w * L.slope * inv * R.inv_t);
+      sh_g[0] = -g * st.f;
+      sh_g[1] = g * st.rest;
+      if (rank == 0) {
+        double* const o = A.partials + static_cast<size_t>(row) * 4;
+        o[0] = w * L.loss * inv;
+        o[1] = w;
+        o[2] = w * L.kl * inv;
+        o[3] = L.clipped ? w : 0.0;
+      }
+    }
     if (rank == 0) {
-      A.logp[row] = static_cast<float>(st.logp);
-      double* const o = A.partials + static_cast<size_t>(row) * 4;
-      o[0] = w * L.loss * inv;
-      o[1] = w;
-      o[2] = w * L.kl * inv;
-      o[3] = L.clipped ? w : 0.0;
+      if (A.logp) A.logp[row] = static_cast<float>(st.logp);
+      if (A.lse) A.lse[row] = static_cast<float>(st.lse);
+      if (A.logp64) {
+        A.logp64[row] = st.logp;
+        A.coef[row] = 0.f;
+      }
     }
   }
-  if (A.grad == nullptr) return;
+  if (!kPolicy || A.grad == nullptr) return;
   __syncthreads();
-  const float f = sh_g[0] * rescale(m, p.m, inv_t), gy = sh_g[1];
-  if (edge) store_one(out + je, je == y ? gy : ee * f);
+  const float f = sh_g[0], gy = sh_g[1];
+  const float M = p.m == kNegInf ? 0.f : p.m;
+  if (je != 0xffffffffu) {
+    const T* const x = reinterpret_cast<const T*>(sm) + skew + (je - e0);
+    store_one(out + je, je == y ? gy : ex_one(load_one(x), M, R.c_hi, R.c_lo) * f);
+  }
+  const Ex ex(M, R.c_hi, R.c_lo);
+  const uint64_t f2 = pack2(f, f);
+  const uint32_t shift = (skew + so.head - e0) * sizeof(T);   // from an output line's bytes to the slice's (wraps)
+#pragma unroll 2
+  for (uint32_t i = v0 + threadIdx.x; i < v1; i += kThreads) {
+    const uint32_t e = so.head + i * kPer;
+    Pairs<T> q(load_shifted(sm, i * 16 + shift));
 #pragma unroll
-  for (int k = 0; k < kVecs; ++k) {
-    const uint32_t at = begin + threadIdx.x + k * kThreads;
-    if (at >= end) continue;
-    T* const o = out + sp.head + at * kPer;
-    if (wide) {
-      uint4 d;
-      if (W::kPer == 2) {
-        d.x = to_bf16x2(e[k * 8] * f, e[(k * 8 + 1) & 31] * f);
-        d.y = to_bf16x2(e[(k * 8 + 2) & 31] * f, e[(k * 8 + 3) & 31] * f);
-        d.z = to_bf16x2(e[(k * 8 + 4) & 31] * f, e[(k * 8 + 5) & 31] * f);
-        d.w = to_bf16x2(e[(k * 8 + 6) & 31] * f, e[(k * 8 + 7) & 31] * f);
-      } else {
-        d = make_uint4(__float_as_uint(e[k * 4] * f), __float_as_uint(e[(k * 4 + 1) & 31] * f),
-                       __float_as_uint(e[(k * 4 + 2) & 31] * f), __float_as_uint(e[(k * 4 + 3) & 31] * f));
-      }
-      *reinterpret_cast<uint4*>(o) = d;
-    } else {
-#pragma unroll
-      for (int u = 0; u < kPer; ++u) store_one(o + u, e[k * kPer + u] * f);
-    }
-    if (at == yv) store_one(o + ye, gy);
+    for (int u = 0; u < Pairs<T>::kN; ++u) q.p[u] = mul2(ex.two(q.p[u]), f2);
+    *reinterpret_cast<uint4*>(out + e) = q.line();
+    if (y - e < kPer) store_one(out + y, gy);
   }
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
-// The gradient from kept row values: d_j = g ([j == y] - exp(x_j - lse)) / T with one coefficient g per row. Elementwise, so
-// a row may be cut anywhere. Rows with g = 0 are written as zeros and not read.
+// Long rows, the gradient from kept row values: elementwise, so a row is cut into pieces of kGradVecs lines a thread.
 struct GradArgs {
   Rows R;
-  Per logp, lse, coef;    // per position ...
-  const double* logp64;   // ... or by row: the preference loss's own [n] arrays
-  const float* lse_row;
-  const float* coef_row;
+  Kept K;
   void* grad;
-  uint32_t pieces;        // blocks per row (grad_kernel)
-  const double* pair_loss;   // preference: block 0 adds up the pairs' losses
-  int pairs;
-  float* loss;
-};
-struct GradRow {
-  bool live;
-  uint32_t y;
-  float g, gy, l_hi, l_lo;   // g / T, the target's gradient, lse log2(e) as two floats
-};
-__device__ __forceinline__ GradRow grad_row(const GradArgs& A, uint32_t row, uint32_t seq, uint32_t tok) {
-  const Rows& R = A.R;
-  GradRow r;
-  r.y = 0xffffffffu;
-  const int64_t y64 = R.y[seq * R.y_seq + tok * R.y_tok];
-  const float c = A.coef_row ? A.coef_row[row] : A.coef.at(seq, tok);
-  r.live = y64 >= 0 && c != 0.f;
-  if (!r.live) return r;
-  const double lse = A.lse_row ? A.lse_row[row] : A.lse.at(seq, tok);
-  const double lp = A.logp64 ? A.logp64[row] : static_cast<double>(A.logp.at(seq, tok));
-  r.g = static_cast<float>(c * R.inv_t);
-  r.gy = static_cast<float>(-expm1(lp) * c * R.inv_t);
-  r.l_hi = static_cast<float>(lse * kLog2e);
-  r.l_lo = static_cast<float>(lse * kLog2e - static_cast<double>(r.l_hi));
-  if (y64 < static_cast<int64_t>(R.vocab)) r.y = static_cast<uint32_t>(y64);
-  return r;
-}
-struct GradEx {   // -g 2^(z c - lse log2(e)): the large product and its small rest are rounded apart, then added
-  uint64_t hi, lo, l_hi, l_lo, g;
-  __device__ GradEx(const GradRow& r, const Rows& R)
-      : hi(pack2(R.c_hi, R.c_hi)), lo(pack2(R.c_lo, R.c_lo)), l_hi(pack2(-r.l_hi, -r.l_hi)), l_lo(pack2(-r.l_lo, -r.l_lo)),
-        g(pack2(-r.g, -r.g)) {}
-  __device__ __forceinline__ void two(float z0, float z1, float& d0, float& d1) const {
-    const uint64_t z = pack2(z0, z1);
-    float t0, t1;
-    unpack2(add2(fma2(z, hi, l_hi), fma2(z, lo, l_lo)), t0, t1);
-    unpack2(mul2(pack2(ex2(t0), ex2(t1)), g), d0, d1);
-  }
-  __device__ __forceinline__ float one(float z) const {
-    float d0, d1;
-    two(z, z, d0, d1);
-    return d0;
-  }
+  uint32_t pieces;        // blocks per row
 };
 constexpr int kGradThreads = 256, kGradVecs = 4;
-
-__device__ __forceinline__ void sum_pairs(const GradArgs& A) {   // one warp, in a fixed order
-  const int lane = threadIdx.x & 31;
-  double v = 0.0;
-  for (int i = lane; i < A.pairs; i += 32) v += A.pair_loss[i];
-  v = warp_sum(v);
-  if (lane == 0) *A.loss = static_cast<float>(v);
-}
 
 template <typename T>
 __global__ void __launch_bounds__(kGradThreads) grad_kernel(const __grid_constant__ GradArgs A) {
   const Rows& R = A.R;
-  constexpr int kPer = 16 / sizeof(T);
-  const uint32_t row = blockIdx.x / A.pieces, piece = blockIdx.x - row * A.pieces;
+  constexpr uint32_t kPer = 16 / sizeof(T);
+  // from the last row to the first: what the forward pass read last is still in L2
+  const uint32_t row = R.n - 1 - blockIdx.x / A.pieces, piece = blockIdx.x % A.pieces;
   const uint32_t seq = row / R.tokens, tok = row - seq * R.tokens;
   const T* const z = reinterpret_cast<const T*>(R.z) + (seq * R.z_seq + tok * R.z_tok);
   T* const out = static_cast<T*>(A.grad) + static_cast<size_t>(row) * R.vocab;
-  const Split<T> sp(z, R.vocab);
-  const bool wide = Split<T>(out, R.vocab).head == sp.head;
-  pdl_wait();
-  if (A.pair_loss && blockIdx.x == 0 && threadIdx.x < 32) sum_pairs(A);
+  const Split<T> so(out, R.vocab);
   MO_CHECK(row < R.n);
-  const GradRow r = grad_row(A, row, seq, tok);
+  const int64_t y64 = R.y[seq * R.y_seq + tok * R.y_tok];
   const uint32_t begin = piece * (kGradThreads * kGradVecs) + threadIdx.x;
-  const bool edge = piece == 0 && threadIdx.x < sp.head + sp.tail;
-  const uint32_t je = sp.edge(threadIdx.x);
-  if (!r.live) {
+  // an output line's elements: one line of the input, or two and a shift where the two rows are aligned differently
+  const uint64_t a = reinterpret_cast<uint64_t>(z + so.head);
+  const uint32_t by = static_cast<uint32_t>(a & 15);
+  const uint4* const zv = reinterpret_cast<const uint4*>(a & ~15ull);
+  uint4 v[kGradVecs], w[kGradVecs];
+  if (y64 >= 0) {   // inputs: read before the launch in front of this one has ended
+#pragma unroll
+    for (int k = 0; k < kGradVecs; ++k) {
+      const uint32_t at = begin + k * kGradThreads;
+      if (at < so.vecs) v[k] = load_vec(zv + at);
+    }
+    if (by) {
+#pragma unroll
+      for (int k = 0; k < kGradVecs; ++k) {
+        const uint32_t at = begin + k * kGradThreads;
+        if (at < so.vecs) w[k] = load_vec(zv + at + 1);
+      }
+    }
+  }
+  pdl_wait();
+  if (A.K.pair_loss && blockIdx.x == 0 && threadIdx.x < 32) sum_pairs(A.K);
+  const float coef = y64 >= 0 ? kept_coef(A.K, row, seq, tok) : 0.f;
+  const bool edge = piece == 0 && threadIdx.x < so.head + so.tail;
+  const uint32_t je = so.edge(threadIdx.x);
+  uint4* const ov = reinterpret_cast<uint4*>(out + so.head);
+  if (coef == 0.f) {
     if (edge) store_one(out + je, 0.f);
 #pragma unroll
     for (int k = 0; k < kGradVecs; ++k) {
       const uint32_t at = begin + k * kGradThreads;
-      if (at >= sp.vecs) break;
-      T* const o = out + sp.head + at * kPer;
-      if (wide) {
-        *reinterpret_cast<uint4*>(o) = make_uint4(0, 0, 0, 0);
-      } else {
-#pragma unroll
-        for (int u = 0; u < kPer; ++u) store_one(o + u, 0.f);
-      }
+      if (at < so.vecs) ov[at] = make_uint4(0, 0, 0, 0);
     }
     return;
   }
-  const GradEx ex(r, R);
-  const uint32_t yv = r.y != 0xffffffffu && r.y >= sp.head ? (r.y - sp.head) / kPer : 0xffffffffu, ye = (r.y - sp.head) % kPer;
-  const uint4* const zv = reinterpret_cast<const uint4*>(z + sp.head);
-  uint4 v[kGradVecs];
+  const KeptRow r = kept_row(A.K, R, row, seq, tok, coef);
+  const Ex ex(r.m, R.c_hi, R.c_lo);
+  const uint64_t f2 = pack2(r.f, r.f);
+  const uint32_t y = y64 < static_cast<int64_t>(R.vocab) ? static_cast<uint32_t>(y64) : 0xffffffffu;
+  if (edge) store_one(out + je, je == y ? r.gy : ex_one(load_one(z + je), r.m, R.c_hi, R.c_lo) * r.f);
 #pragma unroll
   for (int k = 0; k < kGradVecs; ++k) {
     const uint32_t at = begin + k * kGradThreads;
-    if (at < sp.vecs) v[k] = load_vec(zv + at);
-  }
-  if (edge) store_one(out + je, je == r.y ? r.gy : ex.one(load_one(z + je)));
+    if (at >= so.vecs) break;
+    Pairs<T> q(by ? shift_lines(v[k], w[k], by) : v[k]);
 #pragma unroll
-  for (int k = 0; k < kGradVecs; ++k) {
-    const uint32_t at = begin + k * kGradThreads;
-    if (at >= sp.vecs) break;
-    const uint32_t q[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
-    T* const o = out + sp.head + at * kPer;
-    uint32_t d[4];
-    if (sizeof(T) == 2) {
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        float d0, d1;
-        ex.two(lo_bf16(q[u]), hi_bf16(q[u]), d0, d1);
-        d[u] = to_bf16x2(d0, d1);
-      }
-    } else {
-#pragma unroll
-      for (int u = 0; u < 4; u += 2) {
-        float d0, d1;
-        ex.two(__uint_as_float(q[u]), __uint_as_float(q[u + 1]), d0, d1);
-        d[u] = __float_as_uint(d0);
-        d[u + 1] = __float_as_uint(d1);
-      }
-    }
-    if (wide) {
-      *reinterpret_cast<uint4*>(o) = make_uint4(d[0], d[1], d[2], d[3]);
-    } else if (sizeof(T) == 2) {
-#pragma unroll
-      for (int u = 0; u < kPer; ++u) reinterpret_cast<uint16_t*>(o)[u] = static_cast<uint16_t>(d[u >> 1] >> (16 * (u & 1)));
-    } else {
-#pragma unroll
-      for (int u = 0; u < kPer; ++u) reinterpret_cast<uint32_t*>(o)[u] = d[u & 3];
-    }
-    if (at == yv) store_one(o + ye, r.gy);
-  }
-}
-
-// Short rows: a warp per row, in words of 4 bytes (16-byte vectors would leave most lanes of a row of a few hundred logits
-// without one).
-template <typename T>
-__global__ void __launch_bounds__(kGradThreads) grad_short_kernel(const __grid_constant__ GradArgs A) {
-  using W = Word<T>;
-  const Rows& R = A.R;
-  const int lane = threadIdx.x & 31;
-  const uint32_t row = blockIdx.x * (kGradThreads / 32) + (threadIdx.x >> 5);
-  pdl_wait();
-  if (A.pair_loss && blockIdx.x == 0 && threadIdx.x < 32) sum_pairs(A);
-  if (row >= R.n) return;
-  const uint32_t seq = row / R.tokens, tok = row - seq * R.tokens;
-  const T* const z = reinterpret_cast<const T*>(R.z) + (seq * R.z_seq + tok * R.z_tok);
-  T* const out = static_cast<T*>(A.grad) + static_cast<size_t>(row) * R.vocab;
-  const GradRow r = grad_row(A, row, seq, tok);
-  if (!r.live) {
-    for (uint32_t j = lane; j < R.vocab; j += 32) store_one(out + j, 0.f);
-    return;
-  }
-  const GradEx ex(r, R);
-  // words of the input; an output whose row has the other parity is stored element by element
-  const uint32_t sk = W::kPer == 2 ? (reinterpret_cast<uint64_t>(z) >> 1) & 1 : 0;
-  const bool wide = W::kPer == 1 || ((reinterpret_cast<uint64_t>(out) >> 1) & 1) == sk;
-  const uint32_t words = (sk + R.vocab + W::kPer - 1) / W::kPer;
-  const T* const zw = z - sk;
-  T* const ow = out - sk;
-#pragma unroll 4
-  for (uint32_t w = lane; w < words; w += 32) {
-    if (W::kPer == 1) {
-      store_one(out + w, w == r.y ? r.gy : ex.one(load_one(z + w)));
-      continue;
-    }
-    const uint32_t j = 2 * w - sk;   // wraps where only the second element lies in the row
-    const bool in0 = j < R.vocab, in1 = j + 1 < R.vocab;
-    float z0 = 0.f, z1 = 0.f;
-    if (in0 && in1) {
-      const uint32_t v = *reinterpret_cast<const uint32_t*>(zw + 2 * w);
-      z0 = lo_bf16(v);
-      z1 = hi_bf16(v);
-    } else if (in0) {
-      z0 = load_one(zw + 2 * w);
-    } else {
-      z1 = load_one(zw + 2 * w + 1);
-    }
-    float d0, d1;
-    ex.two(z0, z1, d0, d1);
-    if (j == r.y) d0 = r.gy;
-    if (j + 1 == r.y) d1 = r.gy;
-    const uint32_t d = to_bf16x2(d0, d1);
-    if (wide && in0 && in1) {
-      *reinterpret_cast<uint32_t*>(ow + 2 * w) = d;
-    } else {
-      if (in0) *reinterpret_cast<uint16_t*>(ow + 2 * w) = static_cast<uint16_t>(d);
-      if (in1) *reinterpret_cast<uint16_t*>(ow + 2 * w + 1) = static_cast<uint16_t>(d >> 16);
-    }
+    for (int u = 0; u < Pairs<T>::kN; ++u) q.p[u] = mul2(ex.two(q.p[u]), f2);
+    ov[at] = q.line();
+    const uint32_t e = so.head + at * kPer;
+    if (y - e < kPer) store_one(out + y, r.gy);
   }
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
-// Row values of the policy loss from kept log-probabilities (rows too long to be held): a thread per row.
-struct PolicyRowsArgs {
-  Rows R;
-  Policy P;
-  const double* logp64;
-  float* logp;
-  float* coef;
-  double* partials;       // [blocks][4]
-};
-__global__ void __launch_bounds__(256) policy_rows_kernel(const __grid_constant__ PolicyRowsArgs A) {
-  const Rows& R = A.R;
-  __shared__ double sh[8][4];
-  const uint32_t row = blockIdx.x * 256 + threadIdx.x;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  pdl_wait();
-  pdl_go();
-  double part[4] = {0.0, 0.0, 0.0, 0.0};
-  if (row < R.n) {
-    const uint32_t seq = row / R.tokens, tok = row - seq * R.tokens;
-    const float wt = A.P.weight.p ? A.P.weight.at(seq, tok) : 1.f;
-    const bool live = R.y[seq * R.y_seq + tok * R.y_tok] >= 0 && wt != 0.f;
-    float g = 0.f, lp = 0.f;
-    if (live) {
-      const double l = A.logp64[row];
-      const RowLoss L = policy_row_loss(l, A.P, A.P.old_lp.at(seq, tok), A.P.ref_lp.p ? A.P.ref_lp.at(seq, tok) : 0.f,
-                                        A.P.ref_lp.p != nullptr, A.P.adv.at(seq, tok));
-      const double w = wt, inv = A.P.div ? 1.0 / static_cast<double>(*A.P.div) : A.P.inv_div;
-      part[0] = w * L.loss * inv;
-      part[1] = w;
-      part[2] = w * L.kl * inv;
-      part[3] = L.clipped ? w : 0.0;
-      g = static_cast<float>(w * L.slope * inv);
-      lp = static_cast<float>(l);
-    }
-    A.coef[row] = g;
-    A.logp[row] = lp;
-  }
-#pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    const double v = warp_sum(part[k]);
-    if (lane == 0) sh[warp][k] = v;
-  }
-  __syncthreads();
-  if (threadIdx.x < 4) {
-    double v = 0.0;
-    for (int w = 0; w < 8; ++w) v += sh[w][threadIdx.x];
-    A.partials[static_cast<size_t>(blockIdx.x) * 4 + threadIdx.x] = v;
-  }
-}
-
 // Sums of `n` rows of four partials, in a fixed order: block b adds up its contiguous share. With one block the result goes
 // to out32, else a block's to out64[b].
 struct SumArgs {
@@ -1151,9 +1005,9 @@ __global__ void __launch_bounds__(kPairThreads) pair_kernel(const __grid_constan
 }
 
 // The pairs' losses added up where no gradient pass does it
-__global__ void __launch_bounds__(32) pair_sum_kernel(const __grid_constant__ GradArgs A) {
+__global__ void __launch_bounds__(32) pair_sum_kernel(const __grid_constant__ Kept K) {
   pdl_wait();
-  sum_pairs(A);
+  sum_pairs(K);
 }
 
 }  // namespace loss

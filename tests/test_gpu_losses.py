@@ -13,11 +13,11 @@ pytestmark = pytest.mark.gpu
 
 BF, F32 = torch.bfloat16, torch.float32
 # (sequences, positions, vocabulary): a vocabulary of one, words, warps and 16-byte lines and one beside them, the byte
-# vocabulary, the limits of the warp-per-rows kernels (4600 and 2300 logits), of a block's held rows and of a cluster's,
-# and rows longer than what is held
-SIZES = [(1, 1, 1), (2, 3, 1), (3, 5, 2), (2, 7, 3), (4, 9, 17), (2, 33, 64), (5, 31, 271), (1, 1, 271), (3, 2, 2299),
-         (3, 2, 2300), (2, 2, 2301), (2, 3, 4600), (2, 2, 4601), (1, 3, 8193), (2, 2, 16384), (1, 2, 16391), (1, 2, 50021),
-         (1, 1, 131072), (1, 1, 262144), (1, 2, 262160)]
+# vocabulary, the limits of the warp-per-rows kernels (4592 bf16 and 2296 fp32 logits), slices of one block and of clusters
+# of 2 to 16, and the longest fp32 row
+SIZES = [(1, 1, 1), (2, 3, 1), (3, 5, 2), (2, 7, 3), (4, 9, 17), (2, 33, 64), (5, 31, 271), (1, 1, 271), (3, 2, 2296),
+         (3, 2, 2297), (2, 2, 1100), (2, 3, 4592), (2, 2, 4593), (1, 3, 8193), (80, 2, 16384), (1, 2, 16391), (2, 80, 50021),
+         (1, 1, 131072), (1, 1, 262144), (1, 2, 262160), (1, 1, 900864)]
 
 
 @pytest.fixture(scope="module")
@@ -445,6 +445,8 @@ def test_refusals(dev):
            (MoteoptError, lambda: token_logprobs(z, y, temperature=-1.0)),
            (MoteoptError, lambda: token_logprobs(z, y, temperature=math.nan)),
            (MoteoptError, lambda: token_logprobs(z, y, temperature=math.inf)),
+           (MoteoptError, lambda: token_logprobs(torch.zeros(1, 900865, device=dev), y[:1, 0])),
+           (MoteoptError, lambda: token_logprobs(torch.zeros(1, 1801729, dtype=BF, device=dev), y[:1, 0])),
            (TypeError, lambda: policy_loss(z, y, f.double(), f)), (ValueError, lambda: policy_loss(z, y, f, f[0])),
            (ValueError, lambda: policy_loss(z, y, f[:, 0].cpu(), f)), (ValueError, lambda: policy_loss(z, y, f, f, kl_coef=0.1)),
            (MoteoptError, lambda: policy_loss(z, y, f, f, clip_low=-0.1)),
