@@ -1,4 +1,5 @@
-"""Build libmoteopt.so (the CUDA kernels and the C ABI of include/moteopt.h) for sm_100a, in-tree.
+"""Build libmoteopt.so (the CUDA kernels and the C ABI of include/moteopt.h) for sm_100a and _torch_losses.so (the losses'
+torch binding, host code), in-tree.
 
     python -m mote_b200.build            # or: python mote_b200/build.py
     python -m mote_b200.build --checked  # libmoteopt_checked.so
@@ -16,6 +17,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -25,6 +27,8 @@ LIB = PKG / "libmoteopt.so"
 CHECKED_LIB = PKG / "libmoteopt_checked.so"   # the same library with MOTE_OPT_CHECKS: index checks in every kernel
 RESOURCES = PKG / "_build" / "ptxas_release.txt"   # ptxas's per-kernel registers / spills of the release build
 SOURCES = [CSRC / "moteopt.cu"]
+BINDING = PKG / "_torch_losses.so"
+BINDING_SOURCE = CSRC / "torch_losses.cpp"
 HEADERS = sorted(CSRC.glob("*.cuh")) + sorted(CSRC.glob("*.h")) + [ROOT / "include" / "moteopt.h"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
@@ -44,10 +48,35 @@ def needs_build() -> bool:
     return any(p.stat().st_mtime > t for p in SOURCES + HEADERS)
 
 
+def build_binding(force: bool = False, verbose: bool = False) -> Path:
+    """g++ the torch binding of the losses (no CUDA code; it is given libmoteopt.so's functions when it is imported)."""
+    sources = [BINDING_SOURCE, ROOT / "include" / "moteopt.h"]
+    if not force and BINDING.exists() and all(p.stat().st_mtime <= BINDING.stat().st_mtime for p in sources):
+        return BINDING
+    import torch
+    from torch.utils import cpp_extension as ext
+    tmp = BINDING.with_suffix(".so.tmp")
+    inc = [str(ROOT / "include"), sysconfig.get_paths()["include"], *ext.include_paths("cuda")]
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *[a for d in inc for a in ("-I", d)],
+           str(BINDING_SOURCE), "-o", str(tmp), *[a for d in ext.library_paths("cuda") for a in ("-L", d)], "-lc10",
+           "-lc10_cuda", "-ltorch_cpu", "-ltorch_python"]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        sys.stderr.write(r.stdout + r.stderr)
+        raise subprocess.CalledProcessError(r.returncode, cmd)
+    os.replace(tmp, BINDING)
+    return BINDING
+
+
 def build(force: bool = False, verbose: bool = False, extra: list[str] | None = None, checked: bool = False) -> Path:
-    """nvcc the library; `checked` builds libmoteopt_checked.so, which counts failed index checks
+    """nvcc the library (and build the torch binding); `checked` builds libmoteopt_checked.so, which counts failed index checks
     (moteopt_check_count) instead of the release library."""
     out = CHECKED_LIB if checked else LIB
+    if not checked:
+        build_binding(force, verbose)
     if not force and not checked and not needs_build():
         return LIB
     if checked:

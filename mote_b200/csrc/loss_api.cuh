@@ -101,11 +101,11 @@ int launch_cluster(void (*kernel)(Args), const Args& A, unsigned rows, unsigned 
 bool short_rows(int dtype, int64_t vocab) { return vocab * esize(dtype) <= kShortBytes; }
 
 // The warps' share of short rows: as many rows as fit kTileBytes, at most kTileRows, and fewer while that would leave an SM
-// less than 16 warps (a warp takes its rows one after the other).
+// less than 24 warps (a warp takes its rows four at a time, one lot after the other).
 void tile_shape(int64_t rows, int dtype, int64_t vocab, int sms, int* per_warp, uint32_t* pitch) {
   *pitch = static_cast<uint32_t>(((vocab * esize(dtype) + 16 - esize(dtype) + 15) / 16 + 1) * 16);
   const int64_t most = std::min<int64_t>(kTileRows, kTileBytes / *pitch);
-  *per_warp = static_cast<int>(std::max<int64_t>(1, std::min(most, rows / (16 * sms))));
+  *per_warp = static_cast<int>(std::max<int64_t>(1, std::min(most, rows / (24 * sms))));
 }
 
 // Lanes per row: 8, and the whole warp where a row has more than 16 lines for each of them.

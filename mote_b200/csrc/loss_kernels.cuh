@@ -8,8 +8,8 @@
 // a = x_y - m/T,
 //   a >= 0: logp = -log1p(s e^-a)          1 - p_y = X / (1 + X), X = s e^-a
 //   a <  0: logp = a - log1p(s - 1 + e^a)  1 - p_y = s / (s + e^a)
-// so that neither logp nor 1 - p_y cancels where the model is sure of its target (p_y -> 1). These few values of a row are
-// formed in 64 bits; the exponentials and the sums inside a thread are fp32.
+// so that neither logp nor 1 - p_y cancels where the model is sure of its target (p_y -> 1). The exponentials and their sums
+// are fp32, a position's logp is kept in 64 bits, and the sums over positions are in 64 bits.
 //
 // All kernels are memory-bound in principle (2 or 4 bytes read per logit, as many written for a gradient); the exponential
 // is next: one ex2 per logit at 16 per clock and SM is 0.73 of the copy bandwidth's rate for bf16 logits read once.
@@ -29,9 +29,9 @@ namespace loss {
 constexpr float kNegInf = -INFINITY;
 constexpr double kLog2e = 1.4426950408889634074;
 // ex2.approx's mean relative error below -1 is -5.05e-8, the same for every binade (measured over 4e6 arguments each). It
-// is a bias, so it would add up over the thousands of positions of a sequence; a row's sum, but for the 1 of its largest
-// element, is multiplied by the inverse.
-constexpr double kEx2Bias = 1.0 + 5.05e-8;
+// is a bias, so it would add up over the thousands of positions of a sequence; row_stat takes it out again.
+constexpr float kEx2Bias = 5.05e-8f;
+constexpr double kLn2 = 0.69314718055994530942;
 
 // logits [seqs][tokens][vocab], the last axis contiguous, and the targets [seqs][tokens]
 struct Rows {
@@ -214,36 +214,48 @@ __device__ __forceinline__ Part warp_join(Part p, float inv_t) {
   return Part{M, warp_sum(p.s == 0.f ? 0.f : p.s * rescale(p.m, M, inv_t))};
 }
 
-// What a row's sums give (see the top of this file)
+// What a row's sums give (see the top of this file). The differences and the results are in 64 bits; exp, the logarithm and
+// the quotient between them are fp32 functions, which keep 6e-8 of values of at most 1 in size: log(1 + X) is k log 2 +
+// log(f) + c with 1 + X = 2^k f, 3/4 <= f < 3/2, and c what the fp32 sum 1 + X lost. In 64 bits throughout, these functions
+// took a lane 1500 cycles and as many instructions as the row itself.
 struct RowStat {
   double logp, lse;
   float f;      // exp(m / T - lse): p_j = exp((z_j - m) / T) f
   float rest;   // 1 - p_y
 };
-__device__ __forceinline__ RowStat row_stat(float zy, float m, float s32, double inv_t) {
-  const double s = s32 >= 1.f ? 1.0 + (static_cast<double>(s32) - 1.0) * kEx2Bias : static_cast<double>(s32);
+__device__ __forceinline__ RowStat row_stat(float zy, float m, float s, double inv_t) {
   const double a = (static_cast<double>(zy) - static_cast<double>(m)) * inv_t;
   const bool up = a >= 0.0;
-  const double q = exp(up ? -a : a);
-  const double X = up ? (s == 0.0 ? 0.0 : s * q) : (s - 1.0) + q;
-  const double l = log1p(X), inv = 1.0 / (1.0 + X);
+  const float q = expf(static_cast<float>(up ? -a : a));
+  const float X = up ? (s == 0.f ? 0.f : s * q) : (s - 1.f) + q;
+  const float u = 1.f + X, inv = 1.f / u;
+  const int k = (__float_as_int(u) - 0x3f400000) >> 23;
+  const float f = __int_as_float(__float_as_int(u) - (k << 23));
+  // ex2's bias, in the part of the sum that is not the largest element's 1
+  const float bias = kEx2Bias * fmaxf(s - 1.f, 0.f) * (up ? q : 1.f) * inv;
+  double l = k * kLn2 + static_cast<double>(logf(f) + (X - (u - 1.f)) * inv + bias);
+  if (X != X) l = static_cast<double>(X);
   RowStat r;
   r.logp = up ? -l : a - l;
   r.lse = static_cast<double>(up ? zy : m) * inv_t + l;
-  r.f = static_cast<float>((up ? q : 1.0) * inv);
-  r.rest = static_cast<float>((up ? X : s) * inv);
+  r.f = (up ? q : 1.f) * inv;
+  r.rest = (up ? X : s) * inv;
   if (zy == INFINITY) r.logp = r.lse = static_cast<double>(r.f = r.rest = NAN);   // inf - inf
   return r;
 }
 
-// The policy loss of one row, unscaled by the weight and the divisor
+// The policy loss of one row, unscaled by the weight and the divisor. The ratio is an fp32 exponential of a 64-bit
+// difference, and taken in 64 bits where it lies within 1e-5 of a border, at which the gradient jumps. k(d) = e^d - d - 1 is
+// its series below 1 in size (the difference would cancel): 2 / (n + 2)! falls below 2^-24 at n = 9.
 struct RowLoss {
   double loss, kl, slope;   // slope: dloss/dlogp
   bool clipped;
 };
 __device__ __forceinline__ RowLoss policy_row_loss(double logp, const Policy& P, float old_lp, float ref_lp, bool has_ref,
                                                    float adv) {
-  const double A = adv, r = exp(logp - static_cast<double>(old_lp));
+  const double A = adv, d_old = logp - static_cast<double>(old_lp);
+  double r = expf(static_cast<float>(d_old));
+  if (fabs(r - P.clip_hi) < 1e-5 * P.clip_hi || fabs(r - P.clip_lo) < 1e-5 * P.clip_lo) r = exp(d_old);
   const double held_r = fmin(fmax(r, P.clip_lo), P.clip_hi);
   const double free = r * A, held = (r != r ? r : held_r) * A;
   RowLoss L;
@@ -252,11 +264,18 @@ __device__ __forceinline__ RowLoss policy_row_loss(double logp, const Policy& P,
   L.slope = L.clipped ? 0.0 : -free;
   L.kl = 0.0;
   if (has_ref) {
-    const double d = static_cast<double>(ref_lp) - logp, e = expm1(d);
-    L.kl = e - d;
+    const float d = static_cast<float>(static_cast<double>(ref_lp) - logp), e = expm1f(d);
+    float k = e - d;
+    if (fabsf(d) < 1.f) {
+      k = 1.f / 11.f;
+#pragma unroll
+      for (int n = 10; n >= 3; --n) k = fmaf(k, d, 1.f) * (1.f / n);
+      k = fmaf(k, d, 1.f) * (0.5f * d * d);
+    }
+    L.kl = k;
     if (P.kl != 0.0) {
       L.loss += P.kl * L.kl;
-      L.slope -= P.kl * e;
+      L.slope -= P.kl * static_cast<double>(e);
     }
   }
   return L;
@@ -413,11 +432,13 @@ __device__ __forceinline__ void sum_pairs(const Kept& K) {   // one warp, in a f
 // 15 bytes beside the row: the same aligned line, so nothing beyond the allocation), which lifts every alignment and stride
 // question and keeps all of a warp's rows in flight at once. kG lanes work on a row in lines of 16 bytes, 32 / kG rows at a
 // time: the quarter of a warp that shared memory serves at once reads 128 bytes in a row whatever the rows' pitch, and the
-// maximum and the sum take 3 shuffles for four rows. One lane per row forms the row's values in 64 bits (they would cost a
-// warp more than the whole row if it formed them for one row at a time). Then, for the gradient, the exponentials again from
+// maximum and the sum take 3 shuffles for four rows. One lane per row forms the row's values (a warp that formed them for one
+// row at a time would spend as much on them as on the row). Then, for the gradient, the exponentials again from
 // shared memory, by the lines of the output.
 constexpr int kTileWarps = 4;
-constexpr int kTileRows = 16;          // most rows of a warp
+constexpr int kTileRows = 8;           // most rows of a warp: 64 x 1024 x 271 bf16, forward, at 4, 8 and 16 rows: 16.2, 14.5
+                                       // and 18.2 us (fewer rows: more of a warp's instructions are not its rows'; more: too
+                                       // few warps an SM), policy loss 31.7, 27.5 and 31.2 us
 constexpr int kTileBytes = 9216;       // most bytes of a warp's rows: 6 blocks of 4 warps in an SM's shared memory
 enum Mode { kForward, kPolicyLoss, kGradient };
 
@@ -634,8 +655,8 @@ __global__ void __launch_bounds__(kTileWarps * 32) tile_kernel(const __grid_cons
 // Long rows: a row per block, or per cluster of blocks that take a slice each. A slice's 16-byte lines come into shared
 // memory at once by cp.async, so a block has all its bytes in flight and several blocks of an SM are at different stages:
 // each row is read once, however often the kernel goes over it. Every thread masks, maximises and sums the lines that it
-// loaded itself; the blocks' parts meet in distributed shared memory; for the policy loss one thread forms the row's values
-// in 64 bits, and all go over the slice again for the gradient, by the lines of the output.
+// loaded itself; the blocks' parts meet in distributed shared memory; for the policy loss one thread forms the row's
+// values, and all go over the slice again for the gradient, by the lines of the output.
 //
 // Exponentials again instead of kept ones: 32 fp32 exponentials a thread in registers left two blocks of 512 threads an SM, whose
 // chain of load, cluster exchange and row values then stands between them (8192 rows of 131072: 1497 us).
