@@ -376,11 +376,13 @@ typedef struct moteopt_positions {
   int64_t seq_stride, token_stride;
 } moteopt_positions;
 
-/* logprobs, lse: [seqs * tokens] fp32, contiguous; lse may be NULL. One launch. */
+/* logprobs, lse: [seqs * tokens] fp32, contiguous; lse may be NULL. Rows of up to 9184 bytes need no workspace. */
+MOTEOPT_API size_t moteopt_token_logprobs_workspace_size(const moteopt_logits* logits);
 MOTEOPT_API int moteopt_token_logprobs(const moteopt_logits* logits, const moteopt_positions* targets, double temperature,
-                                       float* logprobs, float* lse, moteopt_stream_t stream);
+                                       float* logprobs, float* lse, void* workspace, size_t workspace_bytes,
+                                       moteopt_stream_t stream);
 /* grad_logits = grad_logprobs ([j == y] - exp(x_j - lse)) / temperature from the logprobs and lse that
- * moteopt_token_logprobs gave for these logits. A position whose grad_logprobs is 0 is not read and gets 0. */
+ * moteopt_token_logprobs gave for these logits. A position whose grad_logprobs is 0 gets 0, whatever its logits hold. */
 MOTEOPT_API int moteopt_token_logprobs_backward(const moteopt_logits* logits, const moteopt_positions* targets,
                                                 double temperature, const moteopt_positions* logprobs,
                                                 const moteopt_positions* lse, const moteopt_positions* grad_logprobs,

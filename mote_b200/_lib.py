@@ -38,7 +38,7 @@ EXPORTS = (
     "moteopt_newton_schulz_workspace_size_variant", "moteopt_newton_schulz_variant",
     "moteopt_grad_sumsq_tensors", "moteopt_peer_reduce_workspace_size", "moteopt_peer_reduce_sumsq",
     "moteopt_clip_coef_from_tensor_sums", "moteopt_selftest_grad_divide",
-    "moteopt_token_logprobs", "moteopt_token_logprobs_backward",
+    "moteopt_token_logprobs_workspace_size", "moteopt_token_logprobs", "moteopt_token_logprobs_backward",
     "moteopt_policy_loss_workspace_size", "moteopt_policy_loss",
     "moteopt_preference_loss_workspace_size", "moteopt_preference_loss",
 )
@@ -170,7 +170,8 @@ def _load() -> C.CDLL:
         "moteopt_peer_reduce_workspace_size": (sz, [C.POINTER(PeerPiece), i32]),
         "moteopt_peer_reduce_sumsq": (i32, [C.POINTER(PeerPiece), i32, i32, i32, dbl, vp, vp, sz, vp]),
         "moteopt_clip_coef_from_tensor_sums": (i32, [vp, i32, i32, i32, dbl, vp, vp]),
-        "moteopt_token_logprobs": (i32, [C.POINTER(Logits), C.POINTER(Positions), dbl, vp, vp, vp]),
+        "moteopt_token_logprobs_workspace_size": (sz, [C.POINTER(Logits)]),
+        "moteopt_token_logprobs": (i32, [C.POINTER(Logits), C.POINTER(Positions), dbl, vp, vp, vp, sz, vp]),
         "moteopt_token_logprobs_backward": (i32, [C.POINTER(Logits), C.POINTER(Positions), dbl, C.POINTER(Positions),
                                                   C.POINTER(Positions), C.POINTER(Positions), vp, vp]),
         "moteopt_policy_loss_workspace_size": (sz, [C.POINTER(Logits)]),

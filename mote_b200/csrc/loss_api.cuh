@@ -18,6 +18,12 @@ bool positions_fit(const moteopt_logits* z) {
   return z->tokens == 0 || z->seqs <= ((int64_t{1} << 27) - 1) / z->tokens;
 }
 
+bool shape_fits(const moteopt_logits* z) {   // for the workspace sizes
+  return z && z->seqs >= 0 && z->tokens >= 0 && z->vocab >= 1 &&
+         (z->dtype == MOTEOPT_DTYPE_F32 || z->dtype == MOTEOPT_DTYPE_BF16) && z->vocab <= kRowMost / esize(z->dtype) &&
+         positions_fit(z);
+}
+
 int check_logits(const char* who, const moteopt_logits* z, const moteopt_positions* y, Rows* R, double temperature) {
   const std::string w(who);
   if (!z || !y) return fail(MOTEOPT_ERR_INVALID, w + ": null logits or targets");
@@ -100,25 +106,34 @@ int launch_cluster(void (*kernel)(Args), const Args& A, unsigned rows, unsigned 
 
 bool short_rows(int dtype, int64_t vocab) { return vocab * esize(dtype) <= kShortBytes; }
 
-// The warps' share of short rows: as many rows as fit kTileBytes, at most kTileRows, and fewer while that would leave an SM
-// less than 24 warps (a warp takes its rows four at a time, one lot after the other).
-void tile_shape(int64_t rows, int dtype, int64_t vocab, int sms, int* per_warp, uint32_t* pitch) {
-  *pitch = static_cast<uint32_t>(((vocab * esize(dtype) + 16 - esize(dtype) + 15) / 16 + 1) * 16);
-  const int64_t most = std::min<int64_t>(kTileRows, kTileBytes / *pitch);
-  *per_warp = static_cast<int>(std::max<int64_t>(1, std::min(most, rows / (24 * sms))));
-}
-
-// Lanes per row: 8, and the whole warp where a row has more than 16 lines for each of them.
+// Tiles: as many rows as fit kTileBytes, at most kTileRows, and fewer while that would leave an SM less than 24 warps (a warp
+// takes its rows four at a time, one lot after the other). Lanes per row: 8, and the whole warp where a row has more than 16
+// lines for each of them.
 constexpr uint32_t kNarrowPitch = 8 * 16 * 16;
+struct TileShape {
+  int per_warp;
+  uint32_t pitch, tiles;
+};
+TileShape tile_shape(int64_t rows, int64_t line_bytes, int sms) {
+  TileShape s;
+  s.pitch = static_cast<uint32_t>((line_bytes / 16 + 1) * 16);
+  const int64_t most = std::min<int64_t>(kTileRows, kTileBytes / s.pitch);
+  s.per_warp = static_cast<int>(std::max<int64_t>(1, std::min(most, rows / (24 * sms))));
+  s.tiles = static_cast<uint32_t>(cdiv(rows, s.per_warp));
+  return s;
+}
+int64_t line_bytes(int dtype, int64_t vocab) { return (vocab * esize(dtype) + 16 - esize(dtype) + 15) / 16 * 16; }
+
 template <Mode kMode>
-int launch_tile(int dtype, TileArgs A, int sms, cudaStream_t st, bool after = false) {
-  tile_shape(A.R.n, dtype, A.R.vocab, sms, &A.per_warp, &A.pitch);
-  const bool bf = dtype == MOTEOPT_DTYPE_BF16, narrow = A.pitch <= kNarrowPitch;
+int launch_tile(int dtype, TileArgs A, const TileShape& s, cudaStream_t st, bool after = false) {
+  A.per_warp = s.per_warp;
+  A.pitch = s.pitch;
+  const bool bf = dtype == MOTEOPT_DTYPE_BF16, narrow = s.pitch <= kNarrowPitch;
   auto* const k = narrow ? (bf ? tile_kernel<__nv_bfloat16, 8, kMode> : tile_kernel<float, 8, kMode>)
                          : (bf ? tile_kernel<__nv_bfloat16, 32, kMode> : tile_kernel<float, 32, kMode>);
-  const size_t smem = static_cast<size_t>(kTileWarps) * A.per_warp * A.pitch;
-  const int64_t blocks = cdiv(cdiv(A.R.n, A.per_warp), kTileWarps);
-  return launch_after(k, A, static_cast<unsigned>(blocks), kTileWarps * 32, smem, st, "loss tile_kernel", !after);
+  const size_t smem = static_cast<size_t>(kTileWarps) * s.per_warp * s.pitch;
+  return launch_after(k, A, static_cast<unsigned>(cdiv(s.tiles, kTileWarps)), kTileWarps * 32, smem, st, "loss tile_kernel",
+                      !after);
 }
 
 // Long rows: blocks per row and bytes of shared memory each. A slice of up to kSliceBytes leaves three blocks an SM; a
@@ -139,18 +154,26 @@ SliceShape slice_shape(int64_t rows, int64_t vocab, int dtype, int sms) {
   return s;
 }
 
-template <bool kPolicy>
 int launch_slices(int dtype, SliceArgs A, int sms, cudaStream_t st) {
   const SliceShape s = slice_shape(A.R.n, A.R.vocab, dtype, sms);
   const bool bf = dtype == MOTEOPT_DTYPE_BF16;
   A.cl = s.cl;
-  auto* const k = s.threads == 128 ? (bf ? slice_kernel<__nv_bfloat16, 128, kPolicy> : slice_kernel<float, 128, kPolicy>)
-                                   : (bf ? slice_kernel<__nv_bfloat16, 256, kPolicy> : slice_kernel<float, 256, kPolicy>);
+  auto* const k = s.threads == 128 ? (bf ? slice_kernel<__nv_bfloat16, 128> : slice_kernel<float, 128>)
+                                   : (bf ? slice_kernel<__nv_bfloat16, 256> : slice_kernel<float, 256>);
   return launch_cluster(k, A, A.R.n, s.cl, s.threads, s.smem, st, "loss slice_kernel");
 }
 
-// logp, lse (or logp64, coef = 0) of every row
-int launch_forward(int dtype, const Rows& R, float* logp, float* lse, double* logp64, float* coef, int sms, cudaStream_t st) {
+// Long rows go in pieces, whose parts are kept: pieces of a row, and the bytes of all parts. 8 KB a piece; fewer bytes for
+// fewer rows would not fill the GPU's warps any better where it counts, the longest rows of a few positions.
+constexpr uint32_t kPieceLines = 512;
+int64_t row_pieces(int dtype, int64_t vocab) { return cdiv(line_bytes(dtype, vocab) / 16, kPieceLines); }
+size_t parts_bytes(int dtype, int64_t rows, int64_t vocab) {
+  return short_rows(dtype, vocab) ? 0 : sizeof(Part) * static_cast<size_t>(rows) * static_cast<size_t>(row_pieces(dtype, vocab));
+}
+
+// logp, lse (or logp64, lse, coef = 0) of every row
+int launch_forward(int dtype, const Rows& R, float* logp, float* lse, double* logp64, float* coef, Part* parts, int sms,
+                   cudaStream_t st) {
   if (short_rows(dtype, R.vocab)) {
     TileArgs A;
     std::memset(&A, 0, sizeof(A));
@@ -159,16 +182,33 @@ int launch_forward(int dtype, const Rows& R, float* logp, float* lse, double* lo
     A.lse = lse;
     A.logp64 = logp64;
     A.coef = coef;
-    return launch_tile<kForward>(dtype, A, sms, st);
+    return launch_tile<kForward>(dtype, A, tile_shape(R.n, line_bytes(dtype, R.vocab), sms), st);
   }
-  SliceArgs A;
+  const int64_t pieces = row_pieces(dtype, R.vocab);
+  if (R.n * pieces >= (int64_t{1} << 31)) return fail(MOTEOPT_ERR_LIMIT, "losses: too many logits for one call");
+  StreamArgs A;
   std::memset(&A, 0, sizeof(A));
   A.R = R;
-  A.logp = logp;
-  A.lse = lse;
-  A.logp64 = logp64;
-  A.coef = coef;
-  return launch_slices<false>(dtype, A, sms, st);
+  A.pieces = static_cast<uint32_t>(pieces);
+  A.n = R.n * A.pieces;
+  A.lines = kPieceLines;
+  A.parts = parts;
+  const unsigned blocks = static_cast<unsigned>(std::min<int64_t>(cdiv(A.n, kStreamThreads / 32), kStreamBlocks * sms));
+  MO_TRY(dtype == MOTEOPT_DTYPE_BF16
+             ? launch_after(stream_kernel<__nv_bfloat16>, A, blocks, kStreamThreads, 0, st, "loss stream_kernel", true)
+             : launch_after(stream_kernel<float>, A, blocks, kStreamThreads, 0, st, "loss stream_kernel", true));
+  JoinArgs J;
+  std::memset(&J, 0, sizeof(J));
+  J.R = R;
+  J.pieces = A.pieces;
+  J.parts = parts;
+  J.logp = logp;
+  J.lse = lse;
+  J.logp64 = logp64;
+  J.coef = coef;
+  const unsigned grid = static_cast<unsigned>(cdiv(R.n, kJoinThreads / 32));
+  return dtype == MOTEOPT_DTYPE_BF16 ? launch_after(join_kernel<__nv_bfloat16>, J, grid, kJoinThreads, 0, st, "loss join_kernel")
+                                     : launch_after(join_kernel<float>, J, grid, kJoinThreads, 0, st, "loss join_kernel");
 }
 
 int launch_gradient(int dtype, const Rows& R, const Kept& K, void* grad, int sms, cudaStream_t st, bool after) {
@@ -178,7 +218,7 @@ int launch_gradient(int dtype, const Rows& R, const Kept& K, void* grad, int sms
     A.R = R;
     A.K = K;
     A.grad = grad;
-    return launch_tile<kGradient>(dtype, A, sms, st, after);
+    return launch_tile<kGradient>(dtype, A, tile_shape(R.n, line_bytes(dtype, R.vocab), sms), st, after);
   }
   GradArgs A;
   std::memset(&A, 0, sizeof(A));
@@ -220,21 +260,37 @@ int launch_sums(const double* partials, int64_t n, double* mid, float* out, cuda
 }
 
 struct PreferenceLayout {
-  size_t logp64, lse, coef, pairs, bytes;
+  size_t logp64, lse, coef, pairs, parts, bytes;
 };
-PreferenceLayout preference_layout(int64_t n, int64_t pairs) {
+PreferenceLayout preference_layout(int dtype, int64_t n, int64_t vocab, int64_t pairs) {
   PreferenceLayout L;
   L.logp64 = kHeaderBytes;
   L.lse = align_up(L.logp64 + 8 * static_cast<size_t>(n), 256);
   L.coef = align_up(L.lse + 4 * static_cast<size_t>(n), 256);
   L.pairs = align_up(L.coef + 4 * static_cast<size_t>(n), 256);
-  L.bytes = align_up(L.pairs + 8 * static_cast<size_t>(pairs), 256);
+  L.parts = align_up(L.pairs + 8 * static_cast<size_t>(pairs), 256);
+  L.bytes = align_up(L.parts + parts_bytes(dtype, n, vocab), 256);
   return L;
 }
 
 int check_divisor(const char* who, double divisor, const float* divisor_device) {
   if (!divisor_device && (!(divisor != 0.0) || !std::isfinite(divisor)))
     return fail(MOTEOPT_ERR_INVALID, std::string(who) + ": the divisor must be finite and not 0");
+  return MOTEOPT_OK;
+}
+
+template <typename K>
+int allow_smem(K* kernel, int bytes) {
+  MO_CUDA(cudaFuncSetAttribute(reinterpret_cast<const void*>(kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  return MOTEOPT_OK;
+}
+template <typename T>
+int kernel_setup() {
+  MO_TRY(allow_smem(slice_kernel<T, 128>, static_cast<int>(kSliceMost)));
+  MO_TRY(allow_smem(slice_kernel<T, 256>, static_cast<int>(kSliceMost)));
+  const void* const wide[] = {reinterpret_cast<const void*>(slice_kernel<T, 128>),
+                              reinterpret_cast<const void*>(slice_kernel<T, 256>)};
+  for (const void* k : wide) MO_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
   return MOTEOPT_OK;
 }
 
@@ -245,19 +301,8 @@ int loss_setup(int* sms) {
   int dev = 0;
   MO_CUDA(cudaGetDevice(&dev));
   if (ready.load(std::memory_order_acquire) >> dev & 1) return MOTEOPT_OK;
-  const void* const kernels[] = {
-      reinterpret_cast<const void*>(slice_kernel<__nv_bfloat16, 128, false>),
-      reinterpret_cast<const void*>(slice_kernel<__nv_bfloat16, 128, true>),
-      reinterpret_cast<const void*>(slice_kernel<__nv_bfloat16, 256, false>),
-      reinterpret_cast<const void*>(slice_kernel<__nv_bfloat16, 256, true>),
-      reinterpret_cast<const void*>(slice_kernel<float, 128, false>),
-      reinterpret_cast<const void*>(slice_kernel<float, 128, true>),
-      reinterpret_cast<const void*>(slice_kernel<float, 256, false>),
-      reinterpret_cast<const void*>(slice_kernel<float, 256, true>)};
-  for (const void* k : kernels) {
-    MO_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
-    MO_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kSliceMost)));
-  }
+  MO_TRY(kernel_setup<__nv_bfloat16>());
+  MO_TRY(kernel_setup<float>());
   ready.fetch_or(1ull << dev, std::memory_order_release);
   return MOTEOPT_OK;
 }
@@ -266,15 +311,26 @@ int loss_setup(int* sms) {
 
 extern "C" {
 
+size_t moteopt_token_logprobs_workspace_size(const moteopt_logits* logits) {
+  if (!shape_fits(logits)) return 0;
+  return align_up(kHeaderBytes + parts_bytes(logits->dtype, logits->seqs * logits->tokens, logits->vocab), 256);
+}
+
 int moteopt_token_logprobs(const moteopt_logits* logits, const moteopt_positions* targets, double temperature,
-                           float* logprobs, float* lse, moteopt_stream_t stream) {
+                           float* logprobs, float* lse, void* workspace, size_t workspace_bytes, moteopt_stream_t stream) {
   Rows R;
   MO_TRY(check_logits("moteopt_token_logprobs", logits, targets, &R, temperature));
   if (R.n == 0) return MOTEOPT_OK;
   if (!logprobs) return fail(MOTEOPT_ERR_INVALID, "moteopt_token_logprobs: null output");
+  Part* parts = nullptr;
+  if (!short_rows(logits->dtype, R.vocab)) {
+    MO_TRY(check_ws(workspace, workspace_bytes, moteopt_token_logprobs_workspace_size(logits)));
+    parts = reinterpret_cast<Part*>(static_cast<char*>(workspace) + kHeaderBytes);
+  }
   int sms = 0;
   MO_TRY(loss_setup(&sms));
-  return launch_forward(logits->dtype, R, logprobs, lse, nullptr, nullptr, sms, reinterpret_cast<cudaStream_t>(stream));
+  return launch_forward(logits->dtype, R, logprobs, lse, nullptr, nullptr, parts, sms,
+                        reinterpret_cast<cudaStream_t>(stream));
 }
 
 int moteopt_token_logprobs_backward(const moteopt_logits* logits, const moteopt_positions* targets, double temperature,
@@ -296,9 +352,7 @@ int moteopt_token_logprobs_backward(const moteopt_logits* logits, const moteopt_
 }
 
 size_t moteopt_policy_loss_workspace_size(const moteopt_logits* logits) {
-  if (!logits || logits->seqs < 0 || logits->tokens < 0 || logits->vocab < 1 ||
-      (logits->dtype != MOTEOPT_DTYPE_F32 && logits->dtype != MOTEOPT_DTYPE_BF16) || !positions_fit(logits))
-    return 0;
+  if (!shape_fits(logits)) return 0;
   return policy_layout(logits->seqs * logits->tokens).bytes;
 }
 
@@ -347,9 +401,9 @@ int moteopt_policy_loss(const moteopt_logits* logits, const moteopt_positions* t
     A.logp = logprobs;
     A.grad = grad_logits;
     A.partials = partials;
-    MO_TRY(launch_tile<kPolicyLoss>(logits->dtype, A, sms, st));
-    tile_shape(R.n, logits->dtype, R.vocab, sms, &A.per_warp, &A.pitch);
-    return launch_sums(partials, cdiv(R.n, A.per_warp), mid, sums, st);
+    const TileShape s = tile_shape(R.n, line_bytes(logits->dtype, R.vocab), sms);
+    MO_TRY(launch_tile<kPolicyLoss>(logits->dtype, A, s, st));
+    return launch_sums(partials, s.tiles, mid, sums, st);
   }
   SliceArgs A;
   std::memset(&A, 0, sizeof(A));
@@ -358,13 +412,13 @@ int moteopt_policy_loss(const moteopt_logits* logits, const moteopt_positions* t
   A.logp = logprobs;
   A.grad = grad_logits;
   A.partials = partials;
-  MO_TRY(launch_slices<true>(logits->dtype, A, sms, st));
+  MO_TRY(launch_slices(logits->dtype, A, sms, st));
   return launch_sums(partials, R.n, mid, sums, st);
 }
 
 size_t moteopt_preference_loss_workspace_size(const moteopt_logits* logits, int64_t sequences) {
-  if (!logits || logits->seqs < 0 || logits->tokens < 0 || sequences < 0 || !positions_fit(logits)) return 0;
-  return preference_layout(logits->seqs * logits->tokens, sequences / 2).bytes;
+  if (!shape_fits(logits) || sequences < 0) return 0;
+  return preference_layout(logits->dtype, logits->seqs * logits->tokens, logits->vocab, sequences / 2).bytes;
 }
 
 int moteopt_preference_loss(const moteopt_logits* logits, const moteopt_positions* targets,
@@ -384,7 +438,7 @@ int moteopt_preference_loss(const moteopt_logits* logits, const moteopt_position
   if (!std::isfinite(p.beta) || !(p.label_smoothing >= 0.0 && p.label_smoothing <= 1.0))
     return fail(MOTEOPT_ERR_INVALID, "moteopt_preference_loss: beta must be finite, label_smoothing in [0, 1]");
   if (p.sequences > 0 && (!rewards || !logprobs)) return fail(MOTEOPT_ERR_INVALID, "moteopt_preference_loss: null pointer");
-  const PreferenceLayout L = preference_layout(R.n, p.sequences / 2);
+  const PreferenceLayout L = preference_layout(logits->dtype, R.n, R.vocab, p.sequences / 2);
   MO_TRY(check_ws(workspace, workspace_bytes, L.bytes));
   int sms = 0;
   MO_TRY(loss_setup(&sms));
@@ -402,7 +456,8 @@ int moteopt_preference_loss(const moteopt_logits* logits, const moteopt_position
   double* const pair_loss = reinterpret_cast<double*>(ws + L.pairs);
   R.cu = p.cu_seqlens;
   R.n_seqs = static_cast<int>(p.sequences);
-  if (R.n > 0) MO_TRY(launch_forward(logits->dtype, R, nullptr, lse, logp64, coef, sms, st));
+  if (R.n > 0)
+    MO_TRY(launch_forward(logits->dtype, R, nullptr, lse, logp64, coef, reinterpret_cast<Part*>(ws + L.parts), sms, st));
   PairArgs A;
   std::memset(&A, 0, sizeof(A));
   A.R = R;

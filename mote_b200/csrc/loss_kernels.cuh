@@ -44,7 +44,7 @@ struct Rows {
   uint32_t vocab;
   const int32_t* cu;      // packed: n_seqs + 1 row offsets, or null. Rows outside [cu[0], cu[n_seqs]) do not count
   int n_seqs;
-  float c_hi, c_lo;       // log2(e) / T as two floats, c_lo > 0 (see ex2_of)
+  float c_hi, c_lo;       // log2(e) / T as two floats, c_lo > 0 (see Ex)
   double t, inv_t;        // T and 1 / T
 };
 
@@ -61,8 +61,6 @@ struct Policy {
   const float* div;                  // or the divisor on the device
 };
 
-// 2^((z - m) c) for z <= m, c = c_hi + c_lo. One rounding of the whole product: log2(e) rounded to one float is a relative
-// error of 1.3e-8 in every exponent, which the same sums would carry. c_lo > 0 keeps -inf a -inf.
 __device__ __forceinline__ float ex2(float t) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(t));
@@ -92,20 +90,34 @@ __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
   return r;
 }
 
-struct Ex {               // the constants of one row's exponentials, two at a time
-  uint64_t neg_m, hi, lo;
-  __device__ Ex(float m, float c_hi, float c_lo) : neg_m(pack2(-m, -m)), hi(pack2(c_hi, c_hi)), lo(pack2(c_lo, c_lo)) {}
+// The exponentials of a row about a logit m, two at a time: exp((z - m) / T) = 2^(z c - b) fix with c = c_hi + c_lo =
+// log2(e) / T, b = m c rounded to fp32 and fix = 2^(b - m c). Two multiply-adds: z c_hi - b is exact before its one rounding,
+// which is of the size of the result, and so is the next. (With one float for c, its rounding, 1.3e-8 of log2(e), would lean
+// every exponent of a row the same way.) c_lo > 0 keeps -inf a -inf. Beyond |m| = 2^60, where a product may overflow, any
+// two different logits are at least 2^37 apart: a scale of 2^-20 gives 1 for z = m and 0 below.
+struct Ex {
+  uint64_t hi, lo, nb;
+  float fix;
+  __device__ Ex(float m, const Rows& R) {
+    const bool far = fabsf(m) > 0x1p60f && fabsf(m) < INFINITY;
+    if (m == kNegInf) m = 0.f;
+    const float h = far ? 0x1p-20f : R.c_hi, l = far ? 0x1p-149f : R.c_lo, b = m * h;
+    fix = far ? 1.f : fmaf(-(fmaf(m, h, -b) + m * l), 0.69314718f, 1.f);
+    hi = pack2(h, h);
+    lo = pack2(l, l);
+    nb = pack2(-b, -b);
+  }
   __device__ __forceinline__ uint64_t two(uint64_t z) const {
-    const uint64_t d = add2(z, neg_m);
     float t0, t1;
-    unpack2(fma2(d, hi, mul2(d, lo)), t0, t1);
+    unpack2(fma2(z, lo, fma2(z, hi, nb)), t0, t1);
     return pack2(ex2(t0), ex2(t1));
   }
+  __device__ __forceinline__ float one(float z) const {
+    float e0, e1;
+    unpack2(two(pack2(z, z)), e0, e1);
+    return e0;
+  }
 };
-__device__ __forceinline__ float ex_one(float z, float m, float c_hi, float c_lo) {
-  const float d = z - m;
-  return ex2(fmaf(d, c_hi, d * c_lo));
-}
 // exp((m - to) / T), the factor of a partial sum that moves to another maximum: once a thread, by expf
 __device__ __forceinline__ float rescale(float m, float to, float inv_t) { return m == kNegInf ? 0.f : expf((m - to) * inv_t); }
 
@@ -428,18 +440,21 @@ __device__ __forceinline__ void sum_pairs(const Kept& K) {   // one warp, in a f
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
-// Short rows: a warp takes `per_warp` rows. Their 16-byte lines come into shared memory by cp.async (a line may hold up to
-// 15 bytes beside the row: the same aligned line, so nothing beyond the allocation), which lifts every alignment and stride
-// question and keeps all of a warp's rows in flight at once. kG lanes work on a row in lines of 16 bytes, 32 / kG rows at a
-// time: the quarter of a warp that shared memory serves at once reads 128 bytes in a row whatever the rows' pitch, and the
-// maximum and the sum take 3 shuffles for four rows. One lane per row forms the row's values (a warp that formed them for one
-// row at a time would spend as much on them as on the row). Then, for the gradient, the exponentials again from
-// shared memory, by the lines of the output.
+// Rows a warp can hold: a warp takes a tile of `per_warp` rows. Their 16-byte lines come into shared memory by cp.async (a
+// line may hold up to 15 bytes beside the row: the same aligned line, so nothing beyond the allocation), which lifts every
+// alignment and stride question and keeps all of a tile in flight at once. kG lanes work on a row in lines of 16 bytes,
+// 32 / kG rows at a time: the quarter of a warp that shared memory serves at once reads 128 bytes in a row whatever the rows'
+// pitch, and the maximum and the sum take 3 shuffles for four rows. One lane per row forms the row's values (a warp that
+// formed them for one row at a time would spend as much on them as on the row). Then, for the gradient, the exponentials
+// again from shared memory, by the lines of the output.
+//
+// Many warps, each with one tile, and not few with the next tile already on its way: a warp waits on its own arithmetic more
+// than on memory (with two buffers for half the warps, 16 x 1024 x 4096: policy loss 78 against 57 us).
 constexpr int kTileWarps = 4;
-constexpr int kTileRows = 8;           // most rows of a warp: 64 x 1024 x 271 bf16, forward, at 4, 8 and 16 rows: 16.2, 14.5
+constexpr int kTileRows = 8;           // most rows of a tile: 64 x 1024 x 271 bf16, forward, at 4, 8 and 16 rows: 16.2, 14.5
                                        // and 18.2 us (fewer rows: more of a warp's instructions are not its rows'; more: too
                                        // few warps an SM), policy loss 31.7, 27.5 and 31.2 us
-constexpr int kTileBytes = 9216;       // most bytes of a warp's rows: 6 blocks of 4 warps in an SM's shared memory
+constexpr int kTileBytes = 9216;       // most bytes of a tile: 6 blocks of 4 warps in an SM's shared memory
 enum Mode { kForward, kPolicyLoss, kGradient };
 
 struct TileArgs {
@@ -478,9 +493,9 @@ __global__ void __launch_bounds__(kTileWarps * 32) tile_kernel(const __grid_cons
   constexpr int kAtOnce = 32 / kG;
   const Rows& R = A.R;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gl = lane % kG, group = lane / kG;
+  if (kMode != kGradient) pdl_go();
   const uint32_t tile = blockIdx.x * kTileWarps + warp;
   const uint32_t first = tile * static_cast<uint32_t>(A.per_warp);
-  if (kMode != kGradient) pdl_go();
   if (first >= R.n) return;
   const int rows = static_cast<int>(min(static_cast<uint32_t>(A.per_warp), R.n - first));
   unsigned char* const base = sm + static_cast<size_t>(warp) * A.per_warp * A.pitch;
@@ -514,6 +529,10 @@ __global__ void __launch_bounds__(kTileWarps * 32) tile_kernel(const __grid_cons
       asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + v * 16), "l"(a + v * 16) : "memory");
   }
   asm volatile("cp.async.commit_group;" ::: "memory");
+  if (kMode == kGradient) {
+    pdl_wait();   // the logits and targets are inputs; the rows' coefficients may come from the launch before
+    if (A.K.pair_loss && tile == 0) sum_pairs(A.K);
+  }
   float adv = 0.f, old_lp = 0.f, ref_lp = 0.f;
   if (kMode == kPolicyLoss && live) {
     adv = A.P.adv.at(seq, tok);
@@ -523,12 +542,9 @@ __global__ void __launch_bounds__(kTileWarps * 32) tile_kernel(const __grid_cons
   // lane r: the row's values; d_j = 2^((z_j - m) c) f, gy at the target
   float m_mine = kNegInf, s_mine = 0.f, f = 0.f, gy = 0.f;
   if (kMode == kGradient) {
-    pdl_wait();   // the rows are inputs; their coefficients may come from the launch before
-    if (A.K.pair_loss && tile == 0) sum_pairs(A.K);
     float coef = 0.f;
     if (live) coef = kept_coef(A.K, first + lane, seq, tok);
     live = live && coef != 0.f;
-    live_rows = __ballot_sync(0xffffffffu, live);
     if (live) {
       const KeptRow k = kept_row(A.K, R, first + lane, seq, tok, coef);
       m_mine = k.m;
@@ -536,6 +552,7 @@ __global__ void __launch_bounds__(kTileWarps * 32) tile_kernel(const __grid_cons
       gy = k.gy;
     }
   }
+  if (kMode == kGradient) live_rows = __ballot_sync(0xffffffffu, live);
   asm volatile("cp.async.wait_group 0;" ::: "memory");
   __syncwarp();
 
@@ -544,9 +561,9 @@ __global__ void __launch_bounds__(kTileWarps * 32) tile_kernel(const __grid_cons
   float zy = NAN;
   if (live) {
     if (has_y) {
-      const uint32_t at = skew + y;
-      zy = load_one(reinterpret_cast<const T*>(mine) + at);
-      reinterpret_cast<T*>(mine)[at] = static_cast<T>(kNegInf);
+      const uint32_t k = skew + y;
+      zy = load_one(reinterpret_cast<const T*>(mine) + k);
+      reinterpret_cast<T*>(mine)[k] = static_cast<T>(kNegInf);
     }
     if (kMode != kGradient) {
       if (skew != 0) keep<T>(mine[0], skew, kPer);
@@ -565,7 +582,7 @@ __global__ void __launch_bounds__(kTileWarps * 32) tile_kernel(const __grid_cons
 #pragma unroll 4
       for (uint32_t l = gl; l < nl; l += kG) top = vec_max<T>(top, row[l]);
       const float m = group_max<kG>(W::top(top));
-      const Ex ex(m == kNegInf ? 0.f : m, R.c_hi, R.c_lo);
+      const Ex ex(m, R);
       uint64_t acc = 0;
 #pragma unroll 4
       for (uint32_t l = gl; l < nl; l += kG) {
@@ -575,7 +592,7 @@ __global__ void __launch_bounds__(kTileWarps * 32) tile_kernel(const __grid_cons
       }
       float s0, s1;
       unpack2(acc, s0, s1);
-      const float s = group_sum<kG>(s0 + s1);
+      const float s = group_sum<kG>(s0 + s1) * ex.fix;
       const int from = ((lane - r0) & (kAtOnce - 1)) * kG;
       const float mr = __shfl_sync(0xffffffffu, m, from), sr = __shfl_sync(0xffffffffu, s, from);
       if (lane >= r0 && lane < r0 + kAtOnce) {
@@ -608,71 +625,236 @@ __global__ void __launch_bounds__(kTileWarps * 32) tile_kernel(const __grid_cons
         A.coef[row] = 0.f;
       }
     }
-    if (kMode == kForward) return;
+    if (kMode == kPolicyLoss) {
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const double v = warp_sum(part[k]);
-      if (lane == k) A.partials[static_cast<size_t>(tile) * 4 + k] = v;
+      for (int k = 0; k < 4; ++k) {
+        const double v = warp_sum(part[k]);
+        if (lane == k) A.partials[static_cast<size_t>(tile) * 4 + k] = v;
+      }
     }
-    if (A.grad == nullptr) return;
-    if (m_mine == kNegInf) m_mine = 0.f;
   }
 
-  for (int r0 = 0; r0 < rows; r0 += kAtOnce) {
-    const int r = r0 + group;
-    const float m = __shfl_sync(0xffffffffu, m_mine, r & 31), k = __shfl_sync(0xffffffffu, f, r & 31);
-    const uint32_t sk = __shfl_sync(0xffffffffu, skew, r & 31);
-    if (r >= rows) continue;
-    T* const out = static_cast<T*>(A.grad) + static_cast<size_t>(first + r) * R.vocab;
-    const Split<T> so(out, R.vocab);
-    uint4* const ov = reinterpret_cast<uint4*>(out + so.head);
-    const unsigned char* const row = base + static_cast<size_t>(r) * A.pitch;
-    if (!(live_rows >> r & 1)) {
-      for (uint32_t l = gl; l < so.vecs; l += kG) ov[l] = make_uint4(0, 0, 0, 0);
-      for (uint32_t i = gl; i < so.head + so.tail; i += kG) store_one(out + so.edge(i), 0.f);
-      continue;
-    }
-    const Ex ex(m, R.c_hi, R.c_lo);
-    const uint64_t k2 = pack2(k, k);
-    const uint32_t shift = (sk + so.head) * sizeof(T);
+  if (kMode == kGradient || (kMode == kPolicyLoss && A.grad != nullptr)) {
+    for (int r0 = 0; r0 < rows; r0 += kAtOnce) {
+      const int r = r0 + group;
+      const float m = __shfl_sync(0xffffffffu, m_mine, r & 31), k = __shfl_sync(0xffffffffu, f, r & 31);
+      const uint32_t sk = __shfl_sync(0xffffffffu, skew, r & 31);
+      if (r >= rows) continue;
+      T* const out = static_cast<T*>(A.grad) + static_cast<size_t>(first + r) * R.vocab;
+      const Split<T> so(out, R.vocab);
+      uint4* const ov = reinterpret_cast<uint4*>(out + so.head);
+      const unsigned char* const row = base + static_cast<size_t>(r) * A.pitch;
+      if (!(live_rows >> r & 1)) {
+        for (uint32_t l = gl; l < so.vecs; l += kG) ov[l] = make_uint4(0, 0, 0, 0);
+        for (uint32_t i = gl; i < so.head + so.tail; i += kG) store_one(out + so.edge(i), 0.f);
+        continue;
+      }
+      const Ex ex(m, R);
+      const float kf = k * ex.fix;
+      const uint64_t k2 = pack2(kf, kf);
+      const uint32_t shift = (sk + so.head) * sizeof(T);
 #pragma unroll 2
-    for (uint32_t l = gl; l < so.vecs; l += kG) {
-      Pairs<T> q(load_shifted(row, l * 16 + shift));
+      for (uint32_t l = gl; l < so.vecs; l += kG) {
+        Pairs<T> q(load_shifted(row, l * 16 + shift));
 #pragma unroll
-      for (int u = 0; u < Pairs<T>::kN; ++u) q.p[u] = mul2(ex.two(q.p[u]), k2);
-      ov[l] = q.line();
+        for (int u = 0; u < Pairs<T>::kN; ++u) q.p[u] = mul2(ex.two(q.p[u]), k2);
+        ov[l] = q.line();
+      }
+      for (uint32_t i = gl; i < so.head + so.tail; i += kG) {
+        const uint32_t j = so.edge(i);
+        store_one(out + j, ex.one(load_one(reinterpret_cast<const T*>(row) + sk + j)) * kf);
+      }
     }
-    for (uint32_t i = gl; i < so.head + so.tail; i += kG) {
-      const uint32_t j = so.edge(i);
-      store_one(out + j, ex_one(load_one(reinterpret_cast<const T*>(row) + sk + j), m, R.c_hi, R.c_lo) * k);
-    }
+    __syncwarp();   // the targets' elements, written as 0 above
+    if (live && has_y) store_one(static_cast<T*>(A.grad) + static_cast<size_t>(first + lane) * R.vocab + y, gy);
   }
-  __syncwarp();   // the targets' elements, written as 0 above
-  if (live && has_y) store_one(static_cast<T*>(A.grad) + static_cast<size_t>(first + lane) * R.vocab + y, gy);
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
-// Long rows: a row per block, or per cluster of blocks that take a slice each. A slice's 16-byte lines come into shared
-// memory at once by cp.async, so a block has all its bytes in flight and several blocks of an SM are at different stages:
-// each row is read once, however often the kernel goes over it. Every thread masks, maximises and sums the lines that it
-// loaded itself; the blocks' parts meet in distributed shared memory; for the policy loss one thread forms the row's
-// values, and all go over the slice again for the gradient, by the lines of the output.
+// Long rows, forward only: a stream of pieces of `lines` lines, a warp each, straight into registers: 4 lines a lane at a
+// time, the next 4 (of this piece or of the warp's next one) on their way meanwhile. A lane's maximum moves only when a logit
+// is more than kSlack units of log2 above it, so its sum is rescaled hardly ever. join_kernel puts a row's parts together.
+struct StreamArgs {
+  Rows R;
+  uint32_t pieces;      // of a row
+  uint32_t n;           // pieces in all
+  uint32_t lines;       // of a piece: a multiple of 128
+  Part* parts;          // [n]
+};
+constexpr int kStreamThreads = 128, kStreamBlocks = 8, kBatch = 4;
+constexpr float kSlack = 16.f;
+
+// One batch of a lane's lines: where, and what of it counts
+struct Batch {
+  const uint4* p;       // the warp's first line
+  uint32_t left;        // lines from there to the piece's end (0: nothing)
+  uint32_t skew;        // elements of the first line in front of the row
+  uint32_t elems;       // elements from the first line's begin to the row's end
+  uint32_t y;           // the target, in elements from the first line's begin (or beyond)
+};
+
+template <typename T>
+__global__ void __launch_bounds__(kStreamThreads, kStreamBlocks) stream_kernel(const __grid_constant__ StreamArgs A) {
+  using W = Word<T>;
+  constexpr uint32_t kPer = 16 / sizeof(T);
+  const Rows& R = A.R;
+  const uint32_t lane = threadIdx.x & 31, step = gridDim.x * (kStreamThreads / 32);
+  const float inv_t = static_cast<float>(R.inv_t);
+  uint32_t piece = blockIdx.x * (kStreamThreads / 32) + (threadIdx.x >> 5);
+  pdl_go();
+  if (piece >= A.n) return;
+
+  const auto begin = [&](uint32_t k) {
+    Batch b = {nullptr, 0, 0, 0, 0xffffffffu};
+    if (k >= A.n) return b;
+    const uint32_t row = k / A.pieces, from = (k - row * A.pieces) * A.lines;
+    const uint32_t seq = row / R.tokens, tok = row - seq * R.tokens;
+    const int64_t y = in_packed(R, row) ? R.y[seq * R.y_seq + tok * R.y_tok] : -1;
+    if (y < 0) return b;
+    const uint64_t a = reinterpret_cast<uint64_t>(R.z) + (seq * R.z_seq + tok * R.z_tok) * sizeof(T);
+    const uint32_t skew = static_cast<uint32_t>(a & 15) / sizeof(T), lines = (skew + R.vocab + kPer - 1) / kPer;
+    if (from >= lines) return b;
+    b.p = reinterpret_cast<const uint4*>(a & ~15ull) + from;
+    b.left = min(A.lines, lines - from);
+    b.skew = from == 0 ? skew : 0;
+    b.elems = skew + R.vocab - from * kPer;
+    b.y = y < static_cast<int64_t>(R.vocab) ? skew + static_cast<uint32_t>(y) - from * kPer : 0xffffffffu;   // wraps in front
+    return b;
+  };
+  const auto load = [&](uint4 (&v)[kBatch], const Batch& b) {
+#pragma unroll
+    for (uint32_t k = 0; k < kBatch; ++k) {
+      v[k] = make_uint4(W::kEmpty, W::kEmpty, W::kEmpty, W::kEmpty);
+      if (lane + 32 * k < b.left) v[k] = load_vec(b.p + lane + 32 * k);
+    }
+  };
+
+  Batch cur = begin(piece);
+  uint4 v[kBatch];
+  load(v, cur);
+  float m = kNegInf;
+  Ex ex(m, R);
+  uint64_t acc = 0;
+  while (true) {
+    // what comes next: this piece's next batch, or the next piece
+    constexpr uint32_t kLines = 32 * kBatch, kElems = kLines * kPer;
+    const bool ends = cur.left <= kLines;
+    Batch next;
+    if (ends) {
+      next = begin(piece + step);
+    } else {
+      next = Batch{cur.p + kLines, cur.left - kLines, 0, cur.elems - kElems, cur.y - kElems};
+    }
+    uint4 w[kBatch];
+    load(w, next);
+    if (cur.skew != 0 || cur.elems < kElems || cur.y < kElems) {   // a batch with an edge or the target in it
+#pragma unroll
+      for (uint32_t k = 0; k < kBatch; ++k) {
+        const uint32_t line = lane + 32 * k, e = line * kPer;
+        if (line >= cur.left) continue;
+        const uint32_t from = line == 0 ? cur.skew : 0;
+        keep<T>(v[k], from, min(kPer, cur.elems - e) - from);
+        if (cur.y - e < kPer) drop_target<T>(v[k], cur.y - e);
+      }
+    }
+    uint32_t t = W::kEmpty;
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) t = vec_max<T>(t, v[k]);
+    const float top = W::top(t);
+    if ((top - m) * R.c_hi > kSlack || (m == kNegInf && top > m)) {
+      const float by = ex.fix * rescale(m, top, inv_t);
+      acc = mul2(acc, pack2(by, by));
+      m = top;
+      ex = Ex(m, R);
+    }
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) {
+      const Pairs<T> q(v[k]);
+#pragma unroll
+      for (int u = 0; u < Pairs<T>::kN; ++u) acc = add2(acc, ex.two(q.p[u]));
+    }
+    if (ends) {
+      float s0, s1;
+      unpack2(acc, s0, s1);
+      const Part p = warp_join(Part{m, (s0 + s1) * ex.fix}, inv_t);
+      if (lane == 0) A.parts[piece] = p;
+      piece += step;
+      if (piece >= A.n) return;
+      m = kNegInf;
+      acc = 0;
+    }
+    cur = next;
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) v[k] = w[k];
+  }
+}
+
+// Rows from their pieces' parts, a warp each
+struct JoinArgs {
+  Rows R;
+  uint32_t pieces;
+  const Part* parts;
+  float* logp;
+  float* lse;
+  double* logp64;
+  float* coef;
+};
+constexpr int kJoinThreads = 128;
+template <typename T>
+__global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constant__ JoinArgs A) {
+  const Rows& R = A.R;
+  const int lane = threadIdx.x & 31;
+  const uint32_t row = blockIdx.x * (kJoinThreads / 32) + (threadIdx.x >> 5);
+  pdl_go();
+  if (row >= R.n) return;
+  const uint32_t seq = row / R.tokens, tok = row - seq * R.tokens;
+  const int64_t y = in_packed(R, row) ? R.y[seq * R.y_seq + tok * R.y_tok] : -1;
+  float zy = NAN;
+  if (y >= 0 && y < static_cast<int64_t>(R.vocab))
+    zy = load_one(reinterpret_cast<const T*>(R.z) + (seq * R.z_seq + tok * R.z_tok) + y);
+  const float inv_t = static_cast<float>(R.inv_t);
+  pdl_wait();
+  RowStat st = {0.0, 0.0, 0.f, 0.f};
+  if (y >= 0) {
+    Part p = {kNegInf, 0.f};
+    for (uint32_t i = lane; i < A.pieces; i += 32) {
+      const Part q = A.parts[static_cast<size_t>(row) * A.pieces + i];
+      const float M = fmaxf(p.m, q.m);
+      p.s = (p.s == 0.f ? 0.f : p.s * rescale(p.m, M, inv_t)) + (q.s == 0.f ? 0.f : q.s * rescale(q.m, M, inv_t));
+      p.m = M;
+    }
+    p = warp_join(p, inv_t);
+    st = row_stat(zy, p.m, p.s, R.inv_t);
+  }
+  if (lane == 0) {
+    if (A.logp) A.logp[row] = static_cast<float>(st.logp);
+    if (A.lse) A.lse[row] = static_cast<float>(st.lse);
+    if (A.logp64) {
+      A.logp64[row] = st.logp;
+      A.coef[row] = 0.f;
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+// Long rows, the policy loss: a row per block, or per cluster of blocks that take a slice each. A slice's 16-byte lines come
+// into shared memory at once by cp.async, so a block has all its bytes in flight and several blocks of an SM are at different
+// stages: each row is read once, however often the kernel goes over it. Every thread masks, maximises and sums the lines that
+// it loaded itself; the blocks' parts meet in distributed shared memory; one thread forms the row's values, and all go over
+// the slice again for the gradient, by the lines of the output.
 //
-// Exponentials again instead of kept ones: 32 fp32 exponentials a thread in registers left two blocks of 512 threads an SM, whose
-// chain of load, cluster exchange and row values then stands between them (8192 rows of 131072: 1497 us).
+// Exponentials again instead of kept ones: 32 fp32 exponentials a thread in registers left two blocks of 512 threads an SM,
+// whose chain of load, cluster exchange and row values then stands between them (8192 rows of 131072: 1497 us).
 struct SliceArgs {
   Rows R;
   int cl;               // blocks per row
-  float* logp;          // [n], or null
-  float* lse;           // [n], or null
-  double* logp64;       // [n] with coef [n] (preference), or null
-  float* coef;
+  float* logp;          // [n]
   Policy P;
   void* grad;           // [n][vocab], or null
-  double* partials;     // [n][4] (policy)
+  double* partials;     // [n][4]
 };
 
-template <typename T, int kThreads, bool kPolicy>
+template <typename T, int kThreads>
 __global__ void __launch_bounds__(kThreads, 1024 / kThreads) slice_kernel(const __grid_constant__ SliceArgs A) {
   extern __shared__ __align__(16) unsigned char sm[];
   using W = Word<T>;
@@ -689,7 +871,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) slice_kernel(const 
   const T* const z = reinterpret_cast<const T*>(R.z) + (seq * R.z_seq + tok * R.z_tok);
   T* const out = static_cast<T*>(A.grad) + static_cast<size_t>(row) * R.vocab;
   // the slice [e0, e1) is cut at the output's lines where there is a gradient, at the input's otherwise
-  const Split<T> so(kPolicy && A.grad ? out : z, R.vocab);
+  const Split<T> so(A.grad ? out : z, R.vocab);
   const uint32_t share = (so.vecs + A.cl - 1) / A.cl;
   const uint32_t v0 = min(rank * share, so.vecs), v1 = min(v0 + share, so.vecs);
   const bool last = rank == static_cast<uint32_t>(A.cl) - 1;
@@ -699,24 +881,15 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) slice_kernel(const 
   if (rank == 0 && threadIdx.x < so.head) je = threadIdx.x;
   if (last && threadIdx.x >= 32 && threadIdx.x < 32 + so.tail) je = so.head + so.vecs * kPer + threadIdx.x - 32;
 
-  int64_t y64 = in_packed(R, row) ? R.y[seq * R.y_seq + tok * R.y_tok] : -1;
-  if (kPolicy && A.P.weight.p && A.P.weight.at(seq, tok) == 0.f) y64 = -1;
+  int64_t y64 = R.y[seq * R.y_seq + tok * R.y_tok];
+  if (A.P.weight.p && A.P.weight.at(seq, tok) == 0.f) y64 = -1;
   if (y64 < 0) {   // the whole cluster
-    if (rank == 0 && threadIdx.x == 0) {
-      if (A.logp) A.logp[row] = 0.f;
-      if (A.lse) A.lse[row] = 0.f;
-      if (A.logp64) {
-        A.logp64[row] = 0.0;
-        A.coef[row] = 0.f;
-      }
-    }
-    if (kPolicy) {
-      if (rank == 0 && threadIdx.x < 4) A.partials[static_cast<size_t>(row) * 4 + threadIdx.x] = 0.0;
-      if (A.grad) {
-        if (je != 0xffffffffu) store_one(out + je, 0.f);
-        for (uint32_t i = v0 + threadIdx.x; i < v1; i += kThreads)
-          reinterpret_cast<uint4*>(out + so.head)[i] = make_uint4(0, 0, 0, 0);
-      }
+    if (rank == 0 && threadIdx.x == 0) A.logp[row] = 0.f;
+    if (rank == 0 && threadIdx.x < 4) A.partials[static_cast<size_t>(row) * 4 + threadIdx.x] = 0.0;
+    if (A.grad) {
+      if (je != 0xffffffffu) store_one(out + je, 0.f);
+      for (uint32_t i = v0 + threadIdx.x; i < v1; i += kThreads)
+        reinterpret_cast<uint4*>(out + so.head)[i] = make_uint4(0, 0, 0, 0);
     }
     return;
   }
@@ -737,7 +910,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) slice_kernel(const 
     float x = NAN;
     if (threadIdx.x == 0) {
       if (has_y) x = load_one(z + y);
-    } else if (kPolicy) {
+    } else {
       const Per& per = threadIdx.x == 1 ? A.P.adv : threadIdx.x == 2 ? A.P.old_lp : A.P.ref_lp;
       if (per.p) x = per.at(seq, tok);
     }
@@ -752,6 +925,7 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) slice_kernel(const 
   if (lines > 0 && threadIdx.x == (lines - 1) % kThreads) keep<T>(line[lines - 1], 0, skew + len - (lines - 1) * kPer);
   if (ty != 0xffffffffu && threadIdx.x == ty / kPer % kThreads) drop_target<T>(line[ty / kPer], ty % kPer);
   float m = kNegInf;
+  Ex ex(m, R);
   uint64_t acc = 0;
   for (uint32_t i = threadIdx.x; i < lines; i += 2 * kThreads) {   // two lines at a time under a running maximum
     const uint4 va = line[i];
@@ -759,53 +933,43 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) slice_kernel(const 
     if (i + kThreads < lines) vb = line[i + kThreads];
     const float top = W::top(vec_max<T>(vec_max<T>(W::kEmpty, va), vb));
     if (top > m) {
-      const float by = rescale(m, top, inv_t);
+      const float by = ex.fix * rescale(m, top, inv_t);
       acc = mul2(acc, pack2(by, by));
       m = top;
+      ex = Ex(m, R);
     }
-    const Ex ex(m == kNegInf ? 0.f : m, R.c_hi, R.c_lo);
     const Pairs<T> qa(va), qb(vb);
 #pragma unroll
     for (int u = 0; u < Pairs<T>::kN; ++u) acc = add2(acc, add2(ex.two(qa.p[u]), ex.two(qb.p[u])));
   }
   float s0, s1;
   unpack2(acc, s0, s1);
-  const Part p = row_join<kThreads>(Part{m, s0 + s1}, A.cl, rank, inv_t, sh_warp, sh_block);
-  if (threadIdx.x == 0 && (kPolicy || rank == 0)) {
+  const Part p = row_join<kThreads>(Part{m, (s0 + s1) * ex.fix}, A.cl, rank, inv_t, sh_warp, sh_block);
+  if (threadIdx.x == 0) {
     const RowStat st = row_stat(sh_in[0], p.m, p.s, R.inv_t);
-    if (kPolicy) {
-      const RowLoss L = policy_row_loss(st.logp, A.P, sh_in[2], sh_in[3], A.P.ref_lp.p != nullptr, sh_in[1]);
-      const double w = A.P.weight.p ? A.P.weight.at(seq, tok) : 1.f;
-      const double inv = A.P.div ? 1.0 / static_cast<double>(*A.P.div) : A.P.inv_div;
-      const float g = static_cast<float>(w * L.slope * inv * R.inv_t);
-      sh_g[0] = -g * st.f;
-      sh_g[1] = g * st.rest;
-      if (rank == 0) {
-        double* const o = A.partials + static_cast<size_t>(row) * 4;
-        o[0] = w * L.loss * inv;
-        o[1] = w;
-        o[2] = w * L.kl * inv;
-        o[3] = L.clipped ? w : 0.0;
-      }
-    }
+    const RowLoss L = policy_row_loss(st.logp, A.P, sh_in[2], sh_in[3], A.P.ref_lp.p != nullptr, sh_in[1]);
+    const double w = A.P.weight.p ? A.P.weight.at(seq, tok) : 1.f;
+    const double inv = A.P.div ? 1.0 / static_cast<double>(*A.P.div) : A.P.inv_div;
+    const float g = static_cast<float>(w * L.slope * inv * R.inv_t);
+    sh_g[0] = -g * st.f;
+    sh_g[1] = g * st.rest;
     if (rank == 0) {
-      if (A.logp) A.logp[row] = static_cast<float>(st.logp);
-      if (A.lse) A.lse[row] = static_cast<float>(st.lse);
-      if (A.logp64) {
-        A.logp64[row] = st.logp;
-        A.coef[row] = 0.f;
-      }
+      A.logp[row] = static_cast<float>(st.logp);
+      double* const o = A.partials + static_cast<size_t>(row) * 4;
+      o[0] = w * L.loss * inv;
+      o[1] = w;
+      o[2] = w * L.kl * inv;
+      o[3] = L.clipped ? w : 0.0;
     }
   }
-  if (!kPolicy || A.grad == nullptr) return;
+  if (A.grad == nullptr) return;
   __syncthreads();
-  const float f = sh_g[0], gy = sh_g[1];
-  const float M = p.m == kNegInf ? 0.f : p.m;
+  ex = Ex(p.m, R);
+  const float f = sh_g[0] * ex.fix, gy = sh_g[1];
   if (je != 0xffffffffu) {
     const T* const x = reinterpret_cast<const T*>(sm) + skew + (je - e0);
-    store_one(out + je, je == y ? gy : ex_one(load_one(x), M, R.c_hi, R.c_lo) * f);
+    store_one(out + je, je == y ? gy : ex.one(load_one(x)) * f);
   }
-  const Ex ex(M, R.c_hi, R.c_lo);
   const uint64_t f2 = pack2(f, f);
   const uint32_t shift = (skew + so.head - e0) * sizeof(T);   // from an output line's bytes to the slice's (wraps)
 #pragma unroll 2
@@ -877,10 +1041,11 @@ __global__ void __launch_bounds__(kGradThreads) grad_kernel(const __grid_constan
     return;
   }
   const KeptRow r = kept_row(A.K, R, row, seq, tok, coef);
-  const Ex ex(r.m, R.c_hi, R.c_lo);
-  const uint64_t f2 = pack2(r.f, r.f);
+  const Ex ex(r.m, R);
+  const float f = r.f * ex.fix;
+  const uint64_t f2 = pack2(f, f);
   const uint32_t y = y64 < static_cast<int64_t>(R.vocab) ? static_cast<uint32_t>(y64) : 0xffffffffu;
-  if (edge) store_one(out + je, je == y ? r.gy : ex_one(load_one(z + je), r.m, R.c_hi, R.c_lo) * r.f);
+  if (edge) store_one(out + je, je == y ? r.gy : ex.one(load_one(z + je)) * f);
 #pragma unroll
   for (int k = 0; k < kGradVecs; ++k) {
     const uint32_t at = begin + k * kGradThreads;

@@ -18,6 +18,7 @@ namespace {
 
 struct Api {
   decltype(&moteopt_last_error) last_error;
+  decltype(&moteopt_token_logprobs_workspace_size) logprobs_size;
   decltype(&moteopt_token_logprobs) token_logprobs;
   decltype(&moteopt_token_logprobs_backward) token_logprobs_backward;
   decltype(&moteopt_policy_loss_workspace_size) policy_size;
@@ -27,6 +28,8 @@ struct Api {
 } api;
 PyObject* lib_error = nullptr;   // _lib.MoteoptError
 PyObject* oom_error = nullptr;   // torch.OutOfMemoryError
+
+constexpr size_t kHeader = 256;   // a workspace of no more than its header is not needed
 
 struct Raised {};   // a Python error is set
 
@@ -159,7 +162,11 @@ PyObject* token_logprobs(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const c10::cuda::CUDAGuard guard(z.device());
     const auto f32 = z.options().dtype(at::kFloat);
     const at::Tensor logp = at::empty(y.sizes(), f32), lse = at::empty(y.sizes(), f32);
-    checked(api.token_logprobs(&L, &Y, t, logp.data_ptr<float>(), lse.data_ptr<float>(), stream_of(z)),
+    const size_t bytes = api.logprobs_size(&L);
+    at::Tensor ws;
+    if (bytes > kHeader) ws = at::empty({static_cast<int64_t>(bytes)}, z.options().dtype(at::kByte));
+    checked(api.token_logprobs(&L, &Y, t, logp.data_ptr<float>(), lse.data_ptr<float>(),
+                               ws.defined() ? ws.data_ptr() : nullptr, ws.defined() ? bytes : 0, stream_of(z)),
             "moteopt_token_logprobs");
     return tuple({logp, lse});
   });

@@ -40,7 +40,7 @@ def _load():
     spec = importlib.util.spec_from_file_location("mote_b200._torch_losses", BINDING)
     mod = importlib.util.module_from_spec(spec)
     spec.loader.exec_module(mod)
-    names = ("moteopt_last_error", "moteopt_token_logprobs", "moteopt_token_logprobs_backward",
+    names = ("moteopt_last_error", "moteopt_token_logprobs_workspace_size", "moteopt_token_logprobs", "moteopt_token_logprobs_backward",
              "moteopt_policy_loss_workspace_size", "moteopt_policy_loss", "moteopt_preference_loss_workspace_size",
              "moteopt_preference_loss")
     mod.init(*[C.cast(getattr(L.lib, n), C.c_void_p).value for n in names], L.MoteoptError, torch.OutOfMemoryError)
