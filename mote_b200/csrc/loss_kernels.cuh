@@ -66,27 +66,17 @@ __device__ __forceinline__ float ex2(float t) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(t));
   return r;
 }
-__device__ __forceinline__ uint64_t pack2(float a, float b) {
-  uint64_t r;
+// Two fp32 values in one register pair, and a multiply-add of both at once
+using F2 = uint64_t;
+__device__ __forceinline__ F2 pack2(float a, float b) {
+  F2 r;
   asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
   return r;
 }
-__device__ __forceinline__ void unpack2(uint64_t v, float& a, float& b) {
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+__device__ __forceinline__ void unpack2(F2 v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ F2 fma2(F2 x, F2 y, F2 z) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(x), "l"(y), "l"(z));
   return r;
 }
 
@@ -96,7 +86,7 @@ __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
 // every exponent of a row the same way.) c_lo > 0 keeps -inf a -inf. Beyond |m| = 2^60, where a product may overflow, any
 // two different logits are at least 2^37 apart: a scale of 2^-20 gives 1 for z = m and 0 below.
 struct Ex {
-  uint64_t hi, lo, nb;
+  F2 hi, lo, nb;
   float fix;
   __device__ Ex(float m, const Rows& R) {
     const bool far = fabsf(m) > 0x1p60f && fabsf(m) < INFINITY;
@@ -107,14 +97,21 @@ struct Ex {
     lo = pack2(l, l);
     nb = pack2(-b, -b);
   }
-  __device__ __forceinline__ uint64_t two(uint64_t z) const {
+  __device__ __forceinline__ void two(F2 z, float& e0, float& e1) const {
     float t0, t1;
     unpack2(fma2(z, lo, fma2(z, hi, nb)), t0, t1);
-    return pack2(ex2(t0), ex2(t1));
+    e0 = ex2(t0);
+    e1 = ex2(t1);
+  }
+  __device__ __forceinline__ void add(F2 z, float& s0, float& s1) const {
+    float e0, e1;
+    two(z, e0, e1);
+    s0 += e0;
+    s1 += e1;
   }
   __device__ __forceinline__ float one(float z) const {
     float e0, e1;
-    unpack2(two(pack2(z, z)), e0, e1);
+    two(pack2(z, z), e0, e1);
     return e0;
   }
 };
@@ -191,29 +188,33 @@ struct Pairs;
 template <>
 struct Pairs<__nv_bfloat16> {
   static constexpr int kN = 4;
-  uint64_t p[4];
+  F2 p[4];
   __device__ __forceinline__ explicit Pairs(const uint4& v)
       : p{pack2(lo_bf16(v.x), hi_bf16(v.x)), pack2(lo_bf16(v.y), hi_bf16(v.y)), pack2(lo_bf16(v.z), hi_bf16(v.z)),
           pack2(lo_bf16(v.w), hi_bf16(v.w))} {}
-  __device__ __forceinline__ uint4 line() const {   // rounded once
+  __device__ __forceinline__ uint4 scaled(const Ex& ex, float f) const {   // f exp, rounded once
     float a[8];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) unpack2(p[u], a[2 * u], a[2 * u + 1]);
+    for (int u = 0; u < 4; ++u) {
+      ex.two(p[u], a[2 * u], a[2 * u + 1]);
+      a[2 * u] *= f;
+      a[2 * u + 1] *= f;
+    }
     return make_uint4(to_bf16x2(a[0], a[1]), to_bf16x2(a[2], a[3]), to_bf16x2(a[4], a[5]), to_bf16x2(a[6], a[7]));
   }
 };
 template <>
 struct Pairs<float> {
   static constexpr int kN = 2;
-  uint64_t p[2];
+  F2 p[2];
   __device__ __forceinline__ explicit Pairs(const uint4& v)
       : p{pack2(bits(v.x), bits(v.y)), pack2(bits(v.z), bits(v.w))} {}
   static __device__ __forceinline__ float bits(uint32_t w) { return __uint_as_float(w); }
-  __device__ __forceinline__ uint4 line() const {
+  __device__ __forceinline__ uint4 scaled(const Ex& ex, float f) const {
     float a[4];
-    unpack2(p[0], a[0], a[1]);
-    unpack2(p[1], a[2], a[3]);
-    return make_uint4(__float_as_uint(a[0]), __float_as_uint(a[1]), __float_as_uint(a[2]), __float_as_uint(a[3]));
+    ex.two(p[0], a[0], a[1]);
+    ex.two(p[1], a[2], a[3]);
+    return make_uint4(__float_as_uint(a[0] * f), __float_as_uint(a[1] * f), __float_as_uint(a[2] * f), __float_as_uint(a[3] * f));
   }
 };
 
@@ -357,6 +358,58 @@ __device__ __forceinline__ uint4 load_shifted(const unsigned char* p, uint32_t o
   const uint4* const l = reinterpret_cast<const uint4*>(p + (off & ~15u));
   const uint32_t by = off & 15u;
   return by ? shift_lines(l[0], l[1], by) : l[0];
+}
+
+// A thread's running maximum and sum. The maximum moves only when a logit is more than kSlack units of log2 above it, so the
+// sum is rescaled hardly ever.
+constexpr float kSlack = 16.f;
+struct Running {
+  float m, s0, s1;
+  Ex ex;
+  __device__ explicit Running(const Rows& R) : m(kNegInf), s0(0.f), s1(0.f), ex(kNegInf, R) {}
+  template <typename T, int kN>
+  __device__ __forceinline__ void add(const uint4 (&v)[kN], const Rows& R, float inv_t) {
+    using W = Word<T>;
+    uint32_t t = W::kEmpty;
+#pragma unroll
+    for (int k = 0; k < kN; ++k) t = vec_max<T>(t, v[k]);
+    const float top = W::top(t);
+    if ((top - m) * R.c_hi > kSlack) {
+      const float by = ex.fix * rescale(m, top, inv_t);
+      s0 *= by;
+      s1 *= by;
+      m = top;
+      ex = Ex(m, R);
+    }
+#pragma unroll
+    for (int k = 0; k < kN; ++k) {
+      const Pairs<T> q(v[k]);
+#pragma unroll
+      for (int u = 0; u < Pairs<T>::kN; ++u) ex.add(q.p[u], s0, s1);
+    }
+  }
+  __device__ __forceinline__ Part part() const { return Part{m, (s0 + s1) * ex.fix}; }
+};
+
+// Gradient lines [i, n) by kStride of an output row from lines of shared memory `off` bytes from `src`: f 2^((z - m) c)
+template <typename T, uint32_t kStride, int kUnroll>
+__device__ __forceinline__ void gradient_lines(uint4* __restrict__ out, const unsigned char* src, uint32_t off, uint32_t i,
+                                               uint32_t n, const Ex& ex, float f) {
+  if ((off & 15u) == 0) {   // the two rows are aligned alike
+    const uint4* const in = reinterpret_cast<const uint4*>(src + static_cast<int32_t>(off));
+    for (; i + (kUnroll - 1) * kStride < n; i += kUnroll * kStride) {
+      uint4 v[kUnroll];
+#pragma unroll
+      for (int k = 0; k < kUnroll; ++k) v[k] = in[i + k * kStride];
+#pragma unroll
+      for (int k = 0; k < kUnroll; ++k) out[i + k * kStride] = Pairs<T>(v[k]).scaled(ex, f);
+    }
+#pragma unroll 1
+    for (; i < n; i += kStride) out[i] = Pairs<T>(in[i]).scaled(ex, f);
+  } else {
+#pragma unroll 1
+    for (; i < n; i += kStride) out[i] = Pairs<T>(load_shifted(src, i * 16 + off)).scaled(ex, f);
+  }
 }
 
 __device__ __forceinline__ uint32_t cluster_rank() {
@@ -583,15 +636,13 @@ __global__ void __launch_bounds__(kTileWarps * 32) tile_kernel(const __grid_cons
       for (uint32_t l = gl; l < nl; l += kG) top = vec_max<T>(top, row[l]);
       const float m = group_max<kG>(W::top(top));
       const Ex ex(m, R);
-      uint64_t acc = 0;
+      float s0 = 0.f, s1 = 0.f;
 #pragma unroll 4
       for (uint32_t l = gl; l < nl; l += kG) {
         const Pairs<T> q(row[l]);
 #pragma unroll
-        for (int u = 0; u < Pairs<T>::kN; ++u) acc = add2(acc, ex.two(q.p[u]));
+        for (int u = 0; u < Pairs<T>::kN; ++u) ex.add(q.p[u], s0, s1);
       }
-      float s0, s1;
-      unpack2(acc, s0, s1);
       const float s = group_sum<kG>(s0 + s1) * ex.fix;
       const int from = ((lane - r0) & (kAtOnce - 1)) * kG;
       const float mr = __shfl_sync(0xffffffffu, m, from), sr = __shfl_sync(0xffffffffu, s, from);
@@ -651,15 +702,7 @@ __global__ void __launch_bounds__(kTileWarps * 32) tile_kernel(const __grid_cons
       }
       const Ex ex(m, R);
       const float kf = k * ex.fix;
-      const uint64_t k2 = pack2(kf, kf);
-      const uint32_t shift = (sk + so.head) * sizeof(T);
-#pragma unroll 2
-      for (uint32_t l = gl; l < so.vecs; l += kG) {
-        Pairs<T> q(load_shifted(row, l * 16 + shift));
-#pragma unroll
-        for (int u = 0; u < Pairs<T>::kN; ++u) q.p[u] = mul2(ex.two(q.p[u]), k2);
-        ov[l] = q.line();
-      }
+      gradient_lines<T, kG, 2>(ov, row, (sk + so.head) * static_cast<uint32_t>(sizeof(T)), gl, so.vecs, ex, kf);
       for (uint32_t i = gl; i < so.head + so.tail; i += kG) {
         const uint32_t j = so.edge(i);
         store_one(out + j, ex.one(load_one(reinterpret_cast<const T*>(row) + sk + j)) * kf);
@@ -671,122 +714,122 @@ __global__ void __launch_bounds__(kTileWarps * 32) tile_kernel(const __grid_cons
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
-// Long rows, forward only: a stream of pieces of `lines` lines, a warp each, straight into registers: 4 lines a lane at a
-// time, the next 4 (of this piece or of the warp's next one) on their way meanwhile. A lane's maximum moves only when a logit
-// is more than kSlack units of log2 above it, so its sum is rescaled hardly ever. join_kernel puts a row's parts together.
+// Long rows, forward only: a stream of pieces of `lines` lines, a warp each, in batches of kBatch lines a lane. A warp has its
+// own ring of kStages batches in shared memory, filled by cp.async two batches ahead, over the end of a piece into its next
+// one, and each lane reads what it asked for itself. join_kernel puts a row's parts together.
 struct StreamArgs {
   Rows R;
   uint32_t pieces;      // of a row
   uint32_t n;           // pieces in all
-  uint32_t lines;       // of a piece: a multiple of 128
+  uint32_t lines;       // of a piece: a multiple of a batch's
   Part* parts;          // [n]
 };
-constexpr int kStreamThreads = 128, kStreamBlocks = 8, kBatch = 4;
-constexpr float kSlack = 16.f;
-
-// One batch of a lane's lines: where, and what of it counts
-struct Batch {
-  const uint4* p;       // the warp's first line
-  uint32_t left;        // lines from there to the piece's end (0: nothing)
-  uint32_t skew;        // elements of the first line in front of the row
-  uint32_t elems;       // elements from the first line's begin to the row's end
-  uint32_t y;           // the target, in elements from the first line's begin (or beyond)
-};
+constexpr int kStreamThreads = 128, kStreamBlocks = 7, kBatch = 4, kStages = 3;
+constexpr int kAhead = 8;   // pieces that may be known and not done: kStages batches of different ones and the next, rounded up
+constexpr size_t kStreamSmem = static_cast<size_t>(kStreamThreads) * kStages * kBatch * 16;
 
 template <typename T>
 __global__ void __launch_bounds__(kStreamThreads, kStreamBlocks) stream_kernel(const __grid_constant__ StreamArgs A) {
+  extern __shared__ __align__(16) unsigned char sm[];
+  __shared__ uint4 sh_known[kStreamThreads / 32][kAhead];
   using W = Word<T>;
-  constexpr uint32_t kPer = 16 / sizeof(T);
+  constexpr uint32_t kPer = 16 / sizeof(T), kLines = 32 * kBatch, kElems = kLines * kPer;
   const Rows& R = A.R;
   const uint32_t lane = threadIdx.x & 31, step = gridDim.x * (kStreamThreads / 32);
   const float inv_t = static_cast<float>(R.inv_t);
   uint32_t piece = blockIdx.x * (kStreamThreads / 32) + (threadIdx.x >> 5);
   pdl_go();
   if (piece >= A.n) return;
+  // this lane's place in its warp's ring, and the warp's pieces
+  uint4* const ring = reinterpret_cast<uint4*>(sm) + (threadIdx.x >> 5) * (kStages * kLines) + lane;
+  uint4* const known = sh_known[threadIdx.x >> 5];
 
-  const auto begin = [&](uint32_t k) {
-    Batch b = {nullptr, 0, 0, 0, 0xffffffffu};
-    if (k >= A.n) return b;
-    const uint32_t row = k / A.pieces, from = (k - row * A.pieces) * A.lines;
-    const uint32_t seq = row / R.tokens, tok = row - seq * R.tokens;
-    const int64_t y = in_packed(R, row) ? R.y[seq * R.y_seq + tok * R.y_tok] : -1;
-    if (y < 0) return b;
-    const uint64_t a = reinterpret_cast<uint64_t>(R.z) + (seq * R.z_seq + tok * R.z_tok) * sizeof(T);
-    const uint32_t skew = static_cast<uint32_t>(a & 15) / sizeof(T), lines = (skew + R.vocab + kPer - 1) / kPer;
-    if (from >= lines) return b;
-    b.p = reinterpret_cast<const uint4*>(a & ~15ull) + from;
-    b.left = min(A.lines, lines - from);
-    b.skew = from == 0 ? skew : 0;
-    b.elems = skew + R.vocab - from * kPer;
-    b.y = y < static_cast<int64_t>(R.vocab) ? skew + static_cast<uint32_t>(y) - from * kPer : 0xffffffffu;   // wraps in front
-    return b;
-  };
-  const auto load = [&](uint4 (&v)[kBatch], const Batch& b) {
-#pragma unroll
-    for (uint32_t k = 0; k < kBatch; ++k) {
-      v[k] = make_uint4(W::kEmpty, W::kEmpty, W::kEmpty, W::kEmpty);
-      if (lane + 32 * k < b.left) v[k] = load_vec(b.p + lane + 32 * k);
-    }
-  };
-
-  Batch cur = begin(piece);
-  uint4 v[kBatch];
-  load(v, cur);
-  float m = kNegInf;
-  Ex ex(m, R);
-  uint64_t acc = 0;
-  while (true) {
-    // what comes next: this piece's next batch, or the next piece
-    constexpr uint32_t kLines = 32 * kBatch, kElems = kLines * kPer;
-    const bool ends = cur.left <= kLines;
-    Batch next;
-    if (ends) {
-      next = begin(piece + step);
-    } else {
-      next = Batch{cur.p + kLines, cur.left - kLines, 0, cur.elems - kElems, cur.y - kElems};
-    }
-    uint4 w[kBatch];
-    load(w, next);
-    if (cur.skew != 0 || cur.elems < kElems || cur.y < kElems) {   // a batch with an edge or the target in it
-#pragma unroll
-      for (uint32_t k = 0; k < kBatch; ++k) {
-        const uint32_t line = lane + 32 * k, e = line * kPer;
-        if (line >= cur.left) continue;
-        const uint32_t from = line == 0 ? cur.skew : 0;
-        keep<T>(v[k], from, min(kPer, cur.elems - e) - from);
-        if (cur.y - e < kPer) drop_target<T>(v[k], cur.y - e);
+  // The asking side. A piece: its lines (0: nothing to read), the elements in front of the row in its first line, the row's
+  // end and the target, in elements from the first line's begin. A piece without lines still takes a (void) batch, so that
+  // both sides count the same.
+  uint32_t ask_piece = piece, asked = 0, ask_lines = 0, ask_count = 0, ask_stage = 0;
+  uint64_t ask_at = 0;
+  const auto look = [&] {
+    uint4 b = make_uint4(0, 0, 0, 0xffffffffu);
+    if (ask_piece < A.n) {
+      const uint32_t row = ask_piece / A.pieces, from = (ask_piece - row * A.pieces) * A.lines;
+      const uint32_t seq = row / R.tokens, tok = row - seq * R.tokens;
+      const int64_t y = in_packed(R, row) ? R.y[seq * R.y_seq + tok * R.y_tok] : -1;
+      const uint64_t a = reinterpret_cast<uint64_t>(R.z) + (seq * R.z_seq + tok * R.z_tok) * sizeof(T);
+      const uint32_t skew = static_cast<uint32_t>(a & 15) / sizeof(T), lines = (skew + R.vocab + kPer - 1) / kPer;
+      if (y >= 0 && from < lines) {
+        b.x = min(A.lines, lines - from);
+        b.y = from == 0 ? skew : 0;
+        b.z = skew + R.vocab - from * kPer;
+        if (y < static_cast<int64_t>(R.vocab)) b.w = skew + static_cast<uint32_t>(y) - from * kPer;   // wraps in front
+        ask_at = (a & ~15ull) + (static_cast<uint64_t>(from) + lane) * 16;
       }
     }
-    uint32_t t = W::kEmpty;
+    ask_lines = b.x;
+    if (lane == 0) known[ask_count % kAhead] = b;
+    ++ask_count;
+    __syncwarp();
+  };
+  const auto request = [&] {
+    const uint32_t dst = smem_u32(ring) + ask_stage * (kLines * 16);
+    if (asked + kLines <= ask_lines) {
 #pragma unroll
-    for (int k = 0; k < kBatch; ++k) t = vec_max<T>(t, v[k]);
-    const float top = W::top(t);
-    if ((top - m) * R.c_hi > kSlack || (m == kNegInf && top > m)) {
-      const float by = ex.fix * rescale(m, top, inv_t);
-      acc = mul2(acc, pack2(by, by));
-      m = top;
-      ex = Ex(m, R);
+      for (uint32_t k = 0; k < kBatch; ++k)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + 512 * k), "l"(ask_at + 512 * k) : "memory");
+    } else {
+#pragma unroll
+      for (uint32_t k = 0; k < kBatch; ++k)
+        if (asked + lane + 32 * k < ask_lines)
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + 512 * k), "l"(ask_at + 512 * k) : "memory");
     }
-#pragma unroll
-    for (int k = 0; k < kBatch; ++k) {
-      const Pairs<T> q(v[k]);
-#pragma unroll
-      for (int u = 0; u < Pairs<T>::kN; ++u) acc = add2(acc, ex.two(q.p[u]));
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    ask_stage = ask_stage == kStages - 1 ? 0 : ask_stage + 1;
+    asked += kLines;
+    ask_at += kLines * 16;
+    if (asked >= ask_lines) {
+      ask_piece += step;
+      asked = 0;
+      look();
     }
-    if (ends) {
-      float s0, s1;
-      unpack2(acc, s0, s1);
-      const Part p = warp_join(Part{m, (s0 + s1) * ex.fix}, inv_t);
-      if (lane == 0) A.parts[piece] = p;
-      piece += step;
-      if (piece >= A.n) return;
-      m = kNegInf;
-      acc = 0;
-    }
-    cur = next;
+  };
+  look();
+#pragma unroll 1
+  for (int k = 0; k < kStages - 1; ++k) request();
+
+  uint32_t count = 0, stage = 0;
+  for (; piece < A.n; piece += step, ++count) {
+    const uint4 b = known[count % kAhead];
+    Running run(R);
+    for (uint32_t done = 0;;) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
+      const uint4* const at = ring + stage * kLines;
+      stage = stage == kStages - 1 ? 0 : stage + 1;
+      uint4 v[kBatch];
 #pragma unroll
-    for (int k = 0; k < kBatch; ++k) v[k] = w[k];
+      for (int k = 0; k < kBatch; ++k) v[k] = at[32 * k];
+      request();   // into the batch that was read before this one
+      const uint32_t e0 = done * kPer, there = b.w - e0;
+      if ((b.x < done + kLines) | (b.z - e0 < kElems) | (e0 < b.y)) {   // an edge of the row, or the piece's end
+#pragma unroll
+        for (uint32_t k = 0; k < kBatch; ++k) {
+          const uint32_t line = done + lane + 32 * k, e = line * kPer;
+          const uint32_t from = line == 0 ? b.y : 0;
+          keep<T>(v[k], from, line < b.x ? min(kPer, b.z - e) - from : 0);
+        }
+      }
+      if (there < kElems) {   // the target
+#pragma unroll
+        for (uint32_t k = 0; k < kBatch; ++k)
+          if (there / kPer == lane + 32 * k) drop_target<T>(v[k], there % kPer);
+      }
+      run.add<T>(v, R, inv_t);
+      done += kLines;
+      if (done >= b.x) break;
+    }
+    const Part p = warp_join(run.part(), inv_t);
+    if (lane == 0) A.parts[piece] = p;
   }
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
 
 // Rows from their pieces' parts, a warp each
@@ -855,7 +898,7 @@ struct SliceArgs {
 };
 
 template <typename T, int kThreads>
-__global__ void __launch_bounds__(kThreads, 1024 / kThreads) slice_kernel(const __grid_constant__ SliceArgs A) {
+__global__ void __launch_bounds__(kThreads, kThreads == 128 ? 6 : 3) slice_kernel(const __grid_constant__ SliceArgs A) {
   extern __shared__ __align__(16) unsigned char sm[];
   using W = Word<T>;
   constexpr uint32_t kPer = 16 / sizeof(T);
@@ -924,27 +967,18 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) slice_kernel(const 
   if (threadIdx.x == 0 && skew != 0 && lines > 0) keep<T>(line[0], skew, kPer);
   if (lines > 0 && threadIdx.x == (lines - 1) % kThreads) keep<T>(line[lines - 1], 0, skew + len - (lines - 1) * kPer);
   if (ty != 0xffffffffu && threadIdx.x == ty / kPer % kThreads) drop_target<T>(line[ty / kPer], ty % kPer);
-  float m = kNegInf;
-  Ex ex(m, R);
-  uint64_t acc = 0;
-  for (uint32_t i = threadIdx.x; i < lines; i += 2 * kThreads) {   // two lines at a time under a running maximum
-    const uint4 va = line[i];
-    uint4 vb = make_uint4(W::kEmpty, W::kEmpty, W::kEmpty, W::kEmpty);
-    if (i + kThreads < lines) vb = line[i + kThreads];
-    const float top = W::top(vec_max<T>(vec_max<T>(W::kEmpty, va), vb));
-    if (top > m) {
-      const float by = ex.fix * rescale(m, top, inv_t);
-      acc = mul2(acc, pack2(by, by));
-      m = top;
-      ex = Ex(m, R);
-    }
-    const Pairs<T> qa(va), qb(vb);
-#pragma unroll
-    for (int u = 0; u < Pairs<T>::kN; ++u) acc = add2(acc, add2(ex.two(qa.p[u]), ex.two(qb.p[u])));
+  Running run(R);
+  uint32_t at = threadIdx.x;
+  for (; at + 3 * kThreads < lines; at += 4 * kThreads) {
+    const uint4 v[4] = {line[at], line[at + kThreads], line[at + 2 * kThreads], line[at + 3 * kThreads]};
+    run.add<T>(v, R, inv_t);
   }
-  float s0, s1;
-  unpack2(acc, s0, s1);
-  const Part p = row_join<kThreads>(Part{m, (s0 + s1) * ex.fix}, A.cl, rank, inv_t, sh_warp, sh_block);
+#pragma unroll 1
+  for (; at < lines; at += kThreads) {
+    const uint4 v[1] = {line[at]};
+    run.add<T>(v, R, inv_t);
+  }
+  const Part p = row_join<kThreads>(run.part(), A.cl, rank, inv_t, sh_warp, sh_block);
   if (threadIdx.x == 0) {
     const RowStat st = row_stat(sh_in[0], p.m, p.s, R.inv_t);
     const RowLoss L = policy_row_loss(st.logp, A.P, sh_in[2], sh_in[3], A.P.ref_lp.p != nullptr, sh_in[1]);
@@ -964,23 +998,18 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) slice_kernel(const 
   }
   if (A.grad == nullptr) return;
   __syncthreads();
-  ex = Ex(p.m, R);
+  const Ex ex(p.m, R);
   const float f = sh_g[0] * ex.fix, gy = sh_g[1];
   if (je != 0xffffffffu) {
     const T* const x = reinterpret_cast<const T*>(sm) + skew + (je - e0);
     store_one(out + je, je == y ? gy : ex.one(load_one(x)) * f);
   }
-  const uint64_t f2 = pack2(f, f);
-  const uint32_t shift = (skew + so.head - e0) * sizeof(T);   // from an output line's bytes to the slice's (wraps)
-#pragma unroll 2
-  for (uint32_t i = v0 + threadIdx.x; i < v1; i += kThreads) {
-    const uint32_t e = so.head + i * kPer;
-    Pairs<T> q(load_shifted(sm, i * 16 + shift));
-#pragma unroll
-    for (int u = 0; u < Pairs<T>::kN; ++u) q.p[u] = mul2(ex.two(q.p[u]), f2);
-    *reinterpret_cast<uint4*>(out + e) = q.line();
-    if (y - e < kPer) store_one(out + y, gy);
-  }
+  // output line i of the row is at byte i * 16 + (skew + head - e0) * size of the slice (the sum may wrap, not the address)
+  gradient_lines<T, kThreads, 4>(reinterpret_cast<uint4*>(out + so.head) + v0, sm,
+                                 v0 * 16 + (skew + so.head - e0) * static_cast<uint32_t>(sizeof(T)), threadIdx.x, v1 - v0, ex,
+                                 f);
+  const uint32_t yl = (y - so.head) / kPer;   // the target's line, if it lies in one of this slice's
+  if (y - so.head < so.vecs * kPer && yl >= v0 && yl < v1 && threadIdx.x == (yl - v0) % kThreads) store_one(out + y, gy);
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
@@ -1043,17 +1072,13 @@ __global__ void __launch_bounds__(kGradThreads) grad_kernel(const __grid_constan
   const KeptRow r = kept_row(A.K, R, row, seq, tok, coef);
   const Ex ex(r.m, R);
   const float f = r.f * ex.fix;
-  const uint64_t f2 = pack2(f, f);
   const uint32_t y = y64 < static_cast<int64_t>(R.vocab) ? static_cast<uint32_t>(y64) : 0xffffffffu;
   if (edge) store_one(out + je, je == y ? r.gy : ex.one(load_one(z + je)) * f);
 #pragma unroll
   for (int k = 0; k < kGradVecs; ++k) {
     const uint32_t at = begin + k * kGradThreads;
     if (at >= so.vecs) break;
-    Pairs<T> q(by ? shift_lines(v[k], w[k], by) : v[k]);
-#pragma unroll
-    for (int u = 0; u < Pairs<T>::kN; ++u) q.p[u] = mul2(ex.two(q.p[u]), f2);
-    ov[at] = q.line();
+    ov[at] = Pairs<T>(by ? shift_lines(v[k], w[k], by) : v[k]).scaled(ex, f);
     const uint32_t e = so.head + at * kPer;
     if (y - e < kPer) store_one(out + y, r.gy);
   }
