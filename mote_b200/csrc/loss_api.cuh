@@ -124,16 +124,45 @@ TileShape tile_shape(int64_t rows, int64_t line_bytes, int sms) {
 }
 int64_t line_bytes(int dtype, int64_t vocab) { return (vocab * esize(dtype) + 16 - esize(dtype) + 15) / 16 * 16; }
 
+// 8 lanes a row with at most 2 or 5 lines each, or more, or 32 lanes a row. (10 lines each take so many registers that 8 x 2048
+// x 271 fp32, forward, takes 7.1 us and not 6.1.)
+template <typename T, Mode kMode>
+auto tile_fn(uint32_t pitch) {
+  const uint32_t lines = pitch / 16 - 1;
+  return pitch > kNarrowPitch ? tile_kernel<T, 32, 0, kMode>
+         : lines <= 16        ? tile_kernel<T, 8, 2, kMode>
+         : lines <= 40        ? tile_kernel<T, 8, 5, kMode>
+                              : tile_kernel<T, 8, 0, kMode>;
+}
+template <Mode kMode>
+auto tile_fn(int dtype, uint32_t pitch) {
+  return dtype == MOTEOPT_DTYPE_BF16 ? tile_fn<__nv_bfloat16, kMode>(pitch) : tile_fn<float, kMode>(pitch);
+}
+size_t tile_smem(const TileShape& s) { return static_cast<size_t>(kTileWarps) * s.per_warp * s.pitch; }
+
 template <Mode kMode>
 int launch_tile(int dtype, TileArgs A, const TileShape& s, cudaStream_t st, bool after = false) {
   A.per_warp = s.per_warp;
   A.pitch = s.pitch;
-  const bool bf = dtype == MOTEOPT_DTYPE_BF16, narrow = s.pitch <= kNarrowPitch;
-  auto* const k = narrow ? (bf ? tile_kernel<__nv_bfloat16, 8, kMode> : tile_kernel<float, 8, kMode>)
-                         : (bf ? tile_kernel<__nv_bfloat16, 32, kMode> : tile_kernel<float, 32, kMode>);
-  const size_t smem = static_cast<size_t>(kTileWarps) * s.per_warp * s.pitch;
-  return launch_after(k, A, static_cast<unsigned>(cdiv(s.tiles, kTileWarps)), kTileWarps * 32, smem, st, "loss tile_kernel",
-                      !after);
+  return launch_after(tile_fn<kMode>(dtype, s.pitch), A, static_cast<unsigned>(cdiv(s.tiles, kTileWarps)), kTileWarps * 32,
+                      tile_smem(s), st, "loss tile_kernel", !after);
+}
+// Few rows: the policy or the preference loss in one launch of one cluster, whose blocks' sums meet in its first block, or whose
+// blocks share out the pairs. Two lots of rows a warp take no longer than the launches that this saves.
+bool one_cluster(int64_t rows, const TileShape& s) {
+  return rows <= static_cast<int64_t>(kMaxCluster) * kTileWarps * (s.pitch <= kNarrowPitch ? 8 : 1) &&
+         (s.pitch > kNarrowPitch || 8 * s.pitch <= kTileBytes);
+}
+constexpr int kClusterPairs = 256;
+template <Mode kMode>
+int launch_tile_cluster(int dtype, TileArgs A, TileShape s, cudaStream_t st) {
+  unsigned blocks = 1;
+  while (blocks < kMaxCluster && static_cast<int64_t>(blocks) * kTileWarps < A.R.n) blocks *= 2;
+  s.per_warp = static_cast<int>(cdiv(A.R.n, blocks * kTileWarps));
+  A.per_warp = s.per_warp;
+  A.pitch = s.pitch;
+  return launch_cluster(tile_fn<kMode>(dtype, s.pitch), A, 1, blocks, kTileWarps * 32, tile_smem(s), st,
+                        "loss tile_kernel");
 }
 
 // Long rows: blocks per row and bytes of shared memory each. A slice of up to kSliceBytes leaves three blocks an SM; a
@@ -286,17 +315,25 @@ int allow_smem(K* kernel, int bytes) {
   MO_CUDA(cudaFuncSetAttribute(reinterpret_cast<const void*>(kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
   return MOTEOPT_OK;
 }
+template <typename K>
+int allow_wide(K* kernel) {   // clusters of 16 blocks
+  MO_CUDA(cudaFuncSetAttribute(reinterpret_cast<const void*>(kernel), cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+  return MOTEOPT_OK;
+}
 template <typename T>
 int kernel_setup() {
   MO_TRY(allow_smem(slice_kernel<T, 128>, static_cast<int>(kSliceMost)));
   MO_TRY(allow_smem(slice_kernel<T, 256>, static_cast<int>(kSliceMost)));
-  const void* const wide[] = {reinterpret_cast<const void*>(slice_kernel<T, 128>),
-                              reinterpret_cast<const void*>(slice_kernel<T, 256>)};
-  for (const void* k : wide) MO_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+  MO_TRY(allow_wide(slice_kernel<T, 128>));
+  MO_TRY(allow_wide(slice_kernel<T, 256>));
+  for (uint32_t lines : {16u, 40u, 100u, 500u}) {
+    MO_TRY(allow_wide(tile_fn<T, kPolicyLoss>((lines + 1) * 16)));
+    MO_TRY(allow_wide(tile_fn<T, kPreference>((lines + 1) * 16)));
+  }
   return MOTEOPT_OK;
 }
 
-// the slices' shared memory and their clusters of 16 blocks are beyond the default limits
+// the slices' shared memory, and clusters of 16 blocks, are beyond the default limits
 int loss_setup(int* sms) {
   MO_TRY(device_setup(sms));
   static std::atomic<unsigned long long> ready{0};   // a bit per device
@@ -404,6 +441,10 @@ int moteopt_policy_loss(const moteopt_logits* logits, const moteopt_positions* t
     A.grad = grad_logits;
     A.partials = partials;
     const TileShape s = tile_shape(R.n, line_bytes(logits->dtype, R.vocab), sms);
+    if (one_cluster(R.n, s)) {
+      A.sums = sums;
+      return launch_tile_cluster<kPolicyLoss>(logits->dtype, A, s, st);
+    }
     MO_TRY(launch_tile<kPolicyLoss>(logits->dtype, A, s, st));
     return launch_sums(partials, s.tiles, mid, sums, st);
   }
@@ -458,8 +499,6 @@ int moteopt_preference_loss(const moteopt_logits* logits, const moteopt_position
   double* const pair_loss = reinterpret_cast<double*>(ws + L.pairs);
   R.cu = p.cu_seqlens;
   R.n_seqs = static_cast<int>(p.sequences);
-  if (R.n > 0)
-    MO_TRY(launch_forward(logits->dtype, R, nullptr, lse, logp64, coef, reinterpret_cast<Part*>(ws + L.parts), sms, st));
   PairArgs A;
   std::memset(&A, 0, sizeof(A));
   A.R = R;
@@ -475,7 +514,6 @@ int moteopt_preference_loss(const moteopt_logits* logits, const moteopt_position
   A.pair_loss = pair_loss;
   A.rewards = rewards;
   A.seq_logp = logprobs;
-  MO_TRY(launch_after(pair_kernel, A, static_cast<unsigned>(A.pairs), kPairThreads, 0, st, "loss pair_kernel", R.n == 0));
   Kept K;
   std::memset(&K, 0, sizeof(K));
   K.logp64 = logp64;
@@ -484,6 +522,21 @@ int moteopt_preference_loss(const moteopt_logits* logits, const moteopt_position
   K.pair_loss = pair_loss;
   K.pairs = A.pairs;
   K.loss = loss;
+  const TileShape t = tile_shape(R.n, line_bytes(logits->dtype, R.vocab), sms);
+  if (R.n > 0 && short_rows(logits->dtype, R.vocab) && one_cluster(R.n, t) && A.pairs <= kClusterPairs) {
+    TileArgs B;
+    std::memset(&B, 0, sizeof(B));
+    B.R = R;
+    B.logp64 = logp64;
+    B.coef = coef;
+    B.grad = grad_logits;
+    B.K = K;
+    B.pair = A;
+    return launch_tile_cluster<kPreference>(logits->dtype, B, t, st);
+  }
+  if (R.n > 0)
+    MO_TRY(launch_forward(logits->dtype, R, nullptr, lse, logp64, coef, reinterpret_cast<Part*>(ws + L.parts), sms, st));
+  MO_TRY(launch_after(pair_kernel, A, static_cast<unsigned>(A.pairs), kPairThreads, 0, st, "loss pair_kernel", R.n == 0));
   if (!grad_logits || R.n == 0) return launch_after(pair_sum_kernel, K, 1, 32, 0, st, "loss pair_sum_kernel");
   return launch_gradient(logits->dtype, R, K, grad_logits, sms, st, true);
 }

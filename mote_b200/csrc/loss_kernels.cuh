@@ -160,7 +160,6 @@ __device__ __forceinline__ float load_one(const __nv_bfloat16* p) { return __bfl
 __device__ __forceinline__ float load_one(const float* p) { return *p; }
 __device__ __forceinline__ void store_one(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
 __device__ __forceinline__ void store_one(float* p, float v) { *p = v; }
-
 __device__ __forceinline__ float warp_max(float v) {   // NaN is left out: the exponentials carry it
   float r;
   asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
@@ -294,6 +293,19 @@ __device__ __forceinline__ RowLoss policy_row_loss(double logp, const Policy& P,
   return L;
 }
 
+// The policy loss of a row: its sums' terms, and its gradient's factors
+struct PolicyRow {
+  double part[4];
+  float f, gy;
+};
+__device__ __forceinline__ PolicyRow policy_row(const Policy& P, const RowStat& st, float wt, float adv, float old_lp,
+                                                float ref_lp, double inv_t) {
+  const RowLoss L = policy_row_loss(st.logp, P, old_lp, ref_lp, P.ref_lp.p != nullptr, adv);
+  const double w = wt, inv = P.div ? 1.0 / static_cast<double>(*P.div) : P.inv_div;
+  const float g = static_cast<float>(w * L.slope * inv * inv_t);
+  return PolicyRow{{w * L.loss * inv, w, w * L.kl * inv, L.clipped ? w : 0.0}, -g * st.f, g * st.rest};
+}
+
 __device__ __forceinline__ bool in_packed(const Rows& R, uint32_t row) {
   if (R.cu == nullptr) return true;
   return static_cast<int64_t>(row) >= R.cu[0] && static_cast<int64_t>(row) < R.cu[R.n_seqs];
@@ -331,6 +343,27 @@ template <typename T>
 __device__ __forceinline__ uint32_t vec_max(uint32_t top, const uint4& v) {
   using W = Word<T>;
   return W::max(W::max(W::max(top, v.x), W::max(v.y, v.z)), v.w);
+}
+
+// kBehind[i]: the bytes of a line behind its first 2 i, as masks of its words
+__constant__ const uint4 kBehind[9] = {
+    {0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu}, {0xffff0000u, 0xffffffffu, 0xffffffffu, 0xffffffffu},
+    {0u, 0xffffffffu, 0xffffffffu, 0xffffffffu},          {0u, 0xffff0000u, 0xffffffffu, 0xffffffffu},
+    {0u, 0u, 0xffffffffu, 0xffffffffu},                   {0u, 0u, 0xffff0000u, 0xffffffffu},
+    {0u, 0u, 0u, 0xffffffffu},                            {0u, 0u, 0u, 0xffff0000u},
+    {0u, 0u, 0u, 0u}};
+template <typename T>
+__device__ __forceinline__ uint4 behind(uint32_t elems) {
+  return kBehind[elems * (sizeof(T) / 2)];
+}
+__device__ __forceinline__ void put_in(uint4& v, const uint4& m, uint32_t other) {   // `other` where the mask is 0
+  v.x = (v.x & m.x) | (other & ~m.x);
+  v.y = (v.y & m.y) | (other & ~m.y);
+  v.z = (v.z & m.z) | (other & ~m.z);
+  v.w = (v.w & m.w) | (other & ~m.w);
+}
+__device__ __forceinline__ void put_out(uint4& v, const uint4& m, uint32_t other) {   // where it is 1
+  put_in(v, make_uint4(~m.x, ~m.y, ~m.z, ~m.w), other);
 }
 
 // `n` elements of a line from `from` stay, the others become -inf
@@ -428,6 +461,34 @@ __device__ __forceinline__ void store_remote(void* local, uint32_t rank, float a
 
 constexpr int kMaxCluster = 16;
 
+// The sums of one cluster's warps' terms, in a fixed order: lane 0 of each warp has them
+template <int kWarps>
+__device__ __forceinline__ void cluster_sums(const double (&part)[4], float* out) {
+  __shared__ double sh[kWarps][4], sh_block[kMaxCluster][4];
+  const uint32_t rank = cluster_rank();
+  uint32_t blocks;
+  asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(blocks));
+  if ((threadIdx.x & 31) == 0)
+    for (int k = 0; k < 4; ++k) sh[threadIdx.x >> 5][k] = part[k];
+  __syncthreads();
+  cluster_wait();   // every block runs (arrived at its start)
+  if (threadIdx.x < 4) {
+    double t = 0.0;
+    for (int w = 0; w < kWarps; ++w) t += sh[w][threadIdx.x];
+    uint32_t dst;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(dst) : "r"(smem_u32(&sh_block[rank][threadIdx.x])), "r"(0));
+    asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(dst), "d"(t) : "memory");
+  }
+  __syncwarp();
+  cluster_arrive();
+  cluster_wait();
+  if (rank == 0 && threadIdx.x < 4) {
+    double t = 0.0;
+    for (uint32_t b = 0; b < blocks; ++b) t += sh_block[b][threadIdx.x];
+    out[threadIdx.x] = static_cast<float>(t);
+  }
+}
+
 // The sums of a row from its threads' parts, given to every thread. One block, or a cluster of `cl` blocks whose warps 0
 // write their block's part into every block's shared memory.
 template <int kThreads>
@@ -487,9 +548,105 @@ __device__ __forceinline__ KeptRow kept_row(const Kept& K, const Rows& R, uint32
 __device__ __forceinline__ void sum_pairs(const Kept& K) {   // one warp, in a fixed order
   const int lane = threadIdx.x & 31;
   double v = 0.0;
-  for (int i = lane; i < K.pairs; i += 32) v += K.pair_loss[i];
+  for (int i = lane; i < K.pairs; i += 32) v += __ldcg(K.pair_loss + i);
   v = warp_sum(v);
   if (lane == 0) *K.loss = static_cast<float>(v);
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+// The preference loss of a pair (chosen sequence i, rejected sequence i + pairs), one block each: the sums of the two
+// sequences' log-probabilities in 64 bits, u = beta ((s_i - ref_i) - (s_j - ref_j)), and each sequence's coefficient written
+// to its rows.
+struct PairArgs {
+  Rows R;
+  int pairs;
+  const float* ref;      // [2 pairs], or null
+  double beta, eps, inv_div;
+  const float* div;
+  int average;
+  const double* logp64;
+  float* coef;           // [n], or null (no gradient)
+  double* pair_loss;
+  float* rewards;        // [2 pairs]
+  float* seq_logp;       // [2 pairs]
+};
+template <int kThreads>
+__device__ __forceinline__ void pair_loss(const PairArgs& A, uint32_t pair) {   // all threads of a block
+  const Rows& R = A.R;
+  __shared__ double sh_s[2][kThreads / 32];
+  __shared__ int sh_n[2][kThreads / 32];
+  __shared__ float sh_c[2];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  int64_t b[2], e[2];
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const int64_t q = pair + static_cast<int64_t>(k) * A.pairs, n = R.n;
+    if (R.cu) {   // held to the rows there are
+      b[k] = min(max(static_cast<int64_t>(R.cu[q]), static_cast<int64_t>(0)), n);
+      e[k] = min(max(static_cast<int64_t>(R.cu[q + 1]), b[k]), n);
+    } else {
+      b[k] = q * R.tokens;
+      e[k] = b[k] + R.tokens;
+    }
+    double s = 0.0;
+    int cnt = 0;
+    for (int64_t i = b[k] + threadIdx.x; i < e[k]; i += kThreads) {
+      const uint32_t row = static_cast<uint32_t>(i), seq = row / R.tokens, tok = row - seq * R.tokens;
+      MO_CHECK(row < R.n);
+      if (R.y[seq * R.y_seq + tok * R.y_tok] >= 0) {
+        s += __ldcg(A.logp64 + i);
+        ++cnt;
+      }
+    }
+    s = warp_sum(s);
+    cnt = __reduce_add_sync(0xffffffffu, cnt);
+    if (lane == 0) {
+      sh_s[k][warp] = s;
+      sh_n[k][warp] = cnt;
+    }
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    double s[2], n[2], rw[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      double t = 0.0;
+      int c = 0;
+      for (int w = 0; w < kThreads / 32; ++w) {
+        t += sh_s[k][w];
+        c += sh_n[k][w];
+      }
+      n[k] = A.average ? static_cast<double>(max(c, 1)) : 1.0;
+      s[k] = t / n[k];
+      const int q = pair + k * A.pairs;
+      rw[k] = A.beta * (s[k] - (A.ref ? static_cast<double>(A.ref[q]) : 0.0));
+      A.rewards[q] = static_cast<float>(rw[k]);
+      A.seq_logp[q] = static_cast<float>(s[k]);
+    }
+    const double u = rw[0] - rw[1], inv = A.div ? 1.0 / static_cast<double>(*A.div) : A.inv_div;
+    // -log sigmoid(u) = max(-u, 0) + log1p(e^-|u|); sigmoid(-u) = e^-|u| / (1 + e^-|u|) or 1 / (1 + e^-|u|)
+    const double t = exp(-fabs(u)), l = log1p(t);
+    const double up = (u > 0.0 ? 0.0 : -u) + l, down = (u < 0.0 ? 0.0 : u) + l;
+    const double q = 1.0 / (1.0 + t), sn = (u >= 0.0 ? t : 1.0) * q, sp = (u >= 0.0 ? 1.0 : t) * q;
+    A.pair_loss[pair] = ((1.0 - A.eps) * up + A.eps * down) * inv;
+    const double du = A.beta * (A.eps * sp - (1.0 - A.eps) * sn) * inv;
+    sh_c[0] = static_cast<float>(du / n[0]);
+    sh_c[1] = static_cast<float>(-du / n[1]);
+  }
+  __syncthreads();
+  if (A.coef == nullptr) return;
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const float c = sh_c[k];
+    for (int64_t i = b[k] + threadIdx.x; i < e[k]; i += kThreads) A.coef[i] = c;
+  }
+  __syncthreads();   // sh_c is the next pair's
+}
+constexpr int kPairThreads = 256;
+__global__ void __launch_bounds__(kPairThreads) pair_kernel(const __grid_constant__ PairArgs A) {
+  pdl_wait();
+  pdl_go();
+  pair_loss<kPairThreads>(A, blockIdx.x);
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
@@ -499,7 +656,8 @@ __device__ __forceinline__ void sum_pairs(const Kept& K) {   // one warp, in a f
 // 32 / kG rows at a time: the quarter of a warp that shared memory serves at once reads 128 bytes in a row whatever the rows'
 // pitch, and the maximum and the sum take 3 shuffles for four rows. One lane per row forms the row's values (a warp that
 // formed them for one row at a time would spend as much on them as on the row). Then, for the gradient, the exponentials
-// again from shared memory, by the lines of the output.
+// again from shared memory, by the lines of the output. kL, where it is not 0: no lane has more lines of a row, and the loops
+// over them are unrolled (64 x 1024 x 271 bf16: forward XXX us without, YYY with).
 //
 // Many warps, each with one tile, and not few with the next tile already on its way: a warp waits on its own arithmetic more
 // than on memory (with two buffers for half the warps, 16 x 1024 x 4096: policy loss 78 against 57 us).
@@ -508,7 +666,7 @@ constexpr int kTileRows = 8;           // most rows of a tile: 64 x 1024 x 271 b
                                        // and 18.2 us (fewer rows: more of a warp's instructions are not its rows'; more: too
                                        // few warps an SM), policy loss 31.7, 27.5 and 31.2 us
 constexpr int kTileBytes = 9216;       // most bytes of a tile: 6 blocks of 4 warps in an SM's shared memory
-enum Mode { kForward, kPolicyLoss, kGradient };
+enum Mode { kForward, kPolicyLoss, kGradient, kPreference };   // kPreference: of one cluster
 
 struct TileArgs {
   Rows R;
@@ -521,7 +679,9 @@ struct TileArgs {
   Policy P;
   void* grad;                          // [n][vocab], or null
   double* partials;                    // [warps][4] (policy)
+  float* sums;                         // or, of one cluster, the sums themselves
   Kept K;                              // (gradient)
+  PairArgs pair;                       // (preference)
 };
 
 template <int kG>
@@ -538,18 +698,36 @@ __device__ __forceinline__ float group_sum(float v) {
   return v;
 }
 
-template <typename T, int kG, Mode kMode>
-__global__ void __launch_bounds__(kTileWarps * 32) tile_kernel(const __grid_constant__ TileArgs A) {
-  extern __shared__ __align__(16) unsigned char sm[];
+// Between the rows' log-probabilities and their gradients: the pairs, dealt out to the cluster's blocks. What a block writes
+// to global memory in front of a barrier of the cluster is seen by the others behind it.
+template <int kThreads>
+__device__ __forceinline__ void cluster_pairs(const PairArgs& A, const Kept& K) {
+  uint32_t blocks;
+  asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(blocks));
+  __syncwarp();
+  cluster_arrive();
+  cluster_wait();
+  for (uint32_t p = cluster_rank(); p < static_cast<uint32_t>(A.pairs); p += blocks) pair_loss<kThreads>(A, p);
+  __syncwarp();
+  cluster_arrive();
+  cluster_wait();
+  if (cluster_rank() == 0 && threadIdx.x < 32) sum_pairs(K);
+}
+
+template <typename T, int kG, int kL, Mode kMode>
+__device__ __forceinline__ void tile_rows(const TileArgs& A, unsigned char* sm, double (&part)[4]) {
   using W = Word<T>;
   constexpr uint32_t kPer = 16 / sizeof(T);
   constexpr int kAtOnce = 32 / kG;
   const Rows& R = A.R;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gl = lane % kG, group = lane / kG;
-  if (kMode != kGradient) pdl_go();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = lane / kG;
+  const uint32_t gl = lane % kG;
   const uint32_t tile = blockIdx.x * kTileWarps + warp;
   const uint32_t first = tile * static_cast<uint32_t>(A.per_warp);
-  if (first >= R.n) return;
+  if (first >= R.n) {
+    if (kMode == kPreference) cluster_pairs<kTileWarps * 32>(A.pair, A.K);
+    return;
+  }
   const int rows = static_cast<int>(min(static_cast<uint32_t>(A.per_warp), R.n - first));
   unsigned char* const base = sm + static_cast<size_t>(warp) * A.per_warp * A.pitch;
 
@@ -571,21 +749,28 @@ __global__ void __launch_bounds__(kTileWarps * 32) tile_kernel(const __grid_cons
   if (has_y) y = static_cast<uint32_t>(y64);
   const uint32_t skew = static_cast<uint32_t>(addr & 15) / sizeof(T);   // elements in front of the row in its first line
   const uint32_t lines = (skew + R.vocab + kPer - 1) / kPer;
-  unsigned live_rows = __ballot_sync(0xffffffffu, live);
-  for (int r = 0; r < rows; ++r) {
-    const uint64_t a = __shfl_sync(0xffffffffu, addr, r) & ~15ull;
-    const uint32_t nl = __shfl_sync(0xffffffffu, lines, r);
-    if (!(live_rows >> r & 1)) continue;
-    MO_CHECK((nl + 1) * 16 <= A.pitch);
-    const uint32_t dst = smem_u32(base + static_cast<size_t>(r) * A.pitch);
-    for (uint32_t v = lane; v < nl; v += 32)
-      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + v * 16), "l"(a + v * 16) : "memory");
+  const uint32_t have = live ? lines : 0;
+  // the lots' lines: a lane asks for those that it will sum
+#pragma unroll 1
+  for (int r0 = 0; r0 < rows; r0 += kAtOnce) {
+    const int r = r0 + group;
+    const uint64_t a = (__shfl_sync(0xffffffffu, addr, r & 31) & ~15ull) + gl * 16;
+    const uint32_t nl = __shfl_sync(0xffffffffu, have, r & 31);
+    MO_CHECK(nl == 0 || (nl + 1) * 16 <= A.pitch);
+    MO_CHECK(kL == 0 || nl <= kL * kG);
+    const uint32_t dst = smem_u32(base + static_cast<size_t>(r) * A.pitch) + gl * 16;
+    if (kL > 0) {
+#pragma unroll
+      for (int k = 0; k < kL; ++k)
+        if (gl + k * kG < nl)
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + k * kG * 16), "l"(a + k * kG * 16) : "memory");
+    } else {
+#pragma unroll 4
+      for (uint32_t l = 0; gl + l < nl; l += kG)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + l * 16), "l"(a + l * 16) : "memory");
+    }
   }
   asm volatile("cp.async.commit_group;" ::: "memory");
-  if (kMode == kGradient) {
-    pdl_wait();   // the logits and targets are inputs; the rows' coefficients may come from the launch before
-    if (A.K.pair_loss && tile == 0) sum_pairs(A.K);
-  }
   float adv = 0.f, old_lp = 0.f, ref_lp = 0.f;
   if (kMode == kPolicyLoss && live) {
     adv = A.P.adv.at(seq, tok);
@@ -595,6 +780,8 @@ __global__ void __launch_bounds__(kTileWarps * 32) tile_kernel(const __grid_cons
   // lane r: the row's values; d_j = 2^((z_j - m) c) f, gy at the target
   float m_mine = kNegInf, s_mine = 0.f, f = 0.f, gy = 0.f;
   if (kMode == kGradient) {
+    pdl_wait();   // the logits and targets are inputs; the rows' coefficients may come from the launch before
+    if (A.K.pair_loss && tile == 0) sum_pairs(A.K);
     float coef = 0.f;
     if (live) coef = kept_coef(A.K, first + lane, seq, tok);
     live = live && coef != 0.f;
@@ -605,7 +792,6 @@ __global__ void __launch_bounds__(kTileWarps * 32) tile_kernel(const __grid_cons
       gy = k.gy;
     }
   }
-  if (kMode == kGradient) live_rows = __ballot_sync(0xffffffffu, live);
   asm volatile("cp.async.wait_group 0;" ::: "memory");
   __syncwarp();
 
@@ -614,36 +800,59 @@ __global__ void __launch_bounds__(kTileWarps * 32) tile_kernel(const __grid_cons
   float zy = NAN;
   if (live) {
     if (has_y) {
-      const uint32_t k = skew + y;
-      zy = load_one(reinterpret_cast<const T*>(mine) + k);
-      reinterpret_cast<T*>(mine)[k] = static_cast<T>(kNegInf);
+      T* const at = reinterpret_cast<T*>(mine) + skew + y;
+      zy = load_one(at);
+      *at = static_cast<T>(kNegInf);
     }
     if (kMode != kGradient) {
-      if (skew != 0) keep<T>(mine[0], skew, kPer);
-      keep<T>(mine[lines - 1], 0, skew + R.vocab - (lines - 1) * kPer);
+      const uint32_t tail = skew + R.vocab - (lines - 1) * kPer;
+      if (skew != 0) put_in(mine[0], behind<T>(skew), W::kEmpty);
+      if (tail != kPer) put_out(mine[lines - 1], behind<T>(tail), W::kEmpty);
     }
   }
   __syncwarp();
 
   if (kMode != kGradient) {
+#pragma unroll 1
     for (int r0 = 0; r0 < rows; r0 += kAtOnce) {
       const int r = r0 + group;
-      uint32_t nl = __shfl_sync(0xffffffffu, lines, r & 31);
-      if (r >= rows || !(live_rows >> r & 1)) nl = 0;
-      const uint4* const row = reinterpret_cast<const uint4*>(base + static_cast<size_t>(r) * A.pitch);
+      uint32_t nl = __shfl_sync(0xffffffffu, have, r & 31);
+      if (r >= rows) nl = 0;
+      const uint4* const row = reinterpret_cast<const uint4*>(base + static_cast<size_t>(r) * A.pitch) + gl;
       uint32_t top = W::kEmpty;
-#pragma unroll 4
-      for (uint32_t l = gl; l < nl; l += kG) top = vec_max<T>(top, row[l]);
-      const float m = group_max<kG>(W::top(top));
-      const Ex ex(m, R);
-      float s0 = 0.f, s1 = 0.f;
-#pragma unroll 4
-      for (uint32_t l = gl; l < nl; l += kG) {
-        const Pairs<T> q(row[l]);
+      float s0 = 0.f, s1 = 0.f, m, fix;
+      if (kL > 0) {
+        uint4 v[kL > 0 ? kL : 1];
 #pragma unroll
-        for (int u = 0; u < Pairs<T>::kN; ++u) ex.add(q.p[u], s0, s1);
+        for (int k = 0; k < kL; ++k) {
+          v[k] = make_uint4(W::kEmpty, W::kEmpty, W::kEmpty, W::kEmpty);
+          if (gl + k * kG < nl) v[k] = row[k * kG];
+        }
+#pragma unroll
+        for (int k = 0; k < kL; ++k) top = vec_max<T>(top, v[k]);
+        m = group_max<kG>(W::top(top));
+        const Ex ex(m, R);
+        fix = ex.fix;
+#pragma unroll
+        for (int k = 0; k < kL; ++k) {
+          const Pairs<T> q(v[k]);
+#pragma unroll
+          for (int u = 0; u < Pairs<T>::kN; ++u) ex.add(q.p[u], s0, s1);
+        }
+      } else {
+#pragma unroll 4
+        for (uint32_t l = 0; gl + l < nl; l += kG) top = vec_max<T>(top, row[l]);
+        m = group_max<kG>(W::top(top));
+        const Ex ex(m, R);
+        fix = ex.fix;
+#pragma unroll 4
+        for (uint32_t l = 0; gl + l < nl; l += kG) {
+          const Pairs<T> q(row[l]);
+#pragma unroll
+          for (int u = 0; u < Pairs<T>::kN; ++u) ex.add(q.p[u], s0, s1);
+        }
       }
-      const float s = group_sum<kG>(s0 + s1) * ex.fix;
+      const float s = group_sum<kG>(s0 + s1) * fix;
       const int from = ((lane - r0) & (kAtOnce - 1)) * kG;
       const float mr = __shfl_sync(0xffffffffu, m, from), sr = __shfl_sync(0xffffffffu, s, from);
       if (lane >= r0 && lane < r0 + kAtOnce) {
@@ -652,19 +861,14 @@ __global__ void __launch_bounds__(kTileWarps * 32) tile_kernel(const __grid_cons
       }
     }
     RowStat st = {0.0, 0.0, 0.f, 0.f};
-    double part[4] = {0.0, 0.0, 0.0, 0.0};
     if (live) {
       st = row_stat(zy, m_mine, s_mine, R.inv_t);
       if (kMode == kPolicyLoss) {
-        const RowLoss L = policy_row_loss(st.logp, A.P, old_lp, ref_lp, A.P.ref_lp.p != nullptr, adv);
-        const double w = wt, inv = A.P.div ? 1.0 / static_cast<double>(*A.P.div) : A.P.inv_div;
-        part[0] = w * L.loss * inv;
-        part[1] = w;
-        part[2] = w * L.kl * inv;
-        part[3] = L.clipped ? w : 0.0;
-        const float g = static_cast<float>(w * L.slope * inv * R.inv_t);
-        f = -g * st.f;
-        gy = g * st.rest;
+        const PolicyRow p = policy_row(A.P, st, wt, adv, old_lp, ref_lp, R.inv_t);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) part[k] = p.part[k];
+        f = p.f;
+        gy = p.gy;
       }
     }
     if (lane < rows) {
@@ -676,40 +880,72 @@ __global__ void __launch_bounds__(kTileWarps * 32) tile_kernel(const __grid_cons
         A.coef[row] = 0.f;
       }
     }
-    if (kMode == kPolicyLoss) {
+    if (kMode == kForward) return;
+    if (kMode == kPreference) {
+      cluster_pairs<kTileWarps * 32>(A.pair, A.K);
+      if (A.grad != nullptr && live) {
+        const float coef = __ldcg(A.coef + first + lane), g = static_cast<float>(coef * R.inv_t);
+        live = coef != 0.f;
+        f = -g * st.f;
+        gy = g * st.rest;
+      }
+    } else {
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        const double v = warp_sum(part[k]);
-        if (lane == k) A.partials[static_cast<size_t>(tile) * 4 + k] = v;
+        part[k] = warp_sum(part[k]);
+        if (A.sums == nullptr && lane == k) A.partials[static_cast<size_t>(tile) * 4 + k] = part[k];
       }
     }
+    if (A.grad == nullptr) return;
   }
 
-  if (kMode == kGradient || (kMode == kPolicyLoss && A.grad != nullptr)) {
-    for (int r0 = 0; r0 < rows; r0 += kAtOnce) {
-      const int r = r0 + group;
-      const float m = __shfl_sync(0xffffffffu, m_mine, r & 31), k = __shfl_sync(0xffffffffu, f, r & 31);
-      const uint32_t sk = __shfl_sync(0xffffffffu, skew, r & 31);
-      if (r >= rows) continue;
-      T* const out = static_cast<T*>(A.grad) + static_cast<size_t>(first + r) * R.vocab;
-      const Split<T> so(out, R.vocab);
-      uint4* const ov = reinterpret_cast<uint4*>(out + so.head);
-      const unsigned char* const row = base + static_cast<size_t>(r) * A.pitch;
-      if (!(live_rows >> r & 1)) {
-        for (uint32_t l = gl; l < so.vecs; l += kG) ov[l] = make_uint4(0, 0, 0, 0);
-        for (uint32_t i = gl; i < so.head + so.tail; i += kG) store_one(out + so.edge(i), 0.f);
-        continue;
-      }
-      const Ex ex(m, R);
-      const float kf = k * ex.fix;
-      gradient_lines<T, kG, 2>(ov, row, (sk + so.head) * static_cast<uint32_t>(sizeof(T)), gl, so.vecs, ex, kf);
-      for (uint32_t i = gl; i < so.head + so.tail; i += kG) {
-        const uint32_t j = so.edge(i);
-        store_one(out + j, ex.one(load_one(reinterpret_cast<const T*>(row) + sk + j)) * kf);
-      }
+  const unsigned live_rows = __ballot_sync(0xffffffffu, live);
+#pragma unroll 1
+  for (int r0 = 0; r0 < rows; r0 += kAtOnce) {
+    const int r = r0 + group;
+    const float m = __shfl_sync(0xffffffffu, m_mine, r & 31), k0 = __shfl_sync(0xffffffffu, f, r & 31);
+    const uint32_t sk = __shfl_sync(0xffffffffu, skew, r & 31);
+    if (r >= rows) continue;
+    T* const out = static_cast<T*>(A.grad) + static_cast<size_t>(first + r) * R.vocab;
+    const Split<T> so(out, R.vocab);
+    uint4* const ov = reinterpret_cast<uint4*>(out + so.head);
+    const unsigned char* const row = base + static_cast<size_t>(r) * A.pitch;
+    if (!(live_rows >> r & 1)) {
+      for (uint32_t l = gl; l < so.vecs; l += kG) ov[l] = make_uint4(0, 0, 0, 0);
+      for (uint32_t i = gl; i < so.head + so.tail; i += kG) store_one(out + so.edge(i), 0.f);
+      continue;
     }
-    __syncwarp();   // the targets' elements, written as 0 above
-    if (live && has_y) store_one(static_cast<T*>(A.grad) + static_cast<size_t>(first + lane) * R.vocab + y, gy);
+    const Ex ex(m, R);
+    const float k1 = k0 * ex.fix;
+    const uint32_t off = (sk + so.head) * static_cast<uint32_t>(sizeof(T));
+    if (kL > 0 && (off & 15u) == 0) {
+      const uint4* const in = reinterpret_cast<const uint4*>(row + off) + gl;
+#pragma unroll
+      for (int k = 0; k < kL; ++k)
+        if (gl + k * kG < so.vecs) ov[gl + k * kG] = Pairs<T>(in[k * kG]).scaled(ex, k1);
+    } else {
+      gradient_lines<T, kG, 2>(ov, row, off, gl, so.vecs, ex, k1);
+    }
+    for (uint32_t i = gl; i < so.head + so.tail; i += kG) {
+      const uint32_t j = so.edge(i);
+      store_one(out + j, ex.one(load_one(reinterpret_cast<const T*>(row) + sk + j)) * k1);
+    }
+  }
+  __syncwarp();   // the targets' elements, written as 0 above
+  if (live && has_y) store_one(static_cast<T*>(A.grad) + static_cast<size_t>(first + lane) * R.vocab + y, gy);
+}
+
+template <typename T, int kG, int kL, Mode kMode>
+__global__ void __launch_bounds__(kTileWarps * 32, kMode == kPreference ? 4 : 1) tile_kernel(const __grid_constant__ TileArgs A) {
+  extern __shared__ __align__(16) unsigned char sm[];
+  const bool one_cluster = kMode == kPolicyLoss && A.sums != nullptr;
+  if (kMode != kGradient && kMode != kPreference) pdl_go();
+  if (one_cluster) cluster_arrive_relaxed();
+  double part[4] = {0.0, 0.0, 0.0, 0.0};
+  tile_rows<T, kG, kL, kMode>(A, sm, part);
+  if (kMode == kPolicyLoss && one_cluster) {
+    __syncwarp();
+    cluster_sums<kTileWarps>(part, A.sums);
   }
 }
 
@@ -1125,96 +1361,6 @@ __global__ void __launch_bounds__(kSumThreads) sum_kernel(const __grid_constant_
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
-// The preference loss of a pair (chosen sequence i, rejected sequence i + pairs), one block each: the sums of the two
-// sequences' log-probabilities in 64 bits, u = beta ((s_i - ref_i) - (s_j - ref_j)), and each sequence's coefficient written
-// to its rows.
-struct PairArgs {
-  Rows R;
-  int pairs;
-  const float* ref;      // [2 pairs], or null
-  double beta, eps, inv_div;
-  const float* div;
-  int average;
-  const double* logp64;
-  float* coef;           // [n], or null (no gradient)
-  double* pair_loss;
-  float* rewards;        // [2 pairs]
-  float* seq_logp;       // [2 pairs]
-};
-constexpr int kPairThreads = 256;
-__global__ void __launch_bounds__(kPairThreads) pair_kernel(const __grid_constant__ PairArgs A) {
-  const Rows& R = A.R;
-  __shared__ double sh_s[2][kPairThreads / 32];
-  __shared__ int sh_n[2][kPairThreads / 32];
-  __shared__ float sh_c[2];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  pdl_wait();
-  pdl_go();
-  int64_t b[2], e[2];
-#pragma unroll
-  for (int k = 0; k < 2; ++k) {
-    const int64_t q = blockIdx.x + static_cast<int64_t>(k) * A.pairs, n = R.n;
-    if (R.cu) {   // held to the rows there are
-      b[k] = min(max(static_cast<int64_t>(R.cu[q]), static_cast<int64_t>(0)), n);
-      e[k] = min(max(static_cast<int64_t>(R.cu[q + 1]), b[k]), n);
-    } else {
-      b[k] = q * R.tokens;
-      e[k] = b[k] + R.tokens;
-    }
-    double s = 0.0;
-    int cnt = 0;
-    for (int64_t i = b[k] + threadIdx.x; i < e[k]; i += kPairThreads) {
-      const uint32_t row = static_cast<uint32_t>(i), seq = row / R.tokens, tok = row - seq * R.tokens;
-      MO_CHECK(row < R.n);
-      if (R.y[seq * R.y_seq + tok * R.y_tok] >= 0) {
-        s += A.logp64[i];
-        ++cnt;
-      }
-    }
-    s = warp_sum(s);
-    cnt = __reduce_add_sync(0xffffffffu, cnt);
-    if (lane == 0) {
-      sh_s[k][warp] = s;
-      sh_n[k][warp] = cnt;
-    }
-  }
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    double s[2], n[2], rw[2];
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      double t = 0.0;
-      int c = 0;
-      for (int w = 0; w < kPairThreads / 32; ++w) {
-        t += sh_s[k][w];
-        c += sh_n[k][w];
-      }
-      n[k] = A.average ? static_cast<double>(max(c, 1)) : 1.0;
-      s[k] = t / n[k];
-      const int q = blockIdx.x + k * A.pairs;
-      rw[k] = A.beta * (s[k] - (A.ref ? static_cast<double>(A.ref[q]) : 0.0));
-      A.rewards[q] = static_cast<float>(rw[k]);
-      A.seq_logp[q] = static_cast<float>(s[k]);
-    }
-    const double u = rw[0] - rw[1], inv = A.div ? 1.0 / static_cast<double>(*A.div) : A.inv_div;
-    // -log sigmoid(u) = max(-u, 0) + log1p(e^-|u|); sigmoid(-u) = e^-|u| / (1 + e^-|u|) or 1 / (1 + e^-|u|)
-    const double t = exp(-fabs(u)), l = log1p(t);
-    const double up = (u > 0.0 ? 0.0 : -u) + l, down = (u < 0.0 ? 0.0 : u) + l;
-    const double sn = (u >= 0.0 ? t : 1.0) / (1.0 + t), sp = (u >= 0.0 ? 1.0 : t) / (1.0 + t);
-    A.pair_loss[blockIdx.x] = ((1.0 - A.eps) * up + A.eps * down) * inv;
-    const double du = A.beta * (A.eps * sp - (1.0 - A.eps) * sn) * inv;
-    sh_c[0] = static_cast<float>(du / n[0]);
-    sh_c[1] = static_cast<float>(-du / n[1]);
-  }
-  if (A.coef == nullptr) return;
-  __syncthreads();
-#pragma unroll
-  for (int k = 0; k < 2; ++k) {
-    const float c = sh_c[k];
-    for (int64_t i = b[k] + threadIdx.x; i < e[k]; i += kPairThreads) A.coef[i] = c;
-  }
-}
-
 // The pairs' losses added up where no gradient pass does it
 __global__ void __launch_bounds__(32) pair_sum_kernel(const __grid_constant__ Kept K) {
   pdl_wait();
