@@ -52,11 +52,13 @@ int check_logits(const char* who, const moteopt_logits* z, const moteopt_positio
   R->t = temperature;
   R->inv_t = 1.0 / temperature;
   const double c = kLog2e * R->inv_t;
-  float hi = static_cast<float>(c);
-  if (static_cast<double>(hi) >= c) hi = std::nextafter(hi, 0.f);
+  int exp = 0;
+  double bits = std::floor(std::ldexp(std::frexp(c, &exp), 12));   // c_hi: 12 bits, below c
+  if (std::ldexp(bits, exp - 12) >= c) bits -= 1.0;
+  const float hi = static_cast<float>(std::ldexp(bits, exp - 12));
   R->c_hi = hi;
   R->c_lo = static_cast<float>(c - static_cast<double>(hi));
-  if (!(R->c_lo > 0.f) || !std::isfinite(hi)) return fail(MOTEOPT_ERR_INVALID, w + ": the temperature is out of range");
+  if (!(R->c_lo >= FLT_MIN) || !std::isfinite(hi)) return fail(MOTEOPT_ERR_INVALID, w + ": the temperature is out of range");
   return MOTEOPT_OK;
 }
 
@@ -197,7 +199,14 @@ int launch_slices(int dtype, SliceArgs A, int sms, cudaStream_t st) {
 // so that one that falls behind takes fewer: 4 x 1024 x 32768, 52.4 against 51.1 us.
 constexpr uint32_t kPieceLines = 1024;
 constexpr int kStreamGrid = 4 * 8;   // blocks per SM in all
-int64_t row_pieces(int dtype, int64_t vocab) { return cdiv(line_bytes(dtype, vocab) / 16, kPieceLines); }
+// A row's lines are shared out evenly, in whole batches: about kPieceLines each.
+int64_t row_pieces(int dtype, int64_t vocab) {
+  return std::max<int64_t>(1, (line_bytes(dtype, vocab) / 16 + kPieceLines / 2) / kPieceLines);
+}
+uint32_t piece_lines(int dtype, int64_t vocab) {
+  constexpr int64_t kBatchLines = 32 * kBatch;
+  return static_cast<uint32_t>(cdiv(cdiv(line_bytes(dtype, vocab) / 16, row_pieces(dtype, vocab)), kBatchLines) * kBatchLines);
+}
 size_t parts_bytes(int dtype, int64_t rows, int64_t vocab) {
   return short_rows(dtype, vocab) ? 0 : sizeof(Part) * static_cast<size_t>(rows) * static_cast<size_t>(row_pieces(dtype, vocab));
 }
@@ -222,7 +231,7 @@ int launch_forward(int dtype, const Rows& R, float* logp, float* lse, double* lo
   A.R = R;
   A.pieces = static_cast<uint32_t>(pieces);
   A.n = R.n * A.pieces;
-  A.lines = kPieceLines;
+  A.lines = piece_lines(dtype, R.vocab);
   A.parts = parts;
   const unsigned blocks = static_cast<unsigned>(std::min<int64_t>(cdiv(A.n, kStreamThreads / 32), kStreamGrid * sms));
   MO_TRY(dtype == MOTEOPT_DTYPE_BF16

@@ -28,8 +28,8 @@ namespace loss {
 
 constexpr float kNegInf = -INFINITY;
 constexpr double kLog2e = 1.4426950408889634074;
-// ex2.approx's mean relative error below -1 is -5.05e-8, the same for every binade (measured over 4e6 arguments each). It
-// is a bias, so it would add up over the thousands of positions of a sequence; row_stat takes it out again.
+// ex2.approx's mean relative error below -1 is -5.05e-8, the same for every binade (measured over 4e6 arguments each). A
+// sequence would add up thousands of them.
 constexpr float kEx2Bias = 5.05e-8f;
 constexpr double kLn2 = 0.69314718055994530942;
 
@@ -80,19 +80,49 @@ __device__ __forceinline__ F2 fma2(F2 x, F2 y, F2 z) {
   return r;
 }
 
-// The exponentials of a row about a logit m, two at a time: exp((z - m) / T) = 2^(z c - b) fix with c = c_hi + c_lo =
-// log2(e) / T, b = m c rounded to fp32 and fix = 2^(b - m c). Two multiply-adds: z c_hi - b is exact before its one rounding,
-// which is of the size of the result, and so is the next. (With one float for c, its rounding, 1.3e-8 of log2(e), would lean
-// every exponent of a row the same way.) c_lo > 0 keeps -inf a -inf. Beyond |m| = 2^60, where a product may overflow, any
-// two different logits are at least 2^37 apart: a scale of 2^-20 gives 1 for z = m and 0 below.
+// The exponentials of a row about a logit m, with c = c_hi + c_lo = log2(e) / T: 2^(z c - b) fix is exp(z / T - ref(m)), where
+// ref(m) is m / T rounded to a whole power of two, base(m) = rint(m c). Sums about different m then differ by powers of two,
+// exactly. c_hi has 12 bits, so that what the first multiply-add leaves to the second is not lost under half a unit of its
+// result (with one float for c, or a full one for c_hi, its rounding leans every exponent of a row the same way: 5e-8 of a sum,
+// and the sums of thousands of positions keep it). b is base + 16: ex2 is asked for values below -1 only, where its relative
+// error has the mean of -5.05e-8 that row_stat takes out. c_lo > 0 keeps -inf a -inf.
+//
+// Where |m c| >= 2^18, ref(m) is m / T itself and fix the difference. Beyond |m| = 2^60, where a product may overflow, any two
+// different logits are at least 2^37 apart: a scale of 2^-20 gives 1 for z = m and 0 below.
+constexpr float kAbove = 16.f;
+struct Base {
+  float b;     // rint(m c)
+  bool near;
+  __device__ Base(float m, const Rows& R) {
+    const float p = fmaf(m, R.c_hi, m * R.c_lo);
+    b = rintf(p);
+    near = fabsf(p) < 0x1p18f;   // not of infinities and NaN
+  }
+};
+__device__ __forceinline__ double ref_of(float m, const Rows& R) {
+  const Base b(m, R);
+  return b.near ? b.b * kLn2 : m * R.inv_t;
+}
 struct Ex {
   F2 hi, lo, nb;
   float fix;
   __device__ Ex(float m, const Rows& R) {
-    const bool far = fabsf(m) > 0x1p60f && fabsf(m) < INFINITY;
     if (m == kNegInf) m = 0.f;
-    const float h = far ? 0x1p-20f : R.c_hi, l = far ? 0x1p-149f : R.c_lo, b = m * h;
-    fix = far ? 1.f : fmaf(-(fmaf(m, h, -b) + m * l), 0.69314718f, 1.f);
+    float h = R.c_hi, l = R.c_lo;
+    const Base base(m, R);
+    float b = base.b + kAbove;
+    fix = 65536.f;   // 2^kAbove
+    if (!base.near) {
+      fix = 1.f;
+      if (fabsf(m) > 0x1p60f && fabsf(m) < INFINITY) {
+        h = 0x1p-20f;
+        l = 0x1p-149f;
+        b = m * h;
+      } else {
+        b = fmaf(m, h, m * l);
+        fix = expf(fmaf(m, l, fmaf(m, h, -b)) * -0.69314718f);
+      }
+    }
     hi = pack2(h, h);
     lo = pack2(l, l);
     nb = pack2(-b, -b);
@@ -103,11 +133,10 @@ struct Ex {
     e0 = ex2(t0);
     e1 = ex2(t1);
   }
-  __device__ __forceinline__ void add(F2 z, float& s0, float& s1) const {
+  __device__ __forceinline__ float sum(F2 z) const {
     float e0, e1;
     two(z, e0, e1);
-    s0 += e0;
-    s1 += e1;
+    return e0 + e1;
   }
   __device__ __forceinline__ float one(float z) const {
     float e0, e1;
@@ -115,8 +144,13 @@ struct Ex {
     return e0;
   }
 };
-// exp((m - to) / T), the factor of a partial sum that moves to another maximum: once a thread, by expf
-__device__ __forceinline__ float rescale(float m, float to, float inv_t) { return m == kNegInf ? 0.f : expf((m - to) * inv_t); }
+// exp(ref(m) - ref(to)), the factor of a partial sum that moves from m to a larger logit
+__device__ __forceinline__ float rescale(float m, float to, const Rows& R) {
+  if (m == kNegInf) return 0.f;
+  const Base a(m, R), b(to, R);
+  if (a.near && b.near) return __int_as_float((static_cast<int>(fmaxf(a.b - b.b, -126.f)) + 127) << 23);
+  return expf(static_cast<float>(ref_of(m, R) - ref_of(to, R)));
+}
 
 __device__ __forceinline__ float lo_bf16(uint32_t w) { return __uint_as_float(w << 16); }
 __device__ __forceinline__ float hi_bf16(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
@@ -181,7 +215,8 @@ __device__ __forceinline__ double warp_sum(double v) {
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void pdl_go() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
-// A line's 16 bytes as pairs of fp32: 4 of bf16, 2 of fp32
+// A line's 16 bytes as pairs of fp32: 4 of bf16, 2 of fp32. A line's exponentials are added up before they join a lane's sum:
+// bf16 logits take few values, so the roundings of a long chain of sums lean (20000 of them: 2e-8 of the sum).
 template <typename T>
 struct Pairs;
 template <>
@@ -191,6 +226,9 @@ struct Pairs<__nv_bfloat16> {
   __device__ __forceinline__ explicit Pairs(const uint4& v)
       : p{pack2(lo_bf16(v.x), hi_bf16(v.x)), pack2(lo_bf16(v.y), hi_bf16(v.y)), pack2(lo_bf16(v.z), hi_bf16(v.z)),
           pack2(lo_bf16(v.w), hi_bf16(v.w))} {}
+  __device__ __forceinline__ float sum(const Ex& ex) const {
+    return (ex.sum(p[0]) + ex.sum(p[1])) + (ex.sum(p[2]) + ex.sum(p[3]));
+  }
   __device__ __forceinline__ uint4 scaled(const Ex& ex, float f) const {   // f exp, rounded once
     float a[8];
 #pragma unroll
@@ -209,6 +247,7 @@ struct Pairs<float> {
   __device__ __forceinline__ explicit Pairs(const uint4& v)
       : p{pack2(bits(v.x), bits(v.y)), pack2(bits(v.z), bits(v.w))} {}
   static __device__ __forceinline__ float bits(uint32_t w) { return __uint_as_float(w); }
+  __device__ __forceinline__ float sum(const Ex& ex) const { return ex.sum(p[0]) + ex.sum(p[1]); }
   __device__ __forceinline__ uint4 scaled(const Ex& ex, float f) const {
     float a[4];
     ex.two(p[0], a[0], a[1]);
@@ -217,13 +256,13 @@ struct Pairs<float> {
   }
 };
 
-// (largest logit, sum) of a part of a row
+// (largest logit m, sum of exp(x - ref(m))) of a part of a row
 struct Part {
   float m, s;
 };
-__device__ __forceinline__ Part warp_join(Part p, float inv_t) {
+__device__ __forceinline__ Part warp_join(Part p, const Rows& R) {
   const float M = warp_max(p.m);
-  return Part{M, warp_sum(p.s == 0.f ? 0.f : p.s * rescale(p.m, M, inv_t))};
+  return Part{M, warp_sum(p.s == 0.f ? 0.f : p.s * rescale(p.m, M, R))};
 }
 
 // What a row's sums give (see the top of this file). The differences and the results are in 64 bits; exp, the logarithm and
@@ -232,24 +271,23 @@ __device__ __forceinline__ Part warp_join(Part p, float inv_t) {
 // took a lane 1500 cycles and as many instructions as the row itself.
 struct RowStat {
   double logp, lse;
-  float f;      // exp(m / T - lse): p_j = exp((z_j - m) / T) f
+  float f;      // exp(ref(m) - lse): p_j = exp(x_j - ref(m)) f
   float rest;   // 1 - p_y
 };
-__device__ __forceinline__ RowStat row_stat(float zy, float m, float s, double inv_t) {
-  const double a = (static_cast<double>(zy) - static_cast<double>(m)) * inv_t;
+__device__ __forceinline__ RowStat row_stat(float zy, float m, float s, const Rows& R) {
+  const double x = zy * R.inv_t, ref = ref_of(m, R), a = x - ref;
   const bool up = a >= 0.0;
   const float q = expf(static_cast<float>(up ? -a : a));
   const float X = up ? (s == 0.f ? 0.f : s * q) : (s - 1.f) + q;
   const float u = 1.f + X, inv = 1.f / u;
   const int k = (__float_as_int(u) - 0x3f400000) >> 23;
   const float f = __int_as_float(__float_as_int(u) - (k << 23));
-  // ex2's bias, in the part of the sum that is not the largest element's 1
-  const float bias = kEx2Bias * fmaxf(s - 1.f, 0.f) * (up ? q : 1.f) * inv;
+  const float bias = kEx2Bias * s * (up ? q : 1.f) * inv;   // ex2's, in the others' share of the whole sum
   double l = k * kLn2 + static_cast<double>(logf(f) + (X - (u - 1.f)) * inv + bias);
   if (X != X) l = static_cast<double>(X);
   RowStat r;
   r.logp = up ? -l : a - l;
-  r.lse = static_cast<double>(up ? zy : m) * inv_t + l;
+  r.lse = (up ? x : ref) + l;
   r.f = (up ? q : 1.f) * inv;
   r.rest = (up ? X : s) * inv;
   if (zy == INFINITY) r.logp = r.lse = static_cast<double>(r.f = r.rest = NAN);   // inf - inf
@@ -395,36 +433,33 @@ __device__ __forceinline__ uint4 load_shifted(const unsigned char* p, uint32_t o
 
 // A thread's running maximum and sum. The maximum moves only when a logit is more than kSlack units of log2 above it, so the
 // sum is rescaled hardly ever.
-constexpr float kSlack = 16.f;
+constexpr float kSlack = kAbove - 1.f;
 struct Running {
   float m, s0, s1;
   Ex ex;
   __device__ explicit Running(const Rows& R) : m(kNegInf), s0(0.f), s1(0.f), ex(kNegInf, R) {}
   template <typename T, int kN>
-  __device__ __forceinline__ void add(const uint4 (&v)[kN], const Rows& R, float inv_t) {
+  __device__ __forceinline__ void add(const uint4 (&v)[kN], const Rows& R) {
     using W = Word<T>;
     uint32_t t = W::kEmpty;
 #pragma unroll
     for (int k = 0; k < kN; ++k) t = vec_max<T>(t, v[k]);
     const float top = W::top(t);
     if ((top - m) * R.c_hi > kSlack) {
-      const float by = ex.fix * rescale(m, top, inv_t);
+      const Ex next(top, R);
+      const float by = rescale(m, top, R) * (ex.fix / next.fix);
       s0 *= by;
       s1 *= by;
       m = top;
-      ex = Ex(m, R);
+      ex = next;
     }
 #pragma unroll
-    for (int k = 0; k < kN; ++k) {
-      const Pairs<T> q(v[k]);
-#pragma unroll
-      for (int u = 0; u < Pairs<T>::kN; ++u) ex.add(q.p[u], s0, s1);
-    }
+    for (int k = 0; k < kN; ++k) (k & 1 ? s1 : s0) += Pairs<T>(v[k]).sum(ex);
   }
   __device__ __forceinline__ Part part() const { return Part{m, (s0 + s1) * ex.fix}; }
 };
 
-// Gradient lines [i, n) by kStride of an output row from lines of shared memory `off` bytes from `src`: f 2^((z - m) c)
+// Gradient lines [i, n) by kStride of an output row from lines of shared memory `off` bytes from `src`: f exp(x - ref(m))
 template <typename T, uint32_t kStride, int kUnroll>
 __device__ __forceinline__ void gradient_lines(uint4* __restrict__ out, const unsigned char* src, uint32_t off, uint32_t i,
                                                uint32_t n, const Ex& ex, float f) {
@@ -492,14 +527,14 @@ __device__ __forceinline__ void cluster_sums(const double (&part)[4], float* out
 // The sums of a row from its threads' parts, given to every thread. One block, or a cluster of `cl` blocks whose warps 0
 // write their block's part into every block's shared memory.
 template <int kThreads>
-__device__ __forceinline__ Part row_join(Part p, int cl, uint32_t rank, float inv_t, Part* sh_warp, Part* sh_block) {
+__device__ __forceinline__ Part row_join(Part p, int cl, uint32_t rank, const Rows& R, Part* sh_warp, Part* sh_block) {
   constexpr int kWarps = kThreads / 32;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  p = warp_join(p, inv_t);
+  p = warp_join(p, R);
   if (lane == 0) sh_warp[warp] = p;
   __syncthreads();
   Part b = lane < kWarps ? sh_warp[lane] : Part{kNegInf, 0.f};
-  b = warp_join(b, inv_t);
+  b = warp_join(b, R);
   if (cl > 1) {
     cluster_wait();   // every block of the cluster runs (arrived at its start)
     if (warp == 0) {   // the only writes to be seen by other blocks
@@ -511,7 +546,7 @@ __device__ __forceinline__ Part row_join(Part p, int cl, uint32_t rank, float in
     }
     cluster_wait();
     b = lane < cl ? sh_block[lane] : Part{kNegInf, 0.f};
-    b = warp_join(b, inv_t);
+    b = warp_join(b, R);
   }
   return b;
 }
@@ -528,9 +563,9 @@ struct Kept {
   int pairs;
   float* loss;
 };
-// exp(x_j - lse) = 2^((z_j - m) c) (1 + d) with m = lse T rounded to fp32 and d = m / T - lse, at most 2^-24 lse
+// exp(x_j - lse) = exp(x_j - ref(m)) exp(ref(m) - lse) with m = lse T
 struct KeptRow {
-  float m, f, gy;   // d_j = 2^((z_j - m) c) f, gy at the target
+  float m, f, gy;   // d_j = exp(x_j - ref(m)) f, gy at the target
 };
 __device__ __forceinline__ float kept_coef(const Kept& K, uint32_t row, uint32_t seq, uint32_t tok) {
   return K.coef_row ? K.coef_row[row] : K.coef.at(seq, tok);
@@ -541,7 +576,7 @@ __device__ __forceinline__ KeptRow kept_row(const Kept& K, const Rows& R, uint32
   const float g = static_cast<float>(coef * R.inv_t);
   KeptRow r;
   r.m = static_cast<float>(lse * R.t);
-  r.f = -g * static_cast<float>(1.0 + (r.m * R.inv_t - lse));
+  r.f = -g * expf(static_cast<float>(ref_of(r.m, R) - lse));
   r.gy = -expm1f(lp) * g;
   return r;
 }
@@ -657,7 +692,7 @@ __global__ void __launch_bounds__(kPairThreads) pair_kernel(const __grid_constan
 // pitch, and the maximum and the sum take 3 shuffles for four rows. One lane per row forms the row's values (a warp that
 // formed them for one row at a time would spend as much on them as on the row). Then, for the gradient, the exponentials
 // again from shared memory, by the lines of the output. kL, where it is not 0: no lane has more lines of a row, and the loops
-// over them are unrolled (64 x 1024 x 271 bf16: forward XXX us without, YYY with).
+// over them are unrolled (64 x 1024 x 271 bf16, forward: 14.3 us without, 12.2 with).
 //
 // Many warps, each with one tile, and not few with the next tile already on its way: a warp waits on its own arithmetic more
 // than on memory (with two buffers for half the warps, 16 x 1024 x 4096: policy loss 78 against 57 us).
@@ -777,7 +812,7 @@ __device__ __forceinline__ void tile_rows(const TileArgs& A, unsigned char* sm, 
     old_lp = A.P.old_lp.at(seq, tok);
     if (A.P.ref_lp.p) ref_lp = A.P.ref_lp.at(seq, tok);
   }
-  // lane r: the row's values; d_j = 2^((z_j - m) c) f, gy at the target
+  // lane r: the row's values; d_j = exp(x_j - ref(m)) f, gy at the target
   float m_mine = kNegInf, s_mine = 0.f, f = 0.f, gy = 0.f;
   if (kMode == kGradient) {
     pdl_wait();   // the logits and targets are inputs; the rows' coefficients may come from the launch before
@@ -835,9 +870,7 @@ __device__ __forceinline__ void tile_rows(const TileArgs& A, unsigned char* sm, 
         fix = ex.fix;
 #pragma unroll
         for (int k = 0; k < kL; ++k) {
-          const Pairs<T> q(v[k]);
-#pragma unroll
-          for (int u = 0; u < Pairs<T>::kN; ++u) ex.add(q.p[u], s0, s1);
+          (k & 1 ? s1 : s0) += Pairs<T>(v[k]).sum(ex);
         }
       } else {
 #pragma unroll 4
@@ -847,9 +880,7 @@ __device__ __forceinline__ void tile_rows(const TileArgs& A, unsigned char* sm, 
         fix = ex.fix;
 #pragma unroll 4
         for (uint32_t l = 0; gl + l < nl; l += kG) {
-          const Pairs<T> q(row[l]);
-#pragma unroll
-          for (int u = 0; u < Pairs<T>::kN; ++u) ex.add(q.p[u], s0, s1);
+          s0 += Pairs<T>(row[l]).sum(ex);
         }
       }
       const float s = group_sum<kG>(s0 + s1) * fix;
@@ -862,7 +893,7 @@ __device__ __forceinline__ void tile_rows(const TileArgs& A, unsigned char* sm, 
     }
     RowStat st = {0.0, 0.0, 0.f, 0.f};
     if (live) {
-      st = row_stat(zy, m_mine, s_mine, R.inv_t);
+      st = row_stat(zy, m_mine, s_mine, R);
       if (kMode == kPolicyLoss) {
         const PolicyRow p = policy_row(A.P, st, wt, adv, old_lp, ref_lp, R.inv_t);
 #pragma unroll
@@ -972,7 +1003,6 @@ __global__ void __launch_bounds__(kStreamThreads, kStreamBlocks) stream_kernel(c
   constexpr uint32_t kPer = 16 / sizeof(T), kLines = 32 * kBatch, kElems = kLines * kPer;
   const Rows& R = A.R;
   const uint32_t lane = threadIdx.x & 31, step = gridDim.x * (kStreamThreads / 32);
-  const float inv_t = static_cast<float>(R.inv_t);
   uint32_t piece = blockIdx.x * (kStreamThreads / 32) + (threadIdx.x >> 5);
   pdl_go();
   if (piece >= A.n) return;
@@ -1058,11 +1088,11 @@ __global__ void __launch_bounds__(kStreamThreads, kStreamBlocks) stream_kernel(c
         for (uint32_t k = 0; k < kBatch; ++k)
           if (there / kPer == lane + 32 * k) drop_target<T>(v[k], there % kPer);
       }
-      run.add<T>(v, R, inv_t);
+      run.add<T>(v, R);
       done += kLines;
       if (done >= b.x) break;
     }
-    const Part p = warp_join(run.part(), inv_t);
+    const Part p = warp_join(run.part(), R);
     if (lane == 0) A.parts[piece] = p;
   }
   asm volatile("cp.async.wait_group 0;" ::: "memory");
@@ -1091,7 +1121,6 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
   float zy = NAN;
   if (y >= 0 && y < static_cast<int64_t>(R.vocab))
     zy = load_one(reinterpret_cast<const T*>(R.z) + (seq * R.z_seq + tok * R.z_tok) + y);
-  const float inv_t = static_cast<float>(R.inv_t);
   pdl_wait();
   RowStat st = {0.0, 0.0, 0.f, 0.f};
   if (y >= 0) {
@@ -1099,11 +1128,11 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
     for (uint32_t i = lane; i < A.pieces; i += 32) {
       const Part q = A.parts[static_cast<size_t>(row) * A.pieces + i];
       const float M = fmaxf(p.m, q.m);
-      p.s = (p.s == 0.f ? 0.f : p.s * rescale(p.m, M, inv_t)) + (q.s == 0.f ? 0.f : q.s * rescale(q.m, M, inv_t));
+      p.s = (p.s == 0.f ? 0.f : p.s * rescale(p.m, M, R)) + (q.s == 0.f ? 0.f : q.s * rescale(q.m, M, R));
       p.m = M;
     }
-    p = warp_join(p, inv_t);
-    st = row_stat(zy, p.m, p.s, R.inv_t);
+    p = warp_join(p, R);
+    st = row_stat(zy, p.m, p.s, R);
   }
   if (lane == 0) {
     if (A.logp) A.logp[row] = static_cast<float>(st.logp);
@@ -1122,6 +1151,9 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
 // it loaded itself; the blocks' parts meet in distributed shared memory; one thread forms the row's values, and all go over
 // the slice again for the gradient, by the lines of the output.
 //
+// What bounds it is the two exponentials of a logit and the arithmetic around them (4 x 1024 x 32768 bf16: 106 us, 0.77 of the
+// copy bandwidth's time; the special-function units are busy for 0.63 of it). Blocks that stay, and ask for the next row's
+// lines while they store this one's gradient, took 115 us.
 // Exponentials again instead of kept ones: 32 fp32 exponentials a thread in registers left two blocks of 512 threads an SM,
 // whose chain of load, cluster exchange and row values then stands between them (8192 rows of 131072: 1497 us).
 struct SliceArgs {
@@ -1179,7 +1211,6 @@ __global__ void __launch_bounds__(kThreads, kThreads == 128 ? 6 : 3) slice_kerne
   const uint32_t lines = e1 > e0 ? (skew + (e1 - e0) + kPer - 1) / kPer : 0;
   MO_CHECK(lines <= share + 3);
   const uint32_t dst = smem_u32(sm);
-  const float inv_t = static_cast<float>(R.inv_t);
   for (uint32_t i = threadIdx.x; i < lines; i += kThreads)
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + i * 16), "l"((a0 & ~15ull) + i * 16ull) : "memory");
   asm volatile("cp.async.commit_group;" ::: "memory");
@@ -1207,16 +1238,16 @@ __global__ void __launch_bounds__(kThreads, kThreads == 128 ? 6 : 3) slice_kerne
   uint32_t at = threadIdx.x;
   for (; at + 3 * kThreads < lines; at += 4 * kThreads) {
     const uint4 v[4] = {line[at], line[at + kThreads], line[at + 2 * kThreads], line[at + 3 * kThreads]};
-    run.add<T>(v, R, inv_t);
+    run.add<T>(v, R);
   }
 #pragma unroll 1
   for (; at < lines; at += kThreads) {
     const uint4 v[1] = {line[at]};
-    run.add<T>(v, R, inv_t);
+    run.add<T>(v, R);
   }
-  const Part p = row_join<kThreads>(run.part(), A.cl, rank, inv_t, sh_warp, sh_block);
+  const Part p = row_join<kThreads>(run.part(), A.cl, rank, R, sh_warp, sh_block);
   if (threadIdx.x == 0) {
-    const RowStat st = row_stat(sh_in[0], p.m, p.s, R.inv_t);
+    const RowStat st = row_stat(sh_in[0], p.m, p.s, R);
     const RowLoss L = policy_row_loss(st.logp, A.P, sh_in[2], sh_in[3], A.P.ref_lp.p != nullptr, sh_in[1]);
     const double w = A.P.weight.p ? A.P.weight.at(seq, tok) : 1.f;
     const double inv = A.P.div ? 1.0 / static_cast<double>(*A.P.div) : A.P.inv_div;
@@ -1256,7 +1287,8 @@ struct GradArgs {
   void* grad;
   uint32_t pieces;        // blocks per row
 };
-constexpr int kGradThreads = 256, kGradVecs = 4;
+// 4096 rows of 131072 bf16 at 256 x 4 lines a block 356 us, 128 x 4 344, 128 x 8 341, 512 x 2 437
+constexpr int kGradThreads = 128, kGradVecs = 8;
 
 template <typename T>
 __global__ void __launch_bounds__(kGradThreads) grad_kernel(const __grid_constant__ GradArgs A) {
@@ -1314,7 +1346,11 @@ __global__ void __launch_bounds__(kGradThreads) grad_kernel(const __grid_constan
   for (int k = 0; k < kGradVecs; ++k) {
     const uint32_t at = begin + k * kGradThreads;
     if (at >= so.vecs) break;
-    ov[at] = Pairs<T>(by ? shift_lines(v[k], w[k], by) : v[k]).scaled(ex, f);
+    const uint4 d = Pairs<T>(by ? shift_lines(v[k], w[k], by) : v[k]).scaled(ex, f);
+    // the preference loss has read the logits before: a gradient that leaves L2 first leaves them there (4 x 1024 x 32768
+    // bf16: 137 against 147 us)
+    if (A.K.pair_loss) __stcs(ov + at, d);
+    else ov[at] = d;
     const uint32_t e = so.head + at * kPer;
     if (y - e < kPer) store_one(out + y, r.gy);
   }
