@@ -358,7 +358,8 @@ MOTEOPT_API int moteopt_selftest_wait_timeout(int mode, double limit_seconds, in
  *
  * The logits are [seqs][tokens][vocab], fp32 or bf16, the last axis contiguous and the others with strides (in elements),
  * so a shifted view needs no copy; packed sequences are seqs = 1. `targets` are int64. For a position with logits z,
- * x = z / temperature and target y: lse = log sum_j exp x_j, logp = x_y - lse. A position whose target is negative does
+ * x = z / temperature (a product with the fp32 reciprocal, as torch divides by a number) and target y:
+ * lse = log sum_j exp x_j, logp = x_y - lse. A position whose target is negative does
  * not count: its logits are not read, its logp and lse are 0, its gradient is 0. A target >= vocab gives NaN. -inf logits
  * have probability 0. Gradients are written contiguous, [seqs][tokens][vocab], in the logits' type, each rounded once;
  * the sums behind them are fp32 within a thread and fp64 above, in a fixed order, so the same call gives the same bits.
