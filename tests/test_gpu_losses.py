@@ -14,8 +14,8 @@ pytestmark = pytest.mark.gpu
 BF, F32 = torch.bfloat16, torch.float32
 # (sequences, positions, vocabulary): a vocabulary of one, words, warps and 16-byte lines and one beside them, the byte
 # vocabulary, the limits of the warp-per-rows kernels (4592 bf16 and 2296 fp32 logits), slices of one block and of clusters
-# of 2 to 16, and the longest fp32 row
-SIZES = [(1, 1, 1), (2, 3, 1), (3, 5, 2), (2, 7, 3), (4, 9, 17), (2, 33, 64), (5, 31, 271), (1, 1, 271), (3, 2, 2296),
+# of 2 to 16, the longest fp32 row, and so many short rows that a warp takes several and their sums go through two stages
+SIZES = [(1, 1, 1), (2, 3, 1), (9, 80, 271), (10, 3500, 33), (3, 5, 2), (2, 7, 3), (4, 9, 17), (2, 33, 64), (5, 31, 271), (1, 1, 271), (3, 2, 2296),
          (3, 2, 2297), (2, 2, 1100), (2, 3, 4592), (2, 2, 4593), (1, 3, 8193), (80, 2, 16384), (1, 2, 16391), (2, 80, 50021),
          (1, 1, 131072), (1, 1, 262144), (1, 2, 262160), (1, 1, 900864)]
 
@@ -430,6 +430,32 @@ def test_a_post_training_step_through_the_optimizer(dev):
             ws.append(W.detach().clone())
         moved = float((ws[1] - W0).norm())
         assert moved > 0.1 and float((ws[0] - ws[1]).norm()) < 1e-3 * moved, kind
+
+
+def test_offsets_past_32_bits(dev):
+    """A gradient of more than 2^32 elements from one expanded row, short rows and long ones, and rows of logits that lie more
+    than 2^32 bytes apart."""
+    from mote_b200 import policy_loss, token_logprobs, token_logprobs_backward
+    if torch.cuda.get_device_properties(dev).total_memory < 60e9:
+        pytest.skip("needs 60 GB")
+    gen = torch.Generator().manual_seed(1)
+    for V, n in ((131072, 33000), (272, 15_900_000)):
+        z = torch.randn(1, V, generator=gen).to(BF).to(dev).expand(n, V)
+        y = torch.full((n,), V - 3, device=dev)
+        r = token_logprobs(z[:2], y[:2])
+        lp, ls = r.logprobs[:1].expand(n), r.lse[:1].expand(n)
+        d = token_logprobs_backward(z, y, lp, ls, torch.ones(1, device=dev).expand(n))
+        assert d.numel() > 2 ** 32 and bool(d[0].any())
+        assert _same(d[-1], d[0]) and _same(d[n // 2], d[0])
+        p = policy_loss(z, y, torch.ones(n, device=dev), lp)
+        assert _same(p.grad[-1], p.grad[0]) and float(p.count) == n and float(p.logprobs[-1]) == float(r.logprobs[0])
+        del d, p
+    base = torch.zeros((3 << 30) + 300, dtype=BF, device=dev)
+    z = base.as_strided((3, 271), ((3 << 29) + 7, 1), 5)
+    z.copy_(torch.randn(3, 271, generator=gen))
+    y = torch.tensor([4, 200, 270], device=dev)
+    want, _ = ref.row_values(z.cpu(), y.cpu(), 1.0)
+    assert_close(token_logprobs(z, y).logprobs, want, U * want.abs() + ref.spread(z.cpu(), 1.0), "far rows")
 
 
 def test_refusals(dev):
