@@ -202,14 +202,23 @@ int launch_slices(int dtype, SliceArgs A, int sms, cudaStream_t st) {
 // so that one that falls behind takes fewer: 4 x 1024 x 32768, 52.4 against 51.1 us.
 constexpr uint32_t kPieceLines = 1024;
 constexpr int kStreamGrid = 4 * 8;   // blocks per SM in all
-// A row's lines are shared out evenly, in whole batches: about kPieceLines each.
-int64_t row_pieces(int dtype, int64_t vocab) {
-  return std::max<int64_t>(1, (line_bytes(dtype, vocab) / 16 + kPieceLines / 2) / kPieceLines);
-}
-uint32_t piece_lines(int dtype, int64_t vocab) {
+// A row's lines are shared out in whole batches, in the number of pieces of 5/8 to 5/4 of kPieceLines that leaves the last one
+// the least short.
+struct PieceShape {
+  int64_t pieces, lines;
+};
+PieceShape piece_shape(int dtype, int64_t vocab) {
   constexpr int64_t kBatchLines = 32 * kBatch;
-  return static_cast<uint32_t>(cdiv(cdiv(line_bytes(dtype, vocab) / 16, row_pieces(dtype, vocab)), kBatchLines) * kBatchLines);
+  const int64_t all = line_bytes(dtype, vocab) / 16;
+  const int64_t least = std::max<int64_t>(1, cdiv(all * 4, kPieceLines * 5)), most = std::max(least, all * 8 / (kPieceLines * 5));
+  PieceShape best = {0, 0};
+  for (int64_t p = least; p <= most; ++p) {
+    const int64_t lines = cdiv(cdiv(all, p), kBatchLines) * kBatchLines;
+    if (best.pieces == 0 || p * lines < best.pieces * best.lines) best = {p, lines};
+  }
+  return best;
 }
+int64_t row_pieces(int dtype, int64_t vocab) { return piece_shape(dtype, vocab).pieces; }
 size_t parts_bytes(int dtype, int64_t rows, int64_t vocab) {
   return short_rows(dtype, vocab) ? 0 : sizeof(Part) * static_cast<size_t>(rows) * static_cast<size_t>(row_pieces(dtype, vocab));
 }
@@ -234,7 +243,7 @@ int launch_forward(int dtype, const Rows& R, float* logp, float* lse, double* lo
   A.R = R;
   A.pieces = static_cast<uint32_t>(pieces);
   A.n = R.n * A.pieces;
-  A.lines = piece_lines(dtype, R.vocab);
+  A.lines = static_cast<uint32_t>(piece_shape(dtype, R.vocab).lines);
   A.parts = parts;
   const unsigned blocks = static_cast<unsigned>(std::min<int64_t>(cdiv(A.n, kStreamThreads / 32), kStreamGrid * sms));
   MO_TRY(dtype == MOTEOPT_DTYPE_BF16

@@ -1231,8 +1231,9 @@ __global__ void __launch_bounds__(kThreads, kThreads == 128 ? 6 : 3) slice_kerne
   // a thread's own lines: what lies beside the slice in the first and the last one, and the target, become -inf
   uint4* const line = reinterpret_cast<uint4*>(sm);
   const uint32_t len = e1 - e0, ty = y - e0 < len ? skew + (y - e0) : 0xffffffffu;
-  if (threadIdx.x == 0 && skew != 0 && lines > 0) keep<T>(line[0], skew, kPer);
-  if (lines > 0 && threadIdx.x == (lines - 1) % kThreads) keep<T>(line[lines - 1], 0, skew + len - (lines - 1) * kPer);
+  if (threadIdx.x == 0 && skew != 0 && lines > 0) put_in(line[0], behind<T>(skew), W::kEmpty);
+  if (lines > 0 && threadIdx.x == (lines - 1) % kThreads)
+    put_out(line[lines - 1], behind<T>(skew + len - (lines - 1) * kPer), W::kEmpty);
   if (ty != 0xffffffffu && threadIdx.x == ty / kPer % kThreads) drop_target<T>(line[ty / kPer], ty % kPer);
   Running run(R);
   uint32_t at = threadIdx.x;
