@@ -967,7 +967,7 @@ __device__ __forceinline__ void tile_rows(const TileArgs& A, unsigned char* sm, 
 }
 
 template <typename T, int kG, int kL, Mode kMode>
-__global__ void __launch_bounds__(kTileWarps * 32, kMode == kPreference ? 4 : 1) tile_kernel(const __grid_constant__ TileArgs A) {
+__global__ void __launch_bounds__(kTileWarps * 32, kMode == kPreference ? 4 : 8) tile_kernel(const __grid_constant__ TileArgs A) {
   extern __shared__ __align__(16) unsigned char sm[];
   const bool one_cluster = kMode == kPolicyLoss && A.sums != nullptr;
   if (kMode != kGradient && kMode != kPreference) pdl_go();
