@@ -362,7 +362,8 @@ MOTEOPT_API int moteopt_selftest_wait_timeout(int mode, double limit_seconds, in
  * lse = log sum_j exp x_j, logp = x_y - lse. A position whose target is negative does
  * not count: its logits are not read, its logp and lse are 0, its gradient is 0. A target >= vocab gives NaN. -inf logits
  * have probability 0. Gradients are written contiguous, [seqs][tokens][vocab], in the logits' type, each rounded once;
- * the sums behind them are fp32 within a thread and fp64 above, in a fixed order, so the same call gives the same bits.
+ * the sums behind them are fp32 within a row and fp64 above, in a fixed order, so the same call gives the same bits.
+ * Outputs and workspaces must not overlap the inputs.
  * At most 2^27 - 1 positions, and at most 3,603,456 bytes a row (1,801,728 bf16 or 900,864 fp32 logits). */
 typedef struct moteopt_logits {
   const void* data;
@@ -414,7 +415,8 @@ MOTEOPT_API int moteopt_policy_loss(const moteopt_logits* logits, const moteopt_
 typedef struct moteopt_preference {
   int64_t sequences;
   const int32_t* cu_seqlens;        /* NULL: sequence q is logits' seq q. Else (logits->seqs == 1) device, sequences + 1
-                                       ascending row offsets; rows outside [first, last) do not count */
+                                       ascending row offsets, held to [0, tokens]; rows outside [first, last) do not
+                                       count */
   const float* ref_logprobs;        /* device [sequences], or NULL: 0 */
   double beta, label_smoothing;
   int average;

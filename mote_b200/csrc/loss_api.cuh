@@ -6,7 +6,7 @@ namespace {
 
 using namespace moteopt::loss;
 
-// Rows of up to this many bytes take the warp-per-rows kernels, longer ones a block each.
+// Rows of up to this many bytes take tile_kernel, a warp for several rows; longer ones a block or more each.
 constexpr int64_t kShortBytes = kTileBytes - 32;
 
 constexpr int64_t kSliceBytes = 72 * 1024, kSliceMost = 220 * 1024, kSliceLeast = 8 * 1024;

@@ -4,18 +4,17 @@
 //
 // Per row (one position) with logits z, temperature T, x = z / T and target y:
 //   logp = x_y - lse(x),  dlogp/dz_j = ([j == y] - exp(x_j - lse)) / T
-// The target's column is kept out of the sum: with m the largest of the OTHER logits, s = sum_{j != y} exp(x_j - m/T) and
-// a = x_y - m/T,
+// The target's column is kept out of the sum: with m the largest of the OTHER logits, ref(m) = m / T to a whole power of two
+// (see Ex), s = sum_{j != y} exp(x_j - ref(m)) and a = x_y - ref(m),
 //   a >= 0: logp = -log1p(s e^-a)          1 - p_y = X / (1 + X), X = s e^-a
 //   a <  0: logp = a - log1p(s - 1 + e^a)  1 - p_y = s / (s + e^a)
 // so that neither logp nor 1 - p_y cancels where the model is sure of its target (p_y -> 1). The exponentials and their sums
 // are fp32, a position's logp is kept in 64 bits, and the sums over positions are in 64 bits.
 //
 // All kernels are memory-bound in principle (2 or 4 bytes read per logit, as many written for a gradient); the exponential
-// is next: one ex2 per logit at 16 per clock and SM is 0.73 of the copy bandwidth's rate for bf16 logits read once.
+// is next: one ex2 per logit at 16 per clock and SM takes 0.73 of the time in which the copy bandwidth reads a bf16 logit.
 #pragma once
 
-#include <cooperative_groups.h>
 #include <cstdint>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -39,7 +38,7 @@ struct Rows {
   const int64_t* y;
   int64_t z_seq, z_tok;   // strides in elements
   int64_t y_seq, y_tok;
-  uint32_t n;             // rows: seqs * tokens, below 2^31
+  uint32_t n;             // rows: seqs * tokens, below 2^27
   uint32_t tokens;
   uint32_t vocab;
   const int32_t* cu;      // packed: n_seqs + 1 row offsets, or null. Rows outside [cu[0], cu[n_seqs]) do not count
@@ -616,9 +615,11 @@ __device__ __forceinline__ void pair_loss(const PairArgs& A, uint32_t pair) {   
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
     const int64_t q = pair + static_cast<int64_t>(k) * A.pairs, n = R.n;
-    if (R.cu) {   // held to the rows there are
-      b[k] = min(max(static_cast<int64_t>(R.cu[q]), static_cast<int64_t>(0)), n);
-      e[k] = min(max(static_cast<int64_t>(R.cu[q + 1]), b[k]), n);
+    if (R.cu) {   // held to the rows there are, between the first offset and the last (in_packed)
+      const int64_t lo = max(static_cast<int64_t>(R.cu[0]), static_cast<int64_t>(0));
+      const int64_t hi = min(static_cast<int64_t>(R.cu[R.n_seqs]), n);
+      b[k] = min(max(static_cast<int64_t>(R.cu[q]), lo), max(lo, hi));
+      e[k] = min(max(static_cast<int64_t>(R.cu[q + 1]), b[k]), max(b[k], hi));
     } else {
       b[k] = q * R.tokens;
       e[k] = b[k] + R.tokens;
@@ -663,7 +664,8 @@ __device__ __forceinline__ void pair_loss(const PairArgs& A, uint32_t pair) {   
     const double t = exp(-fabs(u)), l = log1p(t);
     const double up = (u > 0.0 ? 0.0 : -u) + l, down = (u < 0.0 ? 0.0 : u) + l;
     const double q = 1.0 / (1.0 + t), sn = (u >= 0.0 ? t : 1.0) * q, sp = (u >= 0.0 ? 1.0 : t) * q;
-    A.pair_loss[pair] = ((1.0 - A.eps) * up + A.eps * down) * inv;
+    // a term without weight is left out: with a target of probability 0 on one side, the other term is infinite
+    A.pair_loss[pair] = ((A.eps < 1.0 ? (1.0 - A.eps) * up : 0.0) + (A.eps > 0.0 ? A.eps * down : 0.0)) * inv;
     const double du = A.beta * (A.eps * sp - (1.0 - A.eps) * sn) * inv;
     sh_c[0] = static_cast<float>(du / n[0]);
     sh_c[1] = static_cast<float>(-du / n[1]);
@@ -697,9 +699,9 @@ __global__ void __launch_bounds__(kPairThreads) pair_kernel(const __grid_constan
 // Many warps, each with one tile, and not few with the next tile already on its way: a warp waits on its own arithmetic more
 // than on memory (with two buffers for half the warps, 16 x 1024 x 4096: policy loss 78 against 57 us).
 constexpr int kTileWarps = 4;
-constexpr int kTileRows = 8;           // most rows of a tile: 64 x 1024 x 271 bf16, forward, at 4, 8 and 16 rows: 16.2, 14.5
-                                       // and 18.2 us (fewer rows: more of a warp's instructions are not its rows'; more: too
-                                       // few warps an SM), policy loss 31.7, 27.5 and 31.2 us
+constexpr int kTileRows = 8;           // most rows of a tile: 64 x 1024 x 271 bf16, forward, at 4, 8 and 16 rows, loops not
+                                       // unrolled: 16.2, 14.5 and 18.2 us (fewer rows: more of a warp's instructions are not
+                                       // its rows'; more: too few warps an SM), policy loss 31.7, 27.5 and 31.2 us
 constexpr int kTileBytes = 9216;       // most bytes of a tile: 6 blocks of 4 warps in an SM's shared memory
 enum Mode { kForward, kPolicyLoss, kGradient, kPreference };   // kPreference: of one cluster
 
@@ -1151,8 +1153,8 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
 // it loaded itself; the blocks' parts meet in distributed shared memory; one thread forms the row's values, and all go over
 // the slice again for the gradient, by the lines of the output.
 //
-// What bounds it is the two exponentials of a logit and the arithmetic around them (4 x 1024 x 32768 bf16: 106 us, 0.77 of the
-// copy bandwidth's time; the special-function units are busy for 0.63 of it). Blocks that stay, and ask for the next row's
+// What bounds it is the two exponentials of a logit and the arithmetic around them (4 x 1024 x 32768 bf16: 109 us, 0.75 of the
+// copy bandwidth's rate; the special-function units are busy for 0.64 of it). Blocks that stay, and ask for the next row's
 // lines while they store this one's gradient, took 115 us.
 // Exponentials again instead of kept ones: 32 fp32 exponentials a thread in registers left two blocks of 512 threads an SM,
 // whose chain of load, cluster exchange and row values then stands between them (8192 rows of 131072: 1497 us).

@@ -119,7 +119,7 @@ def preference_loss(logits: torch.Tensor, targets: torch.Tensor, ref_logprobs: O
                     grad: bool = True) -> PreferenceLoss:
     """The paired preference loss, and its gradient in the logits (dpo.py's loop). The sequences are the chosen ones, then
     the rejected ones in the same order: [S, T, V] logits with S even, or [N, V] with `cu_seqlens` (int32, S + 1 ascending
-    row offsets on the device; rows outside them do not count). With s a sequence's summed log-probability (its mean with
+    row offsets on the device, held to [0, N]; rows outside them do not count). With s a sequence's summed log-probability (its mean with
     `average`; 0 where no position counts) and ref_logprobs [S] the reference model's (none: 0):
 
         u = beta ((s_i - ref_i) - (s_j - ref_j)),  j = i + S / 2
