@@ -467,7 +467,7 @@ int moteopt_policy_loss(const moteopt_logits* logits, const moteopt_positions* t
       return launch_tile_cluster<kPolicyLoss>(logits->dtype, A, s, st);
     }
     MO_TRY(launch_tile<kPolicyLoss>(logits->dtype, A, s, st));
-    return launch_sums(partials, s.tiles, mid, sums, st);
+    return launch_sums(partials, cdiv(s.tiles, kTileWarps), mid, sums, st);
   }
   SliceArgs A;
   std::memset(&A, 0, sizeof(A));

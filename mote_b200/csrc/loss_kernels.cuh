@@ -495,23 +495,17 @@ __device__ __forceinline__ void store_remote(void* local, uint32_t rank, float a
 
 constexpr int kMaxCluster = 16;
 
-// The sums of one cluster's warps' terms, in a fixed order: lane 0 of each warp has them
-template <int kWarps>
-__device__ __forceinline__ void cluster_sums(const double (&part)[4], float* out) {
-  __shared__ double sh[kWarps][4], sh_block[kMaxCluster][4];
+// The four sums of one cluster's blocks' terms, in a fixed order: the threads with `has` hold their block's term k
+__device__ __forceinline__ void cluster_sums(double part, bool has, int k, float* out) {
+  __shared__ double sh_block[kMaxCluster][4];
   const uint32_t rank = cluster_rank();
   uint32_t blocks;
   asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(blocks));
-  if ((threadIdx.x & 31) == 0)
-    for (int k = 0; k < 4; ++k) sh[threadIdx.x >> 5][k] = part[k];
-  __syncthreads();
   cluster_wait();   // every block runs (arrived at its start)
-  if (threadIdx.x < 4) {
-    double t = 0.0;
-    for (int w = 0; w < kWarps; ++w) t += sh[w][threadIdx.x];
+  if (has) {
     uint32_t dst;
-    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(dst) : "r"(smem_u32(&sh_block[rank][threadIdx.x])), "r"(0));
-    asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(dst), "d"(t) : "memory");
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(dst) : "r"(smem_u32(&sh_block[rank][k])), "r"(0));
+    asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(dst), "d"(part) : "memory");
   }
   __syncwarp();
   cluster_arrive();
@@ -691,10 +685,13 @@ __global__ void __launch_bounds__(kPairThreads) pair_kernel(const __grid_constan
 // line may hold up to 15 bytes beside the row: the same aligned line, so nothing beyond the allocation), which lifts every
 // alignment and stride question and keeps all of a tile in flight at once. kG lanes work on a row in lines of 16 bytes,
 // 32 / kG rows at a time: the quarter of a warp that shared memory serves at once reads 128 bytes in a row whatever the rows'
-// pitch, and the maximum and the sum take 3 shuffles for four rows. One lane per row forms the row's values (a warp that
-// formed them for one row at a time would spend as much on them as on the row). Then, for the gradient, the exponentials
-// again from shared memory, by the lines of the output. kL, where it is not 0: no lane has more lines of a row, and the loops
-// over them are unrolled (64 x 1024 x 271 bf16, forward: 14.3 us without, 12.2 with).
+// pitch, and the maximum and the sum take 3 shuffles for four rows. kL, where it is not 0: no lane has more lines of a row, and
+// the loops over them are unrolled (64 x 1024 x 271 bf16, forward: 14.3 us without, 12.2 with).
+//
+// One warp of the block then forms the values of all its rows, a lane each (64 x 1024 x 271 bf16, policy loss: 22.6 us; with
+// each warp for its own rows, on 8 of its lanes, 24.6. The gradient from kept values needs no sums: a barrier for its rows' few
+// values costs more, 13.8 against 13.4 us, than it saves). Then, for the gradient, the exponentials again from shared memory,
+// by the lines of the output.
 //
 // Many warps, each with one tile, and not few with the next tile already on its way: a warp waits on its own arithmetic more
 // than on memory (with two buffers for half the warps, 16 x 1024 x 4096: policy loss 78 against 57 us).
@@ -715,7 +712,7 @@ struct TileArgs {
   float* coef;
   Policy P;
   void* grad;                          // [n][vocab], or null
-  double* partials;                    // [warps][4] (policy)
+  double* partials;                    // [blocks][4] (policy)
   float* sums;                         // or, of one cluster, the sums themselves
   Kept K;                              // (gradient)
   PairArgs pair;                       // (preference)
@@ -752,36 +749,33 @@ __device__ __forceinline__ void cluster_pairs(const PairArgs& A, const Kept& K) 
 }
 
 template <typename T, int kG, int kL, Mode kMode>
-__device__ __forceinline__ void tile_rows(const TileArgs& A, unsigned char* sm, double (&part)[4]) {
+__device__ __forceinline__ void tile_rows(const TileArgs& A, unsigned char* sm, int chosen, double& sum) {
   using W = Word<T>;
   constexpr uint32_t kPer = 16 / sizeof(T);
   constexpr int kAtOnce = 32 / kG;
+  __shared__ float4 sh_row[kTileWarps * kTileRows];   // (m, s, target logit, counts), then (m, f, gy, counts)
   const Rows& R = A.R;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = lane / kG;
   const uint32_t gl = lane % kG;
-  const uint32_t tile = blockIdx.x * kTileWarps + warp;
-  const uint32_t first = tile * static_cast<uint32_t>(A.per_warp);
-  if (first >= R.n) {
-    if (kMode == kPreference) cluster_pairs<kTileWarps * 32>(A.pair, A.K);
-    return;
-  }
-  const int rows = static_cast<int>(min(static_cast<uint32_t>(A.per_warp), R.n - first));
+  const uint32_t all = blockIdx.x * kTileWarps * static_cast<uint32_t>(A.per_warp);   // the block's first row
+  const int block_rows = all < R.n ? static_cast<int>(min(static_cast<uint32_t>(kTileWarps * A.per_warp), R.n - all)) : 0;
+  const uint32_t first = all + warp * static_cast<uint32_t>(A.per_warp);
+  const int rows = max(0, min(A.per_warp, block_rows - warp * A.per_warp));
   unsigned char* const base = sm + static_cast<size_t>(warp) * A.per_warp * A.pitch;
+  float4* const own = sh_row + warp * A.per_warp;
 
   // lane r: its row
-  uint32_t seq = 0, tok = 0, y = 0;
+  uint32_t y = 0;
   int64_t y64 = -1;
   uint64_t addr = 0;
-  float wt = 1.f;
+  bool live = false;
   if (lane < rows) {
-    const uint32_t row = first + lane;
-    seq = row / R.tokens;
-    tok = row - seq * R.tokens;
+    const uint32_t row = first + lane, seq = row / R.tokens, tok = row - seq * R.tokens;
     y64 = in_packed(R, row) ? R.y[seq * R.y_seq + tok * R.y_tok] : -1;
     addr = reinterpret_cast<uint64_t>(R.z) + (seq * R.z_seq + tok * R.z_tok) * sizeof(T);
-    if (kMode == kPolicyLoss && A.P.weight.p) wt = A.P.weight.at(seq, tok);
+    live = y64 >= 0;
+    if (kMode == kPolicyLoss && A.P.weight.p) live = live && A.P.weight.at(seq, tok) != 0.f;
   }
-  bool live = y64 >= 0 && wt != 0.f;
   const bool has_y = live && y64 < static_cast<int64_t>(R.vocab);
   if (has_y) y = static_cast<uint32_t>(y64);
   const uint32_t skew = static_cast<uint32_t>(addr & 15) / sizeof(T);   // elements in front of the row in its first line
@@ -808,48 +802,50 @@ __device__ __forceinline__ void tile_rows(const TileArgs& A, unsigned char* sm, 
     }
   }
   asm volatile("cp.async.commit_group;" ::: "memory");
-  float adv = 0.f, old_lp = 0.f, ref_lp = 0.f;
-  if (kMode == kPolicyLoss && live) {
+
+  // the chosen warp's lane r: the inputs of the block's row r
+  const bool values = warp == chosen && lane < block_rows;
+  float wt = 1.f, adv = 0.f, old_lp = 0.f, ref_lp = 0.f;
+  if (kMode == kPolicyLoss && values) {
+    const uint32_t row = all + lane, seq = row / R.tokens, tok = row - seq * R.tokens;
+    if (A.P.weight.p) wt = A.P.weight.at(seq, tok);
     adv = A.P.adv.at(seq, tok);
     old_lp = A.P.old_lp.at(seq, tok);
     if (A.P.ref_lp.p) ref_lp = A.P.ref_lp.at(seq, tok);
   }
-  // lane r: the row's values; d_j = exp(x_j - ref(m)) f, gy at the target
-  float m_mine = kNegInf, s_mine = 0.f, f = 0.f, gy = 0.f;
   if (kMode == kGradient) {
     pdl_wait();   // the logits and targets are inputs; the rows' coefficients may come from the launch before
-    if (A.K.pair_loss && tile == 0) sum_pairs(A.K);
-    float coef = 0.f;
-    if (live) coef = kept_coef(A.K, first + lane, seq, tok);
-    live = live && coef != 0.f;
-    if (live) {
-      const KeptRow k = kept_row(A.K, R, first + lane, seq, tok, coef);
-      m_mine = k.m;
-      f = k.f;
-      gy = k.gy;
+    if (A.K.pair_loss && blockIdx.x == 0 && warp == 0) sum_pairs(A.K);
+    if (lane < rows) {
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+      const uint32_t row = first + lane, seq = row / R.tokens, tok = row - seq * R.tokens;
+      const float coef = live ? kept_coef(A.K, row, seq, tok) : 0.f;
+      if (coef != 0.f) {
+        const KeptRow k = kept_row(A.K, R, row, seq, tok, coef);
+        v = make_float4(k.m, k.f, k.gy, 1.f);
+      }
+      own[lane] = v;
     }
   }
   asm volatile("cp.async.wait_group 0;" ::: "memory");
   __syncwarp();
 
-  // lane r: takes the target out of its row, and what lies beside the row in its first and last line
-  uint4* const mine = reinterpret_cast<uint4*>(base + static_cast<size_t>(lane) * A.pitch);
-  float zy = NAN;
-  if (live) {
-    if (has_y) {
-      T* const at = reinterpret_cast<T*>(mine) + skew + y;
-      zy = load_one(at);
-      *at = static_cast<T>(kNegInf);
-    }
-    if (kMode != kGradient) {
+  if (kMode != kGradient) {
+    // lane r: takes the target out of its row, and what lies beside the row in its first and last line
+    uint4* const mine = reinterpret_cast<uint4*>(base + static_cast<size_t>(lane) * A.pitch);
+    float zy = NAN;
+    if (live) {
+      if (has_y) {
+        T* const at = reinterpret_cast<T*>(mine) + skew + y;
+        zy = load_one(at);
+        *at = static_cast<T>(kNegInf);
+      }
       const uint32_t tail = skew + R.vocab - (lines - 1) * kPer;
       if (skew != 0) put_in(mine[0], behind<T>(skew), W::kEmpty);
       if (tail != kPer) put_out(mine[lines - 1], behind<T>(tail), W::kEmpty);
     }
-  }
-  __syncwarp();
-
-  if (kMode != kGradient) {
+    if (lane < rows) own[lane] = make_float4(kNegInf, 0.f, zy, live ? 1.f : 0.f);
+    __syncwarp();
 #pragma unroll 1
     for (int r0 = 0; r0 < rows; r0 += kAtOnce) {
       const int r = r0 + group;
@@ -886,70 +882,74 @@ __device__ __forceinline__ void tile_rows(const TileArgs& A, unsigned char* sm, 
         }
       }
       const float s = group_sum<kG>(s0 + s1) * fix;
-      const int from = ((lane - r0) & (kAtOnce - 1)) * kG;
-      const float mr = __shfl_sync(0xffffffffu, m, from), sr = __shfl_sync(0xffffffffu, s, from);
-      if (lane >= r0 && lane < r0 + kAtOnce) {
-        m_mine = mr;
-        s_mine = sr;
-      }
+      if (gl == 0 && r < rows) *reinterpret_cast<float2*>(own + r) = make_float2(m, s);
     }
-    RowStat st = {0.0, 0.0, 0.f, 0.f};
-    if (live) {
-      st = row_stat(zy, m_mine, s_mine, R);
-      if (kMode == kPolicyLoss) {
-        const PolicyRow p = policy_row(A.P, st, wt, adv, old_lp, ref_lp, R.inv_t);
+    __syncthreads();
+    if (warp == chosen) {
+      const float4 v = values ? sh_row[lane] : make_float4(0.f, 0.f, 0.f, 0.f);
+      const bool counts = v.w != 0.f;
+      RowStat st = {0.0, 0.0, 0.f, 0.f};
+      double part[4] = {0.0, 0.0, 0.0, 0.0};
+      if (counts) {
+        st = row_stat(v.z, v.x, v.y, R);
+        if (kMode == kPolicyLoss) {
+          const PolicyRow p = policy_row(A.P, st, wt, adv, old_lp, ref_lp, R.inv_t);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) part[k] = p.part[k];
-        f = p.f;
-        gy = p.gy;
+          for (int k = 0; k < 4; ++k) part[k] = p.part[k];
+          st.f = p.f;
+          st.rest = p.gy;
+        }
       }
-    }
-    if (lane < rows) {
-      const uint32_t row = first + lane;
-      if (A.logp) A.logp[row] = static_cast<float>(st.logp);
-      if (A.lse) A.lse[row] = static_cast<float>(st.lse);
-      if (A.logp64) {
-        A.logp64[row] = st.logp;
-        A.coef[row] = 0.f;
+      if (values) {
+        const uint32_t row = all + lane;
+        if (A.logp) A.logp[row] = static_cast<float>(st.logp);
+        if (A.lse) A.lse[row] = static_cast<float>(st.lse);
+        if (A.logp64) {
+          A.logp64[row] = st.logp;
+          A.coef[row] = 0.f;
+        }
+        if (kMode != kForward) sh_row[lane] = make_float4(v.x, st.f, st.rest, v.w);
+      }
+      if (kMode == kPolicyLoss) {   // lane k < 4: the block's sum k
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const double t = warp_sum(part[k]);
+          if (lane == k) sum = t;
+        }
+        if (A.sums == nullptr && lane < 4) A.partials[static_cast<size_t>(blockIdx.x) * 4 + lane] = sum;
       }
     }
     if (kMode == kForward) return;
     if (kMode == kPreference) {
       cluster_pairs<kTileWarps * 32>(A.pair, A.K);
-      if (A.grad != nullptr && live) {
+      if (lane < rows) {
         const float coef = __ldcg(A.coef + first + lane), g = static_cast<float>(coef * R.inv_t);
-        live = coef != 0.f;
-        f = -g * st.f;
-        gy = g * st.rest;
+        const float4 v = own[lane];
+        own[lane] = make_float4(v.x, -g * v.y, g * v.z, coef != 0.f ? v.w : 0.f);
       }
-    } else {
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        part[k] = warp_sum(part[k]);
-        if (A.sums == nullptr && lane == k) A.partials[static_cast<size_t>(tile) * 4 + k] = part[k];
-      }
+      __syncwarp();
     }
     if (A.grad == nullptr) return;
   }
+  if (kMode == kPolicyLoss) __syncthreads();
 
-  const unsigned live_rows = __ballot_sync(0xffffffffu, live);
 #pragma unroll 1
   for (int r0 = 0; r0 < rows; r0 += kAtOnce) {
     const int r = r0 + group;
-    const float m = __shfl_sync(0xffffffffu, m_mine, r & 31), k0 = __shfl_sync(0xffffffffu, f, r & 31);
     const uint32_t sk = __shfl_sync(0xffffffffu, skew, r & 31);
     if (r >= rows) continue;
+    const float4 v = own[r];
     T* const out = static_cast<T*>(A.grad) + static_cast<size_t>(first + r) * R.vocab;
     const Split<T> so(out, R.vocab);
     uint4* const ov = reinterpret_cast<uint4*>(out + so.head);
     const unsigned char* const row = base + static_cast<size_t>(r) * A.pitch;
-    if (!(live_rows >> r & 1)) {
+    if (v.w == 0.f) {
       for (uint32_t l = gl; l < so.vecs; l += kG) ov[l] = make_uint4(0, 0, 0, 0);
       for (uint32_t i = gl; i < so.head + so.tail; i += kG) store_one(out + so.edge(i), 0.f);
       continue;
     }
-    const Ex ex(m, R);
-    const float k1 = k0 * ex.fix;
+    const Ex ex(v.x, R);
+    const float k1 = v.y * ex.fix;
     const uint32_t off = (sk + so.head) * static_cast<uint32_t>(sizeof(T));
     if (kL > 0 && (off & 15u) == 0) {
       const uint4* const in = reinterpret_cast<const uint4*>(row + off) + gl;
@@ -964,8 +964,11 @@ __device__ __forceinline__ void tile_rows(const TileArgs& A, unsigned char* sm, 
       store_one(out + j, ex.one(load_one(reinterpret_cast<const T*>(row) + sk + j)) * k1);
     }
   }
-  __syncwarp();   // the targets' elements, written as 0 above
-  if (live && has_y) store_one(static_cast<T*>(A.grad) + static_cast<size_t>(first + lane) * R.vocab + y, gy);
+  __syncwarp();   // the targets' elements, written above
+  if (has_y) {
+    const float4 v = own[lane];
+    if (v.w != 0.f) store_one(static_cast<T*>(A.grad) + static_cast<size_t>(first + lane) * R.vocab + y, v.z);
+  }
 }
 
 template <typename T, int kG, int kL, Mode kMode>
@@ -974,11 +977,14 @@ __global__ void __launch_bounds__(kTileWarps * 32, kMode == kPreference ? 4 : 8)
   const bool one_cluster = kMode == kPolicyLoss && A.sums != nullptr;
   if (kMode != kGradient && kMode != kPreference) pdl_go();
   if (one_cluster) cluster_arrive_relaxed();
-  double part[4] = {0.0, 0.0, 0.0, 0.0};
-  tile_rows<T, kG, kL, kMode>(A, sm, part);
-  if (kMode == kPolicyLoss && one_cluster) {
+  // the block's rows' values are formed by one warp, another one in the next block: a warp's number is its scheduler's
+  const int chosen = blockIdx.x % kTileWarps;
+  double sum = 0.0;
+  tile_rows<T, kG, kL, kMode>(A, sm, chosen, sum);
+  if (one_cluster) {
+    const int lane = threadIdx.x & 31;
     __syncwarp();
-    cluster_sums<kTileWarps>(part, A.sums);
+    cluster_sums(sum, static_cast<int>(threadIdx.x >> 5) == chosen && lane < 4, lane, A.sums);
   }
 }
 
