@@ -60,7 +60,7 @@ def build_binding(force: bool = False, verbose: bool = False) -> Path:
     cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *[a for d in inc for a in ("-I", d)],
            str(BINDING_SOURCE), "-o", str(tmp), *[a for d in ext.library_paths("cuda") for a in ("-L", d)], "-lc10",
-           "-lc10_cuda", "-ltorch_cpu", "-ltorch_python"]
+           "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python"]
     if verbose:
         print(" ".join(cmd), flush=True)
     r = subprocess.run(cmd, capture_output=True, text=True)

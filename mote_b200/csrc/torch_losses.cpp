@@ -6,7 +6,7 @@
 #include <Python.h>
 
 #include <ATen/core/Tensor.h>
-#include <ATen/ops/empty.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/core/impl/LocalDispatchKeySet.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -115,6 +115,12 @@ at::Tensor element(const at::Tensor& v, int64_t i) {
   return t;
 }
 
+// an uninitialised tensor on z's device, from PyTorch's caching allocator without the dispatcher
+at::Tensor make(at::IntArrayRef sizes, at::ScalarType type, const at::Tensor& z) {
+  return at::detail::empty_cuda(sizes, type, z.device(), std::nullopt);
+}
+at::Tensor scratch(size_t bytes, const at::Tensor& z) { return make({static_cast<int64_t>(bytes)}, at::kByte, z); }
+
 void checked(int rc, const char* what) {
   if (rc != MOTEOPT_OK) refuse(lib_error, std::string(what) + " failed (" + std::to_string(rc) + "): " + api.last_error());
 }
@@ -168,11 +174,10 @@ PyObject* token_logprobs(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const moteopt_positions Y = targets_of(y, z);
     const double t = number(a[2]);
     const c10::cuda::CUDAGuard guard(z.device());
-    const auto f32 = z.options().dtype(at::kFloat);
-    const at::Tensor logp = at::empty(y.sizes(), f32), lse = at::empty(y.sizes(), f32);
+    const at::Tensor logp = make(y.sizes(), at::kFloat, z), lse = make(y.sizes(), at::kFloat, z);
     const size_t bytes = api.logprobs_size(&L);
     at::Tensor ws;
-    if (bytes > kHeader) ws = at::empty({static_cast<int64_t>(bytes)}, z.options().dtype(at::kByte));
+    if (bytes > kHeader) ws = scratch(bytes, z);
     checked(api.token_logprobs(&L, &Y, t, logp.data_ptr<float>(), lse.data_ptr<float>(),
                                ws.defined() ? ws.data_ptr() : nullptr, ws.defined() ? bytes : 0, stream_of(z)),
             "moteopt_token_logprobs");
@@ -191,7 +196,7 @@ PyObject* token_logprobs_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const moteopt_positions G = positions_of(a[4], y, "grad_logprobs", true);
     const double t = number(a[5]);
     const c10::cuda::CUDAGuard guard(z.device());
-    const at::Tensor grad = at::empty(z.sizes(), z.options());
+    const at::Tensor grad = make(z.sizes(), z.scalar_type(), z);
     checked(api.token_logprobs_backward(&L, &Y, t, &P, &S, &G, grad.data_ptr(), stream_of(z)),
             "moteopt_token_logprobs_backward");
     return wrap(grad);
@@ -221,12 +226,11 @@ PyObject* policy_loss(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const bool with_grad = truth(a[12]);
     if (P.kl_coef != 0.0 && a[4] == Py_None) refuse(PyExc_ValueError, "policy_loss: kl_coef needs ref_logprobs");
     const c10::cuda::CUDAGuard guard(z.device());
-    const auto f32 = z.options().dtype(at::kFloat);
     const size_t bytes = api.policy_size(&L);
-    const at::Tensor ws = at::empty({static_cast<int64_t>(bytes)}, z.options().dtype(at::kByte));
-    const at::Tensor sums = at::empty({4}, f32), logp = at::empty(y.sizes(), f32);
+    const at::Tensor ws = scratch(bytes, z);
+    const at::Tensor sums = make({4}, at::kFloat, z), logp = make(y.sizes(), at::kFloat, z);
     at::Tensor grad;
-    if (with_grad) grad = at::empty(z.sizes(), z.options());
+    if (with_grad) grad = make(z.sizes(), z.scalar_type(), z);
     checked(api.policy(&L, &Y, &P, t, sums.data_ptr<float>(), logp.data_ptr<float>(), with_grad ? grad.data_ptr() : nullptr,
                        ws.data_ptr(), bytes, stream_of(z)),
             "moteopt_policy_loss");
@@ -273,12 +277,12 @@ PyObject* preference_loss(PyObject*, PyObject* const* a, Py_ssize_t n) {
     P.divisor_device = scalar_of(a[9], z);
     const bool with_grad = truth(a[10]);
     const c10::cuda::CUDAGuard guard(z.device());
-    const auto f32 = z.options().dtype(at::kFloat);
     const size_t bytes = api.preference_size(&L, P.sequences);
-    const at::Tensor ws = at::empty({static_cast<int64_t>(bytes)}, z.options().dtype(at::kByte));
-    const at::Tensor loss = at::empty({}, f32), rewards = at::empty({P.sequences}, f32), logp = at::empty({P.sequences}, f32);
+    const at::Tensor ws = scratch(bytes, z);
+    const at::Tensor loss = make({}, at::kFloat, z), rewards = make({P.sequences}, at::kFloat, z);
+    const at::Tensor logp = make({P.sequences}, at::kFloat, z);
     at::Tensor grad;
-    if (with_grad) grad = at::empty(z.sizes(), z.options());
+    if (with_grad) grad = make(z.sizes(), z.scalar_type(), z);
     checked(api.preference(&L, &Y, &P, t, loss.data_ptr<float>(), rewards.data_ptr<float>(), logp.data_ptr<float>(),
                            with_grad ? grad.data_ptr() : nullptr, ws.data_ptr(), bytes, stream_of(z)),
             "moteopt_preference_loss");

@@ -49,6 +49,8 @@ def test_offsets_are_held_to_the_rows(dev, V):  # noqa: F811
     for wild in (cut(-7, 5, 12), cut(0, 5, 13), cut(-(2 ** 31), 5, 2 ** 31 - 1)):
         got = preference_loss(z, y, cu_seqlens=wild)
         assert all(_same(a, b) for a, b in zip(got, want))
+    none = preference_loss(z[:0], y[:0], cu_seqlens=cut(4, 5, 7))   # no rows at all: log 2
+    assert abs(float(none.loss) - math.log(2.0)) < 1e-6 and none.grad.shape == (0, V)
     # not ascending: a sequence that ends before it begins is empty
     r = preference_loss(z, y, cu_seqlens=cut(8, 3, 12))
     assert float(r.logprobs[0]) == 0.0 and math.isfinite(float(r.loss)) and not bool(r.grad[:8].any())
