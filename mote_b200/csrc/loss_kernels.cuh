@@ -622,20 +622,20 @@ __device__ __forceinline__ void pair_loss(const PairArgs& A, uint32_t pair) {   
       b[k] = q * R.tokens;
       e[k] = b[k] + R.tokens;
     }
-    const auto add = [&](int64_t i) {
-      const uint32_t row = static_cast<uint32_t>(i);
-      MO_CHECK(row < R.n);
-      sum[k] += __ldcg(A.logp64 + i);   // 0 where a position does not count
-      if (A.average) {
-        const uint32_t seq = row / R.tokens, tok = row - seq * R.tokens;
-        if (R.y[seq * R.y_seq + tok * R.y_tok] >= 0) ++cnt[k];
+    if (A.average) {
+      for (int64_t i = b[k] + threadIdx.x; i < e[k]; i += kThreads) {
+        const uint32_t row = static_cast<uint32_t>(i), seq = row / R.tokens, tok = row - seq * R.tokens;
+        MO_CHECK(row < R.n);
+        if (R.y[seq * R.y_seq + tok * R.y_tok] >= 0) {
+          sum[k] += __ldcg(A.logp64 + i);
+          ++cnt[k];
+        }
       }
-    };
-    if (kShort) {
+    } else if (kShort) {   // logp64 is 0 where a position does not count
 #pragma unroll 1
-      for (int64_t i = b[k] + threadIdx.x; i < e[k]; i += kThreads) add(i);
+      for (int64_t i = b[k] + threadIdx.x; i < e[k]; i += kThreads) sum[k] += __ldcg(A.logp64 + i);
     } else {
-      for (int64_t i = b[k] + threadIdx.x; i < e[k]; i += kThreads) add(i);
+      for (int64_t i = b[k] + threadIdx.x; i < e[k]; i += kThreads) sum[k] += __ldcg(A.logp64 + i);
     }
   }
 #pragma unroll
