@@ -263,8 +263,9 @@ def run(state):
             return {"grad": mote.token_logprobs_backward(z, y, state["logprobs"], state["lse"], state["grad_logprobs"],
                                                          temperature=t)}
         if c["op"] == "policy":
+            kl_coef = 0.04 if c["ref"] else 0.0   # no reference model: no KL term
             r = mote.policy_loss(z, y, state["advantages"], state["old_logprobs"], state["ref_logprobs"],
-                                 weights=state["weights"], clip_low=0.2, clip_high=0.2, kl_coef=0.04, temperature=t,
+                                 weights=state["weights"], clip_low=0.2, clip_high=0.2, kl_coef=kl_coef, temperature=t,
                                  divisor=float(c["tokens"]))
             return {"loss": r.loss, "count": r.count, "kl": r.kl, "clipped": r.clipped, "logprobs": r.logprobs,
                     "grad": r.grad}
