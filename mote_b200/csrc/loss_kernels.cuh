@@ -15,6 +15,7 @@
 // is next: one ex2 per logit at 16 per clock and SM takes 0.73 of the time in which the copy bandwidth reads a bf16 logit.
 #pragma once
 
+#include <cfloat>
 #include <cstdint>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -105,7 +106,7 @@ __device__ __forceinline__ double ref_of(float m, const Rows& R) {
 struct Ex {
   F2 hi, lo, nb;
   float fix;
-  __device__ Ex(float m, const Rows& R) {
+  __device__ Ex(float m, const Rows& R, float up = 0.f) {   // up: a power of two that the values carry (policy_row)
     if (m == kNegInf) m = 0.f;
     float h = R.c_hi, l = R.c_lo;
     const Base base(m, R);
@@ -124,6 +125,7 @@ struct Ex {
     }
     hi = pack2(h, h);
     lo = pack2(l, l);
+    b -= up;
     nb = pack2(-b, -b);
   }
   __device__ __forceinline__ void two(F2 z, float& e0, float& e1) const {
@@ -294,8 +296,11 @@ __device__ __forceinline__ RowStat row_stat(float zy, float m, float s, const Ro
 }
 
 // The policy loss of one row, unscaled by the weight and the divisor. The ratio is an fp32 exponential of a 64-bit
-// difference, and taken in 64 bits where it lies within 1e-5 of a border, at which the gradient jumps. k(d) = e^d - d - 1 is
-// its series below 1 in size (the difference would cancel): 2 / (n + 2)! falls below 2^-24 at n = 9.
+// difference, and taken in 64 bits where it lies within 1e-5 of a border, at which the gradient jumps, and beyond e^80, where
+// fp32 ends: an advantage or a weight may bring what it gives back into range. A ratio of a finite difference stays finite, so
+// that an advantage of 0 makes it 0. k(d) = e^d - d - 1 is its series below 1 in size (the difference would cancel):
+// 2 / (n + 2)! falls below 2^-24 at n = 9.
+constexpr double kFarLog = 80.0;
 struct RowLoss {
   double loss, kl, slope;   // slope: dloss/dlogp
   bool clipped;
@@ -304,7 +309,10 @@ __device__ __forceinline__ RowLoss policy_row_loss(double logp, const Policy& P,
                                                    float adv) {
   const double A = adv, d_old = logp - static_cast<double>(old_lp);
   double r = expf(static_cast<float>(d_old));
-  if (fabs(r - P.clip_hi) < 1e-5 * P.clip_hi || fabs(r - P.clip_lo) < 1e-5 * P.clip_lo) r = exp(d_old);
+  if (d_old > kFarLog || fabs(r - P.clip_hi) < 1e-5 * P.clip_hi || fabs(r - P.clip_lo) < 1e-5 * P.clip_lo) {
+    r = exp(d_old);
+    if (d_old < INFINITY) r = fmin(r, DBL_MAX);
+  }
   const double held_r = fmin(fmax(r, P.clip_lo), P.clip_hi);
   const double free = r * A, held = (r != r ? r : held_r) * A;
   RowLoss L;
@@ -313,34 +321,55 @@ __device__ __forceinline__ RowLoss policy_row_loss(double logp, const Policy& P,
   L.slope = L.clipped ? 0.0 : -free;
   L.kl = 0.0;
   if (has_ref) {
-    const float d = static_cast<float>(static_cast<double>(ref_lp) - logp), e = expm1f(d);
-    float k = e - d;
-    if (fabsf(d) < 1.f) {
-      k = 1.f / 11.f;
+    const double far = static_cast<double>(ref_lp) - logp;
+    double e;
+    if (far > kFarLog) {   // the 1 is below 64 bits
+      e = exp(far);
+      L.kl = e - far;
+    } else {
+      const float d = static_cast<float>(far), m1 = expm1f(d);
+      float k = m1 - d;
+      if (fabsf(d) < 1.f) {
+        k = 1.f / 11.f;
 #pragma unroll
-      for (int n = 10; n >= 3; --n) k = fmaf(k, d, 1.f) * (1.f / n);
-      k = fmaf(k, d, 1.f) * (0.5f * d * d);
+        for (int n = 10; n >= 3; --n) k = fmaf(k, d, 1.f) * (1.f / n);
+        k = fmaf(k, d, 1.f) * (0.5f * d * d);
+      }
+      L.kl = k;
+      e = m1;
     }
-    L.kl = k;
     if (P.kl != 0.0) {
       L.loss += P.kl * L.kl;
-      L.slope -= P.kl * static_cast<double>(e);
+      L.slope -= P.kl * e;
     }
   }
   return L;
 }
 
-// The policy loss of a row: its sums' terms, and its gradient's factors
+// The policy loss of a row: its sums' terms, and its gradient's factors: 2^up f exp(x_j - ref(m)), gy at the target. A slope
+// beyond 2^96 stays in 64 bits to the factors, and what is left above 2^64 goes into the exponents (Ex): products with small
+// probabilities are finite then, and those with a probability of 0 are 0.
 struct PolicyRow {
   double part[4];
-  float f, gy;
+  float f, gy, up;
 };
 __device__ __forceinline__ PolicyRow policy_row(const Policy& P, const RowStat& st, float wt, float adv, float old_lp,
                                                 float ref_lp, double inv_t) {
   const RowLoss L = policy_row_loss(st.logp, P, old_lp, ref_lp, P.ref_lp.p != nullptr, adv);
-  const double w = wt, inv = P.div ? 1.0 / static_cast<double>(*P.div) : P.inv_div;
-  const float g = static_cast<float>(w * L.slope * inv * inv_t);
-  return PolicyRow{{w * L.loss * inv, w, w * L.kl * inv, L.clipped ? w : 0.0}, -g * st.f, g * st.rest};
+  const double w = wt, inv = P.div ? 1.0 / static_cast<double>(*P.div) : P.inv_div, slope = w * L.slope * inv * inv_t;
+  const float g = static_cast<float>(slope);
+  PolicyRow r = {{w * L.loss * inv, w, w * L.kl * inv, L.clipped ? w : 0.0}, -g * st.f, g * st.rest, 0.f};
+  if (fabsf(g) >= 0x1p96f) {   // not of NaN
+    const double h = fmin(fmax(slope, -0x1p1020), 0x1p1020);
+    double f = -h * st.f;
+    while (fabs(f) >= 0x1p64) {
+      f *= 0x1p-64;
+      r.up += 64.f;
+    }
+    r.f = static_cast<float>(f);
+    r.gy = static_cast<float>(h * st.rest);
+  }
+  return r;
 }
 
 __device__ __forceinline__ bool in_packed(const Rows& R, uint32_t row) {
@@ -771,7 +800,7 @@ __device__ __forceinline__ void tile_rows(const TileArgs& A, unsigned char* sm, 
   using W = Word<T>;
   constexpr uint32_t kPer = 16 / sizeof(T);
   constexpr int kAtOnce = 32 / kG;
-  __shared__ float4 sh_row[kTileWarps * kTileRows];   // (m, s, target logit, counts), then (m, f, gy, counts)
+  __shared__ float4 sh_row[kTileWarps * kTileRows];   // (m, s, target logit, counts), then (m, f, gy, counts: 1 + up)
   const Rows& R = A.R;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = lane / kG;
   const uint32_t gl = lane % kG;
@@ -908,6 +937,7 @@ __device__ __forceinline__ void tile_rows(const TileArgs& A, unsigned char* sm, 
       const bool counts = v.w != 0.f;
       RowStat st = {0.0, 0.0, 0.f, 0.f};
       double part[4] = {0.0, 0.0, 0.0, 0.0};
+      float up = 0.f;
       if (counts) {
         st = row_stat(v.z, v.x, v.y, R);
         if (kMode == kPolicyLoss) {
@@ -916,6 +946,7 @@ __device__ __forceinline__ void tile_rows(const TileArgs& A, unsigned char* sm, 
           for (int k = 0; k < 4; ++k) part[k] = p.part[k];
           st.f = p.f;
           st.rest = p.gy;
+          up = p.up;
         }
       }
       if (values) {
@@ -926,7 +957,7 @@ __device__ __forceinline__ void tile_rows(const TileArgs& A, unsigned char* sm, 
           A.logp64[row] = st.logp;
           A.coef[row] = 0.f;
         }
-        if (kMode != kForward) sh_row[lane] = make_float4(v.x, st.f, st.rest, v.w);
+        if (kMode != kForward) sh_row[lane] = make_float4(v.x, st.f, st.rest, v.w + up);
       }
       if (kMode == kPolicyLoss) {   // lane k < 4: the block's sum k
 #pragma unroll
@@ -966,7 +997,7 @@ __device__ __forceinline__ void tile_rows(const TileArgs& A, unsigned char* sm, 
       for (uint32_t i = gl; i < so.head + so.tail; i += kG) store_one(out + so.edge(i), 0.f);
       continue;
     }
-    const Ex ex(v.x, R);
+    const Ex ex(v.x, R, kMode == kPolicyLoss ? v.w - 1.f : 0.f);
     const float k1 = v.y * ex.fix;
     const uint32_t off = (sk + so.head) * static_cast<uint32_t>(sizeof(T));
     if (kL > 0 && (off & 15u) == 0) {
@@ -1197,7 +1228,7 @@ __global__ void __launch_bounds__(kThreads, kThreads == 128 ? 6 : 3) slice_kerne
   using W = Word<T>;
   constexpr uint32_t kPer = 16 / sizeof(T);
   __shared__ Part sh_warp[kThreads / 32], sh_block[kMaxCluster];
-  __shared__ float sh_g[2];
+  __shared__ float sh_g[3];
   __shared__ float sh_in[4];   // the row's target logit, advantage, old and reference log-probability
   const Rows& R = A.R;
   const uint32_t rank = A.cl > 1 ? cluster_rank() : 0;
@@ -1275,24 +1306,21 @@ __global__ void __launch_bounds__(kThreads, kThreads == 128 ? 6 : 3) slice_kerne
   const Part p = row_join<kThreads>(run.part(), A.cl, rank, R, sh_warp, sh_block);
   if (threadIdx.x == 0) {
     const RowStat st = row_stat(sh_in[0], p.m, p.s, R);
-    const RowLoss L = policy_row_loss(st.logp, A.P, sh_in[2], sh_in[3], A.P.ref_lp.p != nullptr, sh_in[1]);
-    const double w = A.P.weight.p ? A.P.weight.at(seq, tok) : 1.f;
-    const double inv = A.P.div ? 1.0 / static_cast<double>(*A.P.div) : A.P.inv_div;
-    const float g = static_cast<float>(w * L.slope * inv * R.inv_t);
-    sh_g[0] = -g * st.f;
-    sh_g[1] = g * st.rest;
+    const float wt = A.P.weight.p ? A.P.weight.at(seq, tok) : 1.f;
+    const PolicyRow v = policy_row(A.P, st, wt, sh_in[1], sh_in[2], sh_in[3], R.inv_t);
+    sh_g[0] = v.f;
+    sh_g[1] = v.gy;
+    sh_g[2] = v.up;
     if (rank == 0) {
       A.logp[row] = static_cast<float>(st.logp);
       double* const o = A.partials + static_cast<size_t>(row) * 4;
-      o[0] = w * L.loss * inv;
-      o[1] = w;
-      o[2] = w * L.kl * inv;
-      o[3] = L.clipped ? w : 0.0;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) o[k] = v.part[k];
     }
   }
   if (A.grad == nullptr) return;
   __syncthreads();
-  const Ex ex(p.m, R);
+  const Ex ex(p.m, R, sh_g[2]);
   const float f = sh_g[0] * ex.fix, gy = sh_g[1];
   if (je != 0xffffffffu) {
     const T* const x = reinterpret_cast<const T*>(sm) + skew + (je - e0);

@@ -1,0 +1,85 @@
+"""The losses on logits where fp32 ends: ratios and KL terms beyond e^88, logits far from 0, log-probabilities of one size and
+logits of another. Tolerances: tests/loss_reference.py."""
+
+import math
+
+import pytest
+import torch
+
+from tests import loss_reference as ref
+from tests.loss_reference import U, assert_close, assert_rounded, cpu_case
+from tests.test_gpu_losses import BF, F32, dev  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+# one cluster of tiles, many blocks of them, 32 lanes a row, slices of one block and of a cluster
+ROWS = [(1, 24, 271), (40, 30, 271), (1, 24, 2200), (1, 24, 6000), (2, 12, 50021)]
+
+
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("size", ROWS, ids=str)
+def test_policy_terms_beyond_fp32(dev, size, dtype):  # noqa: F811
+    """Ratios of e^100 and e^300 with advantages -1, 0 and 1 and KL terms of e^100, with weights that keep what comes out of
+    them in fp32's range (the coefficient of the log-probability need not be), beside ordinary rows."""
+    from mote_b200 import policy_loss
+    S, T, V = size
+    z, y, gen = cpu_case(S, T, V, dtype, V + T, prompt=0.1)
+    n = torch.arange(S * T).view(S, T)
+    sure = n % 6 == 3   # a target of probability 1 - V e^-60: a coefficient of 2.7e43 times 1 - p is in range
+    at = torch.where(sure, 60.0, z.float().gather(-1, y.clamp(min=0)[..., None])[..., 0])
+    z.scatter_(-1, y.clamp(min=0)[..., None], at[..., None].to(dtype))
+    z[..., -3:] = torch.where((y < V - 3)[..., None], -math.inf, z[..., -3:])   # columns of probability 0
+    A = (n % 3 - 1).float()
+    logp, _ = ref.row_values(z, y, 1.0)
+    far = torch.where(n % 5 == 0, 300.0, 100.0)
+    far = torch.where((A != 0) & (far > 200), 100.0, far)   # e^300 only where the advantage is 0
+    ordinary = n % 4 == 1
+    old = torch.where(ordinary, logp + 0.1, logp - far).float()
+    rf = torch.where(ordinary | (n % 2 == 0), logp - 0.2, logp + 100.0).float()
+    w = torch.where(ordinary | sure, 1.0, torch.where(n % 8 < 4, 1e-6, 1e-20)).float()   # 2.7e43 * 1e-6: above 2^112
+    rf = torch.where(sure, (logp - 0.2).float(), rf)
+    c, div = 0.04, 2.0
+    to = lambda t: t.to(dev)  # noqa: E731
+    r = policy_loss(to(z), to(y), to(A), to(old), to(rf), weights=to(w), clip_low=0.2, clip_high=0.3, kl_coef=c, divisor=div)
+    want = ref.policy(z, y, A, old, rf, w, 0.2, 0.3, c, 1.0, div)
+    assert bool(torch.isfinite(want["grad"]).all()) and float(want["coef"].abs().max()) > 1e43
+    assert float(want["grad"].abs().max()) < 3e38 / (1 + 1 / 128)
+    Sp = ref.spread(z, 1.0)
+    d = torch.exp(rf.double() - logp)
+    # e^x of a 64-bit difference rounded to fp32 would be off by 150 u at 300; it is of the log-probability's own error
+    bend = torch.where(want["live"], want["w"] * (A.abs().double() * want["ratio"] + c * d) / div, 0.0)
+    # a row's probabilities and its target's 1 - p, which its coefficient's error is multiplied by
+    p = torch.softmax(z.double(), -1)
+    share = torch.where(torch.arange(V) == y.clamp(min=0)[..., None], (1 - p).clamp(min=1e-12), p)
+    tol = want["grad_tol"] + 2 * (bend * (Sp + 4 * U))[..., None] * share
+    assert_rounded(r.grad, want["grad"], tol, "grad")
+    assert not bool(r.grad[..., -3:].cpu()[(y < V - 3) & (y >= 0)].any())   # nothing times a probability of 0
+    # a sure target keeps its relative accuracy, at the target and beside it
+    rows = sure & (y >= 0) & (A < 0)
+    assert bool(rows.any())
+    # in 64 bits too a difference of 1 and p would be 0 there: 1 - p = -expm1(logp)
+    exact = want["grad"].scatter(-1, y.clamp(min=0)[..., None], (-torch.expm1(logp) * want["coef"])[..., None])[rows]
+    got = r.grad.cpu().double()[rows]
+    rel = 8 * float(Sp.max()) + torch.finfo(dtype).eps / 2
+    assert bool(((got - exact).abs() <= rel * exact.abs() + 1e-37).all())
+    assert float(want["loss"]) > 1e39 and float(r.loss) == math.inf   # the sure rows' terms are no fp32 numbers
+    w, div = torch.where(sure, 0.0, w), float(S * T)                  # the means of the others are
+    r = policy_loss(to(z), to(y), to(A), to(old), to(rf), weights=to(w), clip_low=0.2, clip_high=0.3, kl_coef=c, divisor=div)
+    want = ref.policy(z, y, A, old, rf, w, 0.2, 0.3, c, 1.0, div)
+    scale = float((want["w"] * (A.abs().double() * torch.where(A < 0, want["ratio"], 1.3) + c * (d + 110)))[want["live"]].sum())
+    assert_close(r.loss, want["loss"], scale / div * float(Sp.max() + 8 * U) + U * float(want["loss"].abs()), "loss")
+    klt = float((want["w"] * (d + 110))[want["live"]].sum()) / div * float(Sp.max() + 8 * U)
+    assert_close(r.kl, want["kl"], klt + U * float(want["kl"]), "kl")
+    assert_close(r.count, want["count"], 2 * U * float(want["count"]), "count")
+    assert_close(r.clipped, want["clipped"], 2 * U * float(want["clipped"]), "clipped")
+
+
+@pytest.mark.parametrize("V", [271, 6000])
+def test_an_advantage_of_zero_is_zero_whatever_the_ratio(dev, V):  # noqa: F811
+    """A group whose rewards are all equal, with old log-probabilities that no longer fit: no loss and no gradient."""
+    from mote_b200 import policy_loss
+    z, y, _ = cpu_case(2, 6, V, F32, V, prompt=0.0)
+    z, y = z.to(dev), y.to(dev)
+    for low in (-100.0, -500.0, -2000.0, -3e38):
+        r = policy_loss(z, y, torch.zeros(2, device=dev), torch.full((2, 6), low, device=dev))
+        assert float(r.loss) == 0.0 and not bool(r.grad.any()) and float(r.count) == 12.0, low
