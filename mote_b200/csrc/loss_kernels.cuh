@@ -19,6 +19,7 @@
 #include <cstdint>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
+#include <type_traits>
 
 #include "mt_types.h"
 #include "ptx.cuh"
@@ -80,16 +81,17 @@ __device__ __forceinline__ F2 fma2(F2 x, F2 y, F2 z) {
   return r;
 }
 
-// The exponentials of a row about a logit m, with c = c_hi + c_lo = log2(e) / T: 2^(z c - b) fix is exp(z / T - ref(m)), where
+// The exponentials of a row about a logit m, with c = c_hi + c_lo = log2(e) / T: 2^(z c - b) 2^16 is exp(z / T - ref(m)), where
 // ref(m) is m / T rounded to a whole power of two, base(m) = rint(m c). Sums about different m then differ by powers of two,
 // exactly. c_hi has 12 bits, so that what the first multiply-add leaves to the second is not lost under half a unit of its
 // result (with one float for c, or a full one for c_hi, its rounding leans every exponent of a row the same way: 5e-8 of a sum,
 // and the sums of thousands of positions keep it). b is base + 16: ex2 is asked for values below -1 only, where its relative
 // error has the mean of -5.05e-8 that row_stat takes out. c_lo > 0 keeps -inf a -inf.
 //
-// Where |m c| >= 2^18, ref(m) is m / T itself and fix the difference. Beyond |m| = 2^60, where a product may overflow, any two
-// different logits are at least 2^37 apart: a scale of 2^-20 gives 1 for z = m and 0 below.
-constexpr float kAbove = 16.f;
+// Where |m c| >= 2^18 (a far m: a mask of -1e9, say), ref(m) is m / T itself and m is taken from z first: the difference is
+// exact where its exponential is not 0, and b is kAbove alone. A product with m there would leave half a unit of m c, which is
+// 128 from 2^32 on. Loops over a row branch once (two<true>): the subtraction in all rows would be one of five instructions.
+constexpr float kAbove = 16.f, kFix = 65536.f;   // 2^kAbove
 struct Base {
   float b;     // rint(m c)
   bool near;
@@ -105,43 +107,35 @@ __device__ __forceinline__ double ref_of(float m, const Rows& R) {
 }
 struct Ex {
   F2 hi, lo, nb;
-  float fix;
+  float sub;   // a far m, else 0
   __device__ Ex(float m, const Rows& R, float up = 0.f) {   // up: a power of two that the values carry (policy_row)
     if (m == kNegInf) m = 0.f;
-    float h = R.c_hi, l = R.c_lo;
     const Base base(m, R);
-    float b = base.b + kAbove;
-    fix = 65536.f;   // 2^kAbove
-    if (!base.near) {
-      fix = 1.f;
-      if (fabsf(m) > 0x1p60f && fabsf(m) < INFINITY) {
-        h = 0x1p-20f;
-        l = 0x1p-149f;
-        b = m * h;
-      } else {
-        b = fmaf(m, h, m * l);
-        fix = expf(fmaf(m, l, fmaf(m, h, -b)) * -0.69314718f);
-      }
-    }
-    hi = pack2(h, h);
-    lo = pack2(l, l);
-    b -= up;
+    sub = base.near ? 0.f : m;
+    const float b = (base.near ? base.b : 0.f) + kAbove - up;
+    hi = pack2(R.c_hi, R.c_hi);
+    lo = pack2(R.c_lo, R.c_lo);
     nb = pack2(-b, -b);
   }
+  __device__ __forceinline__ bool far() const { return sub != 0.f; }
+  template <bool kFar>
   __device__ __forceinline__ void two(F2 z, float& e0, float& e1) const {
     float t0, t1;
+    if (kFar) z = fma2(z, pack2(1.f, 1.f), pack2(-sub, -sub));
     unpack2(fma2(z, lo, fma2(z, hi, nb)), t0, t1);
     e0 = ex2(t0);
     e1 = ex2(t1);
   }
+  template <bool kFar>
   __device__ __forceinline__ float sum(F2 z) const {
     float e0, e1;
-    two(z, e0, e1);
+    two<kFar>(z, e0, e1);
     return e0 + e1;
   }
-  __device__ __forceinline__ float one(float z) const {
+  __device__ __forceinline__ float one(float z) const {   // of any row
     float e0, e1;
-    two(pack2(z, z), e0, e1);
+    z -= sub;
+    two<false>(pack2(z, z), e0, e1);
     return e0;
   }
 };
@@ -227,14 +221,16 @@ struct Pairs<__nv_bfloat16> {
   __device__ __forceinline__ explicit Pairs(const uint4& v)
       : p{pack2(lo_bf16(v.x), hi_bf16(v.x)), pack2(lo_bf16(v.y), hi_bf16(v.y)), pack2(lo_bf16(v.z), hi_bf16(v.z)),
           pack2(lo_bf16(v.w), hi_bf16(v.w))} {}
+  template <bool kFar>
   __device__ __forceinline__ float sum(const Ex& ex) const {
-    return (ex.sum(p[0]) + ex.sum(p[1])) + (ex.sum(p[2]) + ex.sum(p[3]));
+    return (ex.sum<kFar>(p[0]) + ex.sum<kFar>(p[1])) + (ex.sum<kFar>(p[2]) + ex.sum<kFar>(p[3]));
   }
+  template <bool kFar>
   __device__ __forceinline__ uint4 scaled(const Ex& ex, float f) const {   // f exp, rounded once
     float a[8];
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
-      ex.two(p[u], a[2 * u], a[2 * u + 1]);
+      ex.two<kFar>(p[u], a[2 * u], a[2 * u + 1]);
       a[2 * u] *= f;
       a[2 * u + 1] *= f;
     }
@@ -248,11 +244,15 @@ struct Pairs<float> {
   __device__ __forceinline__ explicit Pairs(const uint4& v)
       : p{pack2(bits(v.x), bits(v.y)), pack2(bits(v.z), bits(v.w))} {}
   static __device__ __forceinline__ float bits(uint32_t w) { return __uint_as_float(w); }
-  __device__ __forceinline__ float sum(const Ex& ex) const { return ex.sum(p[0]) + ex.sum(p[1]); }
+  template <bool kFar>
+  __device__ __forceinline__ float sum(const Ex& ex) const {
+    return ex.sum<kFar>(p[0]) + ex.sum<kFar>(p[1]);
+  }
+  template <bool kFar>
   __device__ __forceinline__ uint4 scaled(const Ex& ex, float f) const {
     float a[4];
-    ex.two(p[0], a[0], a[1]);
-    ex.two(p[1], a[2], a[3]);
+    ex.two<kFar>(p[0], a[0], a[1]);
+    ex.two<kFar>(p[1], a[2], a[3]);
     return make_uint4(__float_as_uint(a[0] * f), __float_as_uint(a[1] * f), __float_as_uint(a[2] * f), __float_as_uint(a[3] * f));
   }
 };
@@ -474,37 +474,44 @@ struct Running {
     for (int k = 0; k < kN; ++k) t = vec_max<T>(t, v[k]);
     const float top = W::top(t);
     if ((top - m) * R.c_hi > kSlack) {
-      const Ex next(top, R);
-      const float by = rescale(m, top, R) * (ex.fix / next.fix);
+      const float by = rescale(m, top, R);
       s0 *= by;
       s1 *= by;
       m = top;
-      ex = next;
+      ex = Ex(top, R);
     }
+    if (ex.far()) {
 #pragma unroll
-    for (int k = 0; k < kN; ++k) (k & 1 ? s1 : s0) += Pairs<T>(v[k]).sum(ex);
+      for (int k = 0; k < kN; ++k) (k & 1 ? s1 : s0) += Pairs<T>(v[k]).template sum<true>(ex);
+    } else {
+#pragma unroll
+      for (int k = 0; k < kN; ++k) (k & 1 ? s1 : s0) += Pairs<T>(v[k]).template sum<false>(ex);
+    }
   }
-  __device__ __forceinline__ Part part() const { return Part{m, (s0 + s1) * ex.fix}; }
+  __device__ __forceinline__ Part part() const { return Part{m, (s0 + s1) * kFix}; }
 };
 
 // Gradient lines [i, n) by kStride of an output row from lines of shared memory `off` bytes from `src`: f exp(x - ref(m))
 template <typename T, uint32_t kStride, int kUnroll>
 __device__ __forceinline__ void gradient_lines(uint4* __restrict__ out, const unsigned char* src, uint32_t off, uint32_t i,
                                                uint32_t n, const Ex& ex, float f) {
-  if ((off & 15u) == 0) {   // the two rows are aligned alike
+  if ((off & 15u) == 0 && !ex.far()) {   // the two rows are aligned alike
     const uint4* const in = reinterpret_cast<const uint4*>(src + static_cast<int32_t>(off));
     for (; i + (kUnroll - 1) * kStride < n; i += kUnroll * kStride) {
       uint4 v[kUnroll];
 #pragma unroll
       for (int k = 0; k < kUnroll; ++k) v[k] = in[i + k * kStride];
 #pragma unroll
-      for (int k = 0; k < kUnroll; ++k) out[i + k * kStride] = Pairs<T>(v[k]).scaled(ex, f);
+      for (int k = 0; k < kUnroll; ++k) out[i + k * kStride] = Pairs<T>(v[k]).template scaled<false>(ex, f);
     }
 #pragma unroll 1
-    for (; i < n; i += kStride) out[i] = Pairs<T>(in[i]).scaled(ex, f);
+    for (; i < n; i += kStride) out[i] = Pairs<T>(in[i]).template scaled<false>(ex, f);
+  } else if (!ex.far()) {
+#pragma unroll 1
+    for (; i < n; i += kStride) out[i] = Pairs<T>(load_shifted(src, i * 16 + off)).template scaled<false>(ex, f);
   } else {
 #pragma unroll 1
-    for (; i < n; i += kStride) out[i] = Pairs<T>(load_shifted(src, i * 16 + off)).scaled(ex, f);
+    for (; i < n; i += kStride) out[i] = Pairs<T>(load_shifted(src, i * 16 + off)).template scaled<true>(ex, f);
   }
 }
 
@@ -587,7 +594,7 @@ struct Kept {
 };
 // exp(x_j - lse) = exp(x_j - ref(m)) exp(ref(m) - lse) with m = lse T
 struct KeptRow {
-  float m, f, gy;   // d_j = exp(x_j - ref(m)) f, gy at the target
+  float m, f, gy, up;   // d_j = 2^up exp(x_j - ref(m)) f, gy at the target
 };
 __device__ __forceinline__ float kept_coef(const Kept& K, uint32_t row, uint32_t seq, uint32_t tok) {
   return K.coef_row ? K.coef_row[row] : K.coef.at(seq, tok);
@@ -598,7 +605,14 @@ __device__ __forceinline__ KeptRow kept_row(const Kept& K, const Rows& R, uint32
   const float g = static_cast<float>(coef * R.inv_t);
   KeptRow r;
   r.m = static_cast<float>(lse * R.t);
-  r.f = -g * expf(static_cast<float>(ref_of(r.m, R) - lse));
+  const Base b(r.m, R);
+  if (b.near) {
+    r.f = -g * expf(static_cast<float>(b.b * kLn2 - lse));
+    r.up = 0.f;
+  } else {   // a far lse may be a large number away from m / T: in the exponents, where nothing overflows before the result does
+    r.f = -g;
+    r.up = static_cast<float>((r.m * R.inv_t - lse) * kLog2e);
+  }
   r.gy = -expm1f(lp) * g;
   return r;
 }
@@ -800,7 +814,7 @@ __device__ __forceinline__ void tile_rows(const TileArgs& A, unsigned char* sm, 
   using W = Word<T>;
   constexpr uint32_t kPer = 16 / sizeof(T);
   constexpr int kAtOnce = 32 / kG;
-  __shared__ float4 sh_row[kTileWarps * kTileRows];   // (m, s, target logit, counts), then (m, f, gy, counts: 1 + up)
+  __shared__ float4 sh_row[kTileWarps * kTileRows];   // (m, s, target logit, counts), then (m, f, gy, up; -inf where the row's gradient is 0)
   const Rows& R = A.R;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = lane / kG;
   const uint32_t gl = lane % kG;
@@ -864,12 +878,12 @@ __device__ __forceinline__ void tile_rows(const TileArgs& A, unsigned char* sm, 
     pdl_wait();   // the logits and targets are inputs; the rows' coefficients may come from the launch before
     if (A.K.pair_loss && blockIdx.x == 0 && warp == 0) sum_pairs(A.K);
     if (lane < rows) {
-      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+      float4 v = make_float4(0.f, 0.f, 0.f, kNegInf);
       const uint32_t row = first + lane, seq = row / R.tokens, tok = row - seq * R.tokens;
       const float coef = live ? kept_coef(A.K, row, seq, tok) : 0.f;
       if (coef != 0.f) {
         const KeptRow k = kept_row(A.K, R, row, seq, tok, coef);
-        v = make_float4(k.m, k.f, k.gy, 1.f);
+        v = make_float4(k.m, k.f, k.gy, k.up);
       }
       own[lane] = v;
     }
@@ -900,7 +914,7 @@ __device__ __forceinline__ void tile_rows(const TileArgs& A, unsigned char* sm, 
       if (r >= rows) nl = 0;
       const uint4* const row = reinterpret_cast<const uint4*>(base + static_cast<size_t>(r) * A.pitch) + gl;
       uint32_t top = W::kEmpty;
-      float s0 = 0.f, s1 = 0.f, m, fix;
+      float s0 = 0.f, s1 = 0.f, m;
       if (kL > 0) {
         uint4 v[kL > 0 ? kL : 1];
 #pragma unroll
@@ -912,23 +926,27 @@ __device__ __forceinline__ void tile_rows(const TileArgs& A, unsigned char* sm, 
         for (int k = 0; k < kL; ++k) top = vec_max<T>(top, v[k]);
         m = group_max<kG>(W::top(top));
         const Ex ex(m, R);
-        fix = ex.fix;
+        if (ex.far()) {
 #pragma unroll
-        for (int k = 0; k < kL; ++k) {
-          (k & 1 ? s1 : s0) += Pairs<T>(v[k]).sum(ex);
+          for (int k = 0; k < kL; ++k) (k & 1 ? s1 : s0) += Pairs<T>(v[k]).template sum<true>(ex);
+        } else {
+#pragma unroll
+          for (int k = 0; k < kL; ++k) (k & 1 ? s1 : s0) += Pairs<T>(v[k]).template sum<false>(ex);
         }
       } else {
 #pragma unroll 4
         for (uint32_t l = 0; gl + l < nl; l += kG) top = vec_max<T>(top, row[l]);
         m = group_max<kG>(W::top(top));
         const Ex ex(m, R);
-        fix = ex.fix;
+        if (ex.far()) {
+#pragma unroll 1
+          for (uint32_t l = 0; gl + l < nl; l += kG) s0 += Pairs<T>(row[l]).template sum<true>(ex);
+        } else {
 #pragma unroll 4
-        for (uint32_t l = 0; gl + l < nl; l += kG) {
-          s0 += Pairs<T>(row[l]).sum(ex);
+          for (uint32_t l = 0; gl + l < nl; l += kG) s0 += Pairs<T>(row[l]).template sum<false>(ex);
         }
       }
-      const float s = group_sum<kG>(s0 + s1) * fix;
+      const float s = group_sum<kG>(s0 + s1) * kFix;
       if (gl == 0 && r < rows) *reinterpret_cast<float2*>(own + r) = make_float2(m, s);
     }
     __syncthreads();
@@ -957,7 +975,7 @@ __device__ __forceinline__ void tile_rows(const TileArgs& A, unsigned char* sm, 
           A.logp64[row] = st.logp;
           A.coef[row] = 0.f;
         }
-        if (kMode != kForward) sh_row[lane] = make_float4(v.x, st.f, st.rest, v.w + up);
+        if (kMode != kForward) sh_row[lane] = make_float4(v.x, st.f, st.rest, counts ? up : kNegInf);
       }
       if (kMode == kPolicyLoss) {   // lane k < 4: the block's sum k
 #pragma unroll
@@ -974,7 +992,7 @@ __device__ __forceinline__ void tile_rows(const TileArgs& A, unsigned char* sm, 
       if (lane < rows) {
         const float coef = __ldcg(A.coef + first + lane), g = static_cast<float>(coef * R.inv_t);
         const float4 v = own[lane];
-        own[lane] = make_float4(v.x, -g * v.y, g * v.z, coef != 0.f ? v.w : 0.f);
+        own[lane] = make_float4(v.x, -g * v.y, g * v.z, coef != 0.f ? v.w : kNegInf);
       }
       __syncwarp();
     }
@@ -992,19 +1010,19 @@ __device__ __forceinline__ void tile_rows(const TileArgs& A, unsigned char* sm, 
     const Split<T> so(out, R.vocab);
     uint4* const ov = reinterpret_cast<uint4*>(out + so.head);
     const unsigned char* const row = base + static_cast<size_t>(r) * A.pitch;
-    if (v.w == 0.f) {
+    if (v.w == kNegInf) {
       for (uint32_t l = gl; l < so.vecs; l += kG) ov[l] = make_uint4(0, 0, 0, 0);
       for (uint32_t i = gl; i < so.head + so.tail; i += kG) store_one(out + so.edge(i), 0.f);
       continue;
     }
-    const Ex ex(v.x, R, kMode == kPolicyLoss ? v.w - 1.f : 0.f);
-    const float k1 = v.y * ex.fix;
+    const Ex ex(v.x, R, v.w);
+    const float k1 = v.y * kFix;
     const uint32_t off = (sk + so.head) * static_cast<uint32_t>(sizeof(T));
-    if (kL > 0 && (off & 15u) == 0) {
+    if (kL > 0 && (off & 15u) == 0 && !ex.far()) {
       const uint4* const in = reinterpret_cast<const uint4*>(row + off) + gl;
 #pragma unroll
       for (int k = 0; k < kL; ++k)
-        if (gl + k * kG < so.vecs) ov[gl + k * kG] = Pairs<T>(in[k * kG]).scaled(ex, k1);
+        if (gl + k * kG < so.vecs) ov[gl + k * kG] = Pairs<T>(in[k * kG]).template scaled<false>(ex, k1);
     } else {
       gradient_lines<T, kG, 2>(ov, row, off, gl, so.vecs, ex, k1);
     }
@@ -1016,7 +1034,7 @@ __device__ __forceinline__ void tile_rows(const TileArgs& A, unsigned char* sm, 
   __syncwarp();   // the targets' elements, written above
   if (has_y) {
     const float4 v = own[lane];
-    if (v.w != 0.f) store_one(static_cast<T*>(A.grad) + static_cast<size_t>(first + lane) * R.vocab + y, v.z);
+    if (v.w != kNegInf) store_one(static_cast<T*>(A.grad) + static_cast<size_t>(first + lane) * R.vocab + y, v.z);
   }
 }
 
@@ -1321,7 +1339,7 @@ __global__ void __launch_bounds__(kThreads, kThreads == 128 ? 6 : 3) slice_kerne
   if (A.grad == nullptr) return;
   __syncthreads();
   const Ex ex(p.m, R, sh_g[2]);
-  const float f = sh_g[0] * ex.fix, gy = sh_g[1];
+  const float f = sh_g[0] * kFix, gy = sh_g[1];
   if (je != 0xffffffffu) {
     const T* const x = reinterpret_cast<const T*>(sm) + skew + (je - e0);
     store_one(out + je, je == y ? gy : ex.one(load_one(x)) * f);
@@ -1393,22 +1411,26 @@ __global__ void __launch_bounds__(kGradThreads) grad_kernel(const __grid_constan
     return;
   }
   const KeptRow r = kept_row(A.K, R, row, seq, tok, coef);
-  const Ex ex(r.m, R);
-  const float f = r.f * ex.fix;
+  const Ex ex(r.m, R, r.up);
+  const float f = r.f * kFix;
   const uint32_t y = y64 < static_cast<int64_t>(R.vocab) ? static_cast<uint32_t>(y64) : 0xffffffffu;
   if (edge) store_one(out + je, je == y ? r.gy : ex.one(load_one(z + je)) * f);
+  const auto write = [&](auto far) {
 #pragma unroll
-  for (int k = 0; k < kGradVecs; ++k) {
-    const uint32_t at = begin + k * kGradThreads;
-    if (at >= so.vecs) break;
-    const uint4 d = Pairs<T>(by ? shift_lines(v[k], w[k], by) : v[k]).scaled(ex, f);
-    // the preference loss has read the logits before: a gradient that leaves L2 first leaves them there (4 x 1024 x 32768
-    // bf16: 137 against 147 us)
-    if (A.K.pair_loss) __stcs(ov + at, d);
-    else ov[at] = d;
-    const uint32_t e = so.head + at * kPer;
-    if (y - e < kPer) store_one(out + y, r.gy);
-  }
+    for (int k = 0; k < kGradVecs; ++k) {
+      const uint32_t at = begin + k * kGradThreads;
+      if (at >= so.vecs) break;
+      const uint4 d = Pairs<T>(by ? shift_lines(v[k], w[k], by) : v[k]).template scaled<decltype(far)::value>(ex, f);
+      // the preference loss has read the logits before: a gradient that leaves L2 first leaves them there (4 x 1024 x 32768
+      // bf16: 137 against 147 us)
+      if (A.K.pair_loss) __stcs(ov + at, d);
+      else ov[at] = d;
+      const uint32_t e = so.head + at * kPer;
+      if (y - e < kPer) store_one(out + y, r.gy);
+    }
+  };
+  if (ex.far()) write(std::true_type());
+  else write(std::false_type());
 }
 
 // ---------------------------------------------------------------------------------------------------------------------

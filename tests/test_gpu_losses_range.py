@@ -83,3 +83,89 @@ def test_an_advantage_of_zero_is_zero_whatever_the_ratio(dev, V):  # noqa: F811
     for low in (-100.0, -500.0, -2000.0, -3e38):
         r = policy_loss(z, y, torch.zeros(2, device=dev), torch.full((2, 6), low, device=dev))
         assert float(r.loss) == 0.0 and not bool(r.grad.any()) and float(r.count) == 12.0, low
+
+
+def _far_rows(V, dtype, mask, gen):
+    """Rows with a finite mask or far logits, and their targets."""
+    z = torch.randn(1, 10, V, generator=gen)
+    y = torch.randint(3, V - 3, (1, 10), generator=gen)
+    z[0, 0] = mask                      # only the target
+    z[0, 0, y[0, 0]] = 1.5
+    z[0, 1, 3:] = mask                  # three columns, the target one of them
+    y[0, 1] = 1
+    z[0, 2, :2 * V // 3] = mask         # the first, the middle, the last columns
+    y[0, 2] = V - 2
+    z[0, 3, V // 5:4 * V // 5] = mask
+    y[0, 3] = V - 1
+    z[0, 4, V // 3:] = mask
+    y[0, 4] = 0
+    z[0, 5, y[0, 5]] = mask             # only the target is masked
+    z[0, 6] = mask                      # all the same: uniform
+    z[0, 7] = mask                      # a far target above a mask
+    z[0, 7, y[0, 7]] = -mask
+    z[0, 8, 2] = -mask                  # another column far above all
+    z[0, 9] = mask                      # two of the same size above the mask
+    z[0, 9, :2] = -mask
+    y[0, 9] = 1
+    return z.to(dtype), y
+
+
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("V", [60, 271, 2200, 6000, 50021, 300000])
+@pytest.mark.parametrize("mask", [-2e5, -1e7, -1e9, -3e9, -1e10, -1e12, -1e15, -1e18, -1e30])
+def test_masks_of_any_size(dev, mask, V, dtype):  # noqa: F811
+    """A finite mask is as good as -inf, at every temperature: in the tiles, the pieces (whole ones that are masked), the
+    slices. x = z times an fp32 reciprocal: 2 u of a difference and of lse."""
+    from mote_b200 import policy_loss, preference_loss, token_logprobs, token_logprobs_backward
+    z, y = _far_rows(V, dtype, mask, torch.Generator().manual_seed(V))
+    zd, yd = z.to(dev), y.to(dev)
+    one = torch.ones(1, 10)
+    near = [0, 1, 2, 3, 4, 5]               # their lse is an ordinary number
+    for T in (1.0, 0.3, 0.1):
+        logp, lse = ref.row_values(z, y, T)
+        S = ref.spread(z, T)
+        r = token_logprobs(zd, yd, temperature=T)
+        assert_close(r.logprobs, logp, 4 * U * logp.abs() + S, f"logprobs {T}")
+        assert_close(r.lse, lse, 4 * U * lse.abs() + S, f"lse {T}")
+        want, tol = ref.gradient(z, y, one.double(), T, y >= 0)
+        kept = tol + want.abs() * 4 * U * torch.where(lse.abs() < 1e3, lse.abs() + 1, 1.0)[..., None] + 1e-30
+        d = token_logprobs_backward(zd, yd, r.logprobs, r.lse, one.to(dev), temperature=T).cpu()
+        assert not bool(torch.isnan(d).any()), T
+        rows = near if T != 1.0 else near + [7, 8]   # at T = 1 their far lse is the logit itself, else it is a rounded number
+        assert_rounded(d[:, rows], want[:, rows], kept[:, rows], f"backward {T}")
+        # the policy loss at a ratio of 1: the gradient of the log-probability, and as exact where lse is far
+        p = policy_loss(zd, yd, one.to(dev), r.logprobs, temperature=T, clip_high=1e9)
+        ratio = want.abs() * (S + 4 * U * logp.abs().clamp(max=1.0))[..., None]
+        fine = [i for i in range(10) if bool(torch.isfinite(logp[0, i])) and float(logp[0, i]) > -1e3]
+        assert_rounded(p.grad.cpu()[:, fine], -want[:, fine], (tol + 2 * ratio + 1e-30)[:, fine], f"policy {T}")
+        assert not bool(torch.isnan(p.grad).any()) and not bool(torch.isnan(p.loss))
+        # the preference loss of two such sequences: a coefficient of 1/20 each, as far as their sums agree
+        q = preference_loss(torch.cat([zd, zd]), torch.cat([yd, yd]), temperature=T)
+        assert not bool(torch.isnan(q.grad).any()) and not bool(torch.isnan(q.loss))
+        e = 0.1 * 2 * float(S.sum()) + 1e-6
+        assert abs(float(q.loss) - math.log(2.0)) < e
+        for s, sign in ((0, -0.05), (1, 0.05)):
+            assert_rounded(q.grad.cpu()[s:s + 1, near], sign * want[:, near],
+                           0.05 * (kept + 2 * e * want.abs())[:, near], f"preference {T}")
+
+
+@pytest.mark.parametrize("V", [271, 2200, 6000, 70000])
+@pytest.mark.parametrize("base,T", [(3e5, 1.0), (3e6, 1.0), (-2e4, 0.1), (3e9, 1e4)])
+def test_far_logits_next_to_each_other(dev, base, T, V):  # noqa: F811
+    """fp32 logits that differ by little and lie far from 0: their differences are exact, so are the results as accurate as
+    those of the same logits at 0 (an fp32 product z / T would be off by half a unit of |z / T| log2 e)."""
+    from mote_b200 import policy_loss, token_logprobs
+    gen = torch.Generator().manual_seed(V)
+    step = 2.0 ** math.floor(math.log2(abs(base)) - 23) * 2   # two units of the logits' last place
+    k = torch.randint(0, 40, (2, 6, V), generator=gen)
+    z = torch.tensor(base).double() + k.double() * step
+    assert torch.equal(z.float().double(), z)
+    y = torch.randint(0, V, (2, 6), generator=gen)
+    r = token_logprobs(z.float().to(dev), y.to(dev), temperature=T)
+    logp, lse = ref.row_values(z, y, T)
+    S = ref.spread(z, T)
+    assert_close(r.logprobs, logp, 3 * U * logp.abs() + S, "logprobs")
+    assert_close(r.lse, lse, 4 * U * lse.abs() + S, "lse")
+    p = policy_loss(z.float().to(dev), y.to(dev), torch.ones(2, device=dev), r.logprobs, temperature=T, clip_high=1e9)
+    want, tol = ref.gradient(z, y, torch.ones(2, 6, dtype=torch.float64), T, y >= 0)
+    assert_rounded(p.grad, -want, tol + (2 * S + 4 * U * logp.abs())[..., None] * want.abs(), "policy")
