@@ -463,30 +463,33 @@ __device__ __forceinline__ uint4 load_shifted(const unsigned char* p, uint32_t o
 // sum is rescaled hardly ever.
 constexpr float kSlack = kAbove - 1.f;
 struct Running {
-  float m, s0, s1;
+  float m, s0, s1, limit;
   Ex ex;
-  __device__ explicit Running(const Rows& R) : m(kNegInf), s0(0.f), s1(0.f), ex(kNegInf, R) {}
+  __device__ explicit Running(const Rows& R) : m(kNegInf), s0(0.f), s1(0.f), limit(kSlack), ex(kNegInf, R) {}
   template <typename T, int kN>
   __device__ __forceinline__ void add(const uint4 (&v)[kN], const Rows& R) {
     using W = Word<T>;
     uint32_t t = W::kEmpty;
 #pragma unroll
     for (int k = 0; k < kN; ++k) t = vec_max<T>(t, v[k]);
-    const float top = W::top(t);
-    if ((top - m) * R.c_hi > kSlack) {
-      const float by = rescale(m, top, R);
-      s0 *= by;
-      s1 *= by;
-      m = top;
-      ex = Ex(top, R);
-    }
-    if (ex.far()) {
+    const float top = W::top(t), above = (top - m) * R.c_hi;
+    if (!(above <= limit)) {   // hardly ever, or always about a far m
+      if (above > kSlack) {
+        const float by = rescale(m, top, R);
+        s0 *= by;
+        s1 *= by;
+        m = top;
+        ex = Ex(top, R);
+        limit = ex.far() ? kNegInf : kSlack;
+      }
+      if (ex.far()) {
 #pragma unroll
-      for (int k = 0; k < kN; ++k) (k & 1 ? s1 : s0) += Pairs<T>(v[k]).template sum<true>(ex);
-    } else {
-#pragma unroll
-      for (int k = 0; k < kN; ++k) (k & 1 ? s1 : s0) += Pairs<T>(v[k]).template sum<false>(ex);
+        for (int k = 0; k < kN; ++k) (k & 1 ? s1 : s0) += Pairs<T>(v[k]).template sum<true>(ex);
+        return;
+      }
     }
+#pragma unroll
+    for (int k = 0; k < kN; ++k) (k & 1 ? s1 : s0) += Pairs<T>(v[k]).template sum<false>(ex);
   }
   __device__ __forceinline__ Part part() const { return Part{m, (s0 + s1) * kFix}; }
 };
