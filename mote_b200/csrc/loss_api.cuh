@@ -223,9 +223,9 @@ size_t parts_bytes(int dtype, int64_t rows, int64_t vocab) {
   return short_rows(dtype, vocab) ? 0 : sizeof(Part) * static_cast<size_t>(rows) * static_cast<size_t>(row_pieces(dtype, vocab));
 }
 
-// logp, lse (or logp64, lse, coef = 0) of every row
-int launch_forward(int dtype, const Rows& R, float* logp, float* lse, double* logp64, float* coef, Part* parts, int sms,
-                   cudaStream_t st) {
+// logp, lse (or logp64, lse64, coef = 0) of every row
+int launch_forward(int dtype, const Rows& R, float* logp, float* lse, double* logp64, double* lse64, float* coef, Part* parts,
+                   int sms, cudaStream_t st) {
   if (short_rows(dtype, R.vocab)) {
     TileArgs A;
     std::memset(&A, 0, sizeof(A));
@@ -233,6 +233,7 @@ int launch_forward(int dtype, const Rows& R, float* logp, float* lse, double* lo
     A.logp = logp;
     A.lse = lse;
     A.logp64 = logp64;
+    A.lse64 = lse64;
     A.coef = coef;
     return launch_tile<kForward>(dtype, A, tile_shape(R.n, line_bytes(dtype, R.vocab), sms), st);
   }
@@ -257,6 +258,7 @@ int launch_forward(int dtype, const Rows& R, float* logp, float* lse, double* lo
   J.logp = logp;
   J.lse = lse;
   J.logp64 = logp64;
+  J.lse64 = lse64;
   J.coef = coef;
   const unsigned grid = static_cast<unsigned>(cdiv(R.n, kJoinThreads / 32));
   return dtype == MOTEOPT_DTYPE_BF16 ? launch_after(join_kernel<__nv_bfloat16>, J, grid, kJoinThreads, 0, st, "loss join_kernel")
@@ -318,7 +320,7 @@ PreferenceLayout preference_layout(int dtype, int64_t n, int64_t vocab, int64_t 
   PreferenceLayout L;
   L.logp64 = kHeaderBytes;
   L.lse = align_up(L.logp64 + 8 * static_cast<size_t>(n), 256);
-  L.coef = align_up(L.lse + 4 * static_cast<size_t>(n), 256);
+  L.coef = align_up(L.lse + 8 * static_cast<size_t>(n), 256);
   L.pairs = align_up(L.coef + 4 * static_cast<size_t>(n), 256);
   L.parts = align_up(L.pairs + 8 * static_cast<size_t>(pairs), 256);
   L.bytes = align_up(L.parts + parts_bytes(dtype, n, vocab), 256);
@@ -389,7 +391,7 @@ int moteopt_token_logprobs(const moteopt_logits* logits, const moteopt_positions
   }
   int sms = 0;
   MO_TRY(loss_setup(&sms));
-  return launch_forward(logits->dtype, R, logprobs, lse, nullptr, nullptr, parts, sms,
+  return launch_forward(logits->dtype, R, logprobs, lse, nullptr, nullptr, nullptr, parts, sms,
                         reinterpret_cast<cudaStream_t>(stream));
 }
 
@@ -515,7 +517,7 @@ int moteopt_preference_loss(const moteopt_logits* logits, const moteopt_position
   }
   char* const ws = static_cast<char*>(workspace);
   double* const logp64 = reinterpret_cast<double*>(ws + L.logp64);
-  float* const lse = reinterpret_cast<float*>(ws + L.lse);
+  double* const lse = reinterpret_cast<double*>(ws + L.lse);
   float* const coef = reinterpret_cast<float*>(ws + L.coef);
   double* const pair_loss = reinterpret_cast<double*>(ws + L.pairs);
   R.cu = p.cu_seqlens;
@@ -538,7 +540,7 @@ int moteopt_preference_loss(const moteopt_logits* logits, const moteopt_position
   Kept K;
   std::memset(&K, 0, sizeof(K));
   K.logp64 = logp64;
-  K.lse_row = lse;
+  K.lse64 = lse;
   K.coef_row = coef;
   K.pair_loss = pair_loss;
   K.pairs = A.pairs;
@@ -556,7 +558,7 @@ int moteopt_preference_loss(const moteopt_logits* logits, const moteopt_position
     return launch_tile_cluster<kPreference>(logits->dtype, B, t, st);
   }
   if (R.n > 0)
-    MO_TRY(launch_forward(logits->dtype, R, nullptr, lse, logp64, coef, reinterpret_cast<Part*>(ws + L.parts), sms, st));
+    MO_TRY(launch_forward(logits->dtype, R, nullptr, nullptr, logp64, lse, coef, reinterpret_cast<Part*>(ws + L.parts), sms, st));
   MO_TRY(launch_after(pair_kernel, A, static_cast<unsigned>(A.pairs), kPairThreads, 0, st, "loss pair_kernel", R.n == 0));
   if (!grad_logits || R.n == 0) return launch_after(pair_sum_kernel, K, 1, 32, 0, st, "loss pair_sum_kernel");
   return launch_gradient(logits->dtype, R, K, grad_logits, sms, st, true);

@@ -588,8 +588,8 @@ __device__ __forceinline__ Part row_join(Part p, int cl, uint32_t rank, const Ro
 // are written as zeros.
 struct Kept {
   Per logp, lse, coef;       // per position ...
-  const double* logp64;      // ... or by row: the preference loss's own [n] arrays
-  const float* lse_row;
+  const double* logp64;      // ... or by row: the preference loss's own [n] arrays. An fp32 lse of 8 to 16 would be off by
+  const double* lse64;       // up to 4.8e-7, and every probability of the gradient with it
   const float* coef_row;
   const double* pair_loss;   // preference: the first block adds up the pairs' losses
   int pairs;
@@ -603,7 +603,7 @@ __device__ __forceinline__ float kept_coef(const Kept& K, uint32_t row, uint32_t
   return K.coef_row ? K.coef_row[row] : K.coef.at(seq, tok);
 }
 __device__ __forceinline__ KeptRow kept_row(const Kept& K, const Rows& R, uint32_t row, uint32_t seq, uint32_t tok, float coef) {
-  const double lse = K.lse_row ? K.lse_row[row] : K.lse.at(seq, tok);
+  const double lse = K.lse64 ? K.lse64[row] : K.lse.at(seq, tok);
   const float lp = K.logp64 ? static_cast<float>(K.logp64[row]) : K.logp.at(seq, tok);
   const float g = static_cast<float>(coef * R.inv_t);
   KeptRow r;
@@ -772,7 +772,8 @@ struct TileArgs {
   uint32_t pitch;                      // bytes of a row's lines in shared memory, and 16 to read over
   float* logp;                         // [n], or null
   float* lse;                          // [n], or null
-  double* logp64;                      // [n] with coef [n] (preference), or null
+  double* logp64;                      // [n] with lse64 (outside a cluster) and coef [n] (preference), or null
+  double* lse64;
   float* coef;
   Policy P;
   void* grad;                          // [n][vocab], or null
@@ -976,6 +977,7 @@ __device__ __forceinline__ void tile_rows(const TileArgs& A, unsigned char* sm, 
         if (A.lse) A.lse[row] = static_cast<float>(st.lse);
         if (A.logp64) {
           A.logp64[row] = st.logp;
+          if (A.lse64) A.lse64[row] = st.lse;
           A.coef[row] = 0.f;
         }
         if (kMode != kForward) sh_row[lane] = make_float4(v.x, st.f, st.rest, counts ? up : kNegInf);
@@ -1184,6 +1186,7 @@ struct JoinArgs {
   float* logp;
   float* lse;
   double* logp64;
+  double* lse64;
   float* coef;
 };
 constexpr int kJoinThreads = 128;
@@ -1217,6 +1220,7 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
     if (A.lse) A.lse[row] = static_cast<float>(st.lse);
     if (A.logp64) {
       A.logp64[row] = st.logp;
+      A.lse64[row] = st.lse;
       A.coef[row] = 0.f;
     }
   }

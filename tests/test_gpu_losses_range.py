@@ -169,3 +169,27 @@ def test_far_logits_next_to_each_other(dev, base, T, V):  # noqa: F811
     p = policy_loss(z.float().to(dev), y.to(dev), torch.ones(2, device=dev), r.logprobs, temperature=T, clip_high=1e9)
     want, tol = ref.gradient(z, y, torch.ones(2, 6, dtype=torch.float64), T, y >= 0)
     assert_rounded(p.grad, -want, tol + (2 * S + 4 * U * logp.abs())[..., None] * want.abs(), "policy")
+
+
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("size", [(4, 8, 64), (64, 32, 64), (2, 300, 256), (20, 8, 1024), (2, 4, 8192), (2, 3, 65536)], ids=str)
+def test_the_preference_gradient_does_not_feel_where_the_logits_lie(dev, size, dtype):  # noqa: F811
+    """Rows whose logits are one number L, around 2000: p = 1 / V, to what the kernels' exponentials are off by. An exponent
+    (base 2) is rounded at most twice below 32, by 2^-20 each, here and in the sum behind lse: 4 ln 2 2^-20 in all, with 16 u
+    for ex2 and the products. An fp32 lse is off by up to 2^-14, and the probabilities as much."""
+    from mote_b200 import preference_loss
+    S, T, V = size
+    gen = torch.Generator().manual_seed(V)
+    L = (2000.0 + 32 * torch.rand(S, T, 1, generator=gen)).to(dtype)
+    lse = L.double() + math.log(V)
+    assert float((lse.float().double() - lse).abs().max()) > 2.0 ** -17   # what an fp32 number would lose: above rel
+    z = L.expand(S, T, V).contiguous()
+    y = torch.randint(0, V, (S, T), generator=gen)
+    r = preference_loss(z.to(dev), y.to(dev), divisor=1.0)
+    coef = torch.where(torch.arange(S) < S // 2, -0.05, 0.05).double().view(S, 1, 1)
+    one = torch.zeros(S, T, V, dtype=torch.float64).scatter_(-1, y[..., None], 1.0)
+    want = coef * (one - 1.0 / V)
+    # the coefficient: both sequences' sums are -T log V, off by T positions of S and by nothing else
+    rel = 4 * math.log(2.0) * 2.0 ** -20 + 16 * U
+    tol = want.abs() * (rel + 0.1 * 2 * T * rel)
+    assert_rounded(r.grad, want, tol, "grad")
