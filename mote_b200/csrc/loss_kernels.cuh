@@ -257,8 +257,9 @@ struct Pairs<float> {
   }
 };
 
-// (largest logit m, sum of exp(x - ref(m))) of a part of a row
-struct Part {
+// (largest logit m, sum of exp(x - ref(m))) of a part of a row. Written to other blocks' shared memory as one value of 8 bytes
+// (store_remote).
+struct alignas(8) Part {
   float m, s;
 };
 __device__ __forceinline__ Part warp_join(Part p, const Rows& R) {
