@@ -363,7 +363,7 @@ MOTEOPT_API int moteopt_selftest_wait_timeout(int mode, double limit_seconds, in
  * not count: its logits are not read, its logp and lse are 0, its gradient is 0. A target >= vocab gives NaN. -inf logits
  * have probability 0. Gradients are written contiguous, [seqs][tokens][vocab], in the logits' type, each rounded once;
  * the sums behind them are fp32 within a row and fp64 above, in a fixed order, so the same call gives the same bits.
- * Outputs and workspaces must not overlap the inputs.
+ * Outputs and workspaces must not overlap the inputs. Every tensor is aligned to its elements (others are refused).
  * At most 2^27 - 1 positions, and at most 3,603,456 bytes a row (1,801,728 bf16 or 900,864 fp32 logits). */
 typedef struct moteopt_logits {
   const void* data;

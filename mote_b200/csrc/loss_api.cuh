@@ -65,6 +65,14 @@ int check_logits(const char* who, const moteopt_logits* z, const moteopt_positio
   return MOTEOPT_OK;
 }
 
+// Pointers of a call, each aligned to its elements of `size` bytes (null ones are)
+int check_aligned(const char* who, size_t size, std::initializer_list<const void*> pointers) {
+  for (const void* p : pointers)
+    if (reinterpret_cast<uint64_t>(p) % size != 0)
+      return fail(MOTEOPT_ERR_INVALID, std::string(who) + ": a tensor is not aligned to its elements");
+  return MOTEOPT_OK;
+}
+
 Per per_of(const moteopt_positions& p) { return Per{static_cast<const float*>(p.data), p.seq_stride, p.token_stride}; }
 
 // A launch behind another one of the same call: its blocks may be placed before that one has ended (they wait for it
@@ -384,6 +392,7 @@ int moteopt_token_logprobs(const moteopt_logits* logits, const moteopt_positions
   MO_TRY(check_logits("moteopt_token_logprobs", logits, targets, &R, temperature));
   if (R.n == 0) return MOTEOPT_OK;
   if (!logprobs) return fail(MOTEOPT_ERR_INVALID, "moteopt_token_logprobs: null output");
+  MO_TRY(check_aligned("moteopt_token_logprobs", 4, {logprobs, lse}));
   Part* parts = nullptr;
   if (!short_rows(logits->dtype, R.vocab)) {
     MO_TRY(check_ws(workspace, workspace_bytes, moteopt_token_logprobs_workspace_size(logits)));
@@ -403,6 +412,8 @@ int moteopt_token_logprobs_backward(const moteopt_logits* logits, const moteopt_
   if (R.n == 0) return MOTEOPT_OK;
   if (!logprobs || !lse || !grad_logprobs || !logprobs->data || !lse->data || !grad_logprobs->data || !grad_logits)
     return fail(MOTEOPT_ERR_INVALID, "moteopt_token_logprobs_backward: null pointer");
+  MO_TRY(check_aligned("moteopt_token_logprobs_backward", 4, {logprobs->data, lse->data, grad_logprobs->data}));
+  MO_TRY(check_aligned("moteopt_token_logprobs_backward", esize(logits->dtype), {grad_logits}));
   int sms = 0;
   MO_TRY(loss_setup(&sms));
   Kept K;
@@ -432,6 +443,9 @@ int moteopt_policy_loss(const moteopt_logits* logits, const moteopt_positions* t
     return fail(MOTEOPT_ERR_INVALID, "moteopt_policy_loss: null pointer");
   if (policy->kl_coef != 0.0 && R.n > 0 && !policy->ref_logprobs.data)
     return fail(MOTEOPT_ERR_INVALID, "moteopt_policy_loss: a KL coefficient without reference log-probabilities");
+  MO_TRY(check_aligned(who, 4, {sums, logprobs, policy->advantages.data, policy->old_logprobs.data, policy->ref_logprobs.data,
+                                policy->weights.data, policy->divisor_device}));
+  MO_TRY(check_aligned(who, esize(logits->dtype), {grad_logits}));
   const PolicyLayout L = policy_layout(R.n);
   MO_TRY(check_ws(workspace, workspace_bytes, L.bytes));
   int sms = 0;
@@ -504,6 +518,8 @@ int moteopt_preference_loss(const moteopt_logits* logits, const moteopt_position
   if (!std::isfinite(p.beta) || !(p.label_smoothing >= 0.0 && p.label_smoothing <= 1.0))
     return fail(MOTEOPT_ERR_INVALID, "moteopt_preference_loss: beta must be finite, label_smoothing in [0, 1]");
   if (p.sequences > 0 && (!rewards || !logprobs)) return fail(MOTEOPT_ERR_INVALID, "moteopt_preference_loss: null pointer");
+  MO_TRY(check_aligned(who, 4, {loss, rewards, logprobs, p.cu_seqlens, p.ref_logprobs, p.divisor_device}));
+  MO_TRY(check_aligned(who, esize(logits->dtype), {grad_logits}));
   const PreferenceLayout L = preference_layout(logits->dtype, R.n, R.vocab, p.sequences / 2);
   MO_TRY(check_ws(workspace, workspace_bytes, L.bytes));
   int sms = 0;

@@ -1,0 +1,39 @@
+"""Calls of the losses on logits that are refused on the host, without a GPU."""
+
+
+def test_tensors_that_are_not_aligned_to_their_elements_are_refused():
+    """Before any device call: the pointers are never followed. One pointer of the call is off by one or two bytes at a time."""
+    from mote_b200 import _lib as L
+    lib, text = L.lib, lambda: L.lib.moteopt_last_error().decode()
+    for dtype, off in ((0, 2), (1, 1)):   # fp32 logits and their gradient, bf16 ones
+        z = L.Logits(256, dtype, 2, 3, 8, 24, 8)
+        y = L.Positions(256, 3, 1)
+        pos = lambda bad: L.Positions(256 + 2 * bad, 3, 1)  # noqa: E731
+
+        def logprobs(k):
+            return lib.moteopt_token_logprobs(z, y, 1.0, 256 + 2 * (k == 0), 256 + 2 * (k == 1), None, 0, None)
+
+        def backward(k):
+            return lib.moteopt_token_logprobs_backward(z, y, 1.0, pos(k == 0), pos(k == 1), pos(k == 2), 256 + off * (k == 3),
+                                                       None)
+
+        def policy(k):
+            p = L.Policy(pos(k == 0), pos(k == 1), pos(k == 2), pos(k == 3), 0.2, 0.2, 0.1, 1.0, 256 + 2 * (k == 4))
+            return lib.moteopt_policy_loss(z, y, p, 1.0, 256 + 2 * (k == 5), 256 + 2 * (k == 6), 256 + off * (k == 7), None, 0,
+                                           None)
+
+        def preference(k):
+            p = L.Preference(2, None, 256 + 2 * (k == 0), 0.1, 0.0, 0, 1.0, 256 + 2 * (k == 1))
+            return lib.moteopt_preference_loss(z, y, p, 1.0, 256 + 2 * (k == 2), 256 + 2 * (k == 3), 256 + 2 * (k == 4),
+                                               256 + off * (k == 5), None, 0, None)
+
+        def packed(k):
+            p = L.Preference(2, 256 + 2 * (k == 0), None, 0.1, 0.0, 0, 1.0, None)
+            return lib.moteopt_preference_loss(L.Logits(256, dtype, 1, 6, 8, 0, 8), y, p, 1.0, 256, 256, 256, 256, None, 0, None)
+
+        # without a GPU no call gets farther than its workspace, so this is what a call with aligned pointers says
+        for call, n in ((backward, 4), (policy, 8), (preference, 6), (packed, 1), (logprobs, 2)):
+            for k in range(n):
+                assert call(k) == -1 and "aligned" in text(), (call.__name__, k, text())
+        for call in (policy, preference, packed):
+            assert call(-1) == -1 and "workspace" in text(), call.__name__
