@@ -72,13 +72,24 @@ def build_binding(force: bool = False, verbose: bool = False) -> Path:
 
 
 def build(force: bool = False, verbose: bool = False, extra: list[str] | None = None, checked: bool = False) -> Path:
-    """nvcc the library (and build the torch binding); `checked` builds libmoteopt_checked.so, which counts failed index checks
-    (moteopt_check_count) instead of the release library."""
-    out = CHECKED_LIB if checked else LIB
-    if not checked:
+    """nvcc the library, then the torch binding, which the library does not need: without torch or a host compiler it is left
+    out with a message. `checked` builds libmoteopt_checked.so, which counts failed index checks (moteopt_check_count), instead
+    of the two."""
+    if checked:
+        return build_library(CHECKED_LIB, verbose, extra)
+    if force or needs_build():
+        build_library(LIB, verbose, extra)
+    try:
         build_binding(force, verbose)
-    if not force and not checked and not needs_build():
-        return LIB
+    except Exception as e:
+        BINDING.unlink(missing_ok=True)   # not the one of another library
+        sys.stderr.write(f"{LIB.name} is built; {BINDING.name} is not, so mote_b200's losses cannot be called: {e}\n")
+    return LIB
+
+
+def build_library(out: Path, verbose: bool = False, extra: list[str] | None = None) -> Path:
+    """nvcc LIB or CHECKED_LIB."""
+    checked = out == CHECKED_LIB
     if checked:
         extra = ["-DMOTE_OPT_CHECKS", *(extra or [])]
     else:   # keep ptxas's resource report (registers, spills, shared memory per kernel) beside the build

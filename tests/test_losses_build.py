@@ -21,3 +21,26 @@ def test_what_goes_to_another_blocks_memory_is_aligned(tmp_path):
     r = subprocess.run([nvcc, *build.ARCH, "-std=c++17", "--expt-relaxed-constexpr", "-I", str(ROOT / "include"), "-I",
                         str(build.CSRC), "-cuda", "-o", str(tmp_path / "part.ii"), str(src)], capture_output=True, text=True)
     assert r.returncode == 0, r.stderr
+
+
+@pytest.mark.parametrize("missing", ["a host compiler", "torch", "a header"])
+def test_the_library_is_built_without_what_the_binding_needs(tmp_path, monkeypatch, capsys, missing):
+    """nvcc alone builds the C library (nvcc is not run here); an older binding does not stay beside it."""
+    import sys
+
+    from mote_b200 import build
+    built = []
+    monkeypatch.setattr(build, "LIB", tmp_path / "libmoteopt.so")
+    monkeypatch.setattr(build, "BINDING", tmp_path / "_torch_losses.so")
+    monkeypatch.setattr(build, "build_library", lambda out, *a, **k: built.append(out) or out, raising=False)
+    build.BINDING.write_bytes(b"of another library")
+    if missing == "a host compiler":
+        monkeypatch.setenv("CXX", str(tmp_path / "no-such-compiler"))
+    elif missing == "torch":
+        monkeypatch.setitem(sys.modules, "torch", None)
+    else:
+        bad = tmp_path / "bad.cpp"
+        bad.write_text('#include "no_such_header.h"\n')
+        monkeypatch.setattr(build, "BINDING_SOURCE", bad)
+    assert build.build(force=True) == build.LIB and built == [build.LIB]
+    assert not build.BINDING.exists() and "_torch_losses.so is not" in capsys.readouterr().err
