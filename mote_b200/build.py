@@ -48,17 +48,28 @@ def needs_build() -> bool:
     return any(p.stat().st_mtime > t for p in SOURCES + HEADERS)
 
 
+def built_for() -> str:
+    """What a binding depends on beside its sources: it uses torch's and Python's C++ objects as their headers lay them out."""
+    import torch
+    return f"torch {torch.__version__}, C++ ABI {int(torch._C._GLIBCXX_USE_CXX11_ABI)}, {sys.implementation.cache_tag}"
+
+
+def binding_fits() -> bool:
+    """Whether the binding is there and was built for this torch and this Python (it holds their names as its doc string)."""
+    return BINDING.exists() and f"built for {built_for()}.".encode() in BINDING.read_bytes()
+
+
 def build_binding(force: bool = False, verbose: bool = False) -> Path:
     """g++ the torch binding of the losses (no CUDA code; it is given libmoteopt.so's functions when it is imported)."""
-    sources = [BINDING_SOURCE, ROOT / "include" / "moteopt.h"]
-    if not force and BINDING.exists() and all(p.stat().st_mtime <= BINDING.stat().st_mtime for p in sources):
-        return BINDING
     import torch
+    sources = [BINDING_SOURCE, ROOT / "include" / "moteopt.h", Path(__file__).resolve()]
+    if not force and binding_fits() and all(p.stat().st_mtime <= BINDING.stat().st_mtime for p in sources):
+        return BINDING
     from torch.utils import cpp_extension as ext
     tmp = BINDING.with_suffix(".so.tmp")
     inc = [str(ROOT / "include"), sysconfig.get_paths()["include"], *ext.include_paths("cuda")]
     cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
-           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *[a for d in inc for a in ("-I", d)],
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f'-DMOTEOPT_BUILT_FOR="{built_for()}"', *[a for d in inc for a in ("-I", d)],
            str(BINDING_SOURCE), "-o", str(tmp), *[a for d in ext.library_paths("cuda") for a in ("-L", d)], "-lc10",
            "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python"]
     if verbose:

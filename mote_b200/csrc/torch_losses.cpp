@@ -322,7 +322,9 @@ PyMethodDef methods[] = {{"init", fast<init>(), METH_FASTCALL, nullptr},
                          {"policy_loss", fast<policy_loss>(), METH_FASTCALL, nullptr},
                          {"preference_loss", fast<preference_loss>(), METH_FASTCALL, nullptr},
                          {nullptr, nullptr, 0, nullptr}};
-PyModuleDef module = {PyModuleDef_HEAD_INIT, "_torch_losses", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
+// looked for by build.py before the binding is loaded
+constexpr const char* kDoc = "The losses' torch binding, built for " MOTEOPT_BUILT_FOR ".";
+PyModuleDef module = {PyModuleDef_HEAD_INIT, "_torch_losses", kDoc, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace
 

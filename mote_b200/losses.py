@@ -27,7 +27,7 @@ from typing import NamedTuple, Optional, Tuple, Union
 import torch
 
 from . import _lib as L
-from .build import BINDING
+from . import build
 from .functional import _device_divisor
 
 Divisor = Union[None, float, torch.Tensor]
@@ -35,9 +35,11 @@ Divisor = Union[None, float, torch.Tensor]
 
 def _load():
     import importlib.util
-    if not BINDING.exists():
-        raise ImportError(f"{BINDING.name} not found at {BINDING}: build it with `python -m mote_b200.build`")
-    spec = importlib.util.spec_from_file_location("mote_b200._torch_losses", BINDING)
+    if not build.BINDING.exists():
+        raise ImportError(f"{build.BINDING.name} not found at {build.BINDING}: build it with `python -m mote_b200.build`")
+    if not build.binding_fits():
+        raise ImportError(f"{build.BINDING} was not built for {build.built_for()}: build it again with `python -m mote_b200.build`")
+    spec = importlib.util.spec_from_file_location("mote_b200._torch_losses", build.BINDING)
     mod = importlib.util.module_from_spec(spec)
     spec.loader.exec_module(mod)
     names = ("moteopt_last_error", "moteopt_token_logprobs_workspace_size", "moteopt_token_logprobs", "moteopt_token_logprobs_backward",

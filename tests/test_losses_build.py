@@ -1,5 +1,7 @@
 """What the compilers see of the losses on logits, without a GPU."""
 
+import os
+import shutil
 import subprocess
 from pathlib import Path
 
@@ -44,3 +46,23 @@ def test_the_library_is_built_without_what_the_binding_needs(tmp_path, monkeypat
         monkeypatch.setattr(build, "BINDING_SOURCE", bad)
     assert build.build(force=True) == build.LIB and built == [build.LIB]
     assert not build.BINDING.exists() and "_torch_losses.so is not" in capsys.readouterr().err
+
+
+def test_a_binding_of_another_torch_is_built_again_and_not_loaded(tmp_path, monkeypatch):
+    import torch
+
+    from mote_b200 import build, losses
+    binding = tmp_path / "_torch_losses.so"
+    shutil.copy2(build.BINDING, binding)
+    monkeypatch.setattr(build, "BINDING", binding)
+    monkeypatch.setattr(losses, "BINDING", binding, raising=False)
+    os.utime(binding)   # newer than every source
+    kept = binding.stat().st_ino
+    assert build.build_binding() == binding and binding.stat().st_ino == kept
+    monkeypatch.setattr(torch, "__version__", "2.0.0+other")
+    with pytest.raises(ImportError, match="built for torch 2.0.0.other"):
+        losses._load()
+    assert build.build_binding() == binding and binding.stat().st_ino != kept
+    binding.unlink()
+    with pytest.raises(ImportError, match="not found"):
+        losses._load()
