@@ -1,5 +1,8 @@
 """Calls of the losses on logits that are refused on the host, without a GPU."""
 
+import pytest
+import torch
+
 
 def test_tensors_that_are_not_aligned_to_their_elements_are_refused():
     """Before any device call: the pointers are never followed. One pointer of the call is off by one or two bytes at a time."""
@@ -37,3 +40,39 @@ def test_tensors_that_are_not_aligned_to_their_elements_are_refused():
                 assert call(k) == -1 and "aligned" in text(), (call.__name__, k, text())
         for call in (policy, preference, packed):
             assert call(-1) == -1 and "workspace" in text(), call.__name__
+
+
+def test_forward_mode_tangents_are_refused():
+    """The losses have no forward mode: a tangent is not dropped without a word."""
+    import torch.autograd.forward_ad as fwd
+
+    import mote_b200 as m
+    z, y, f = torch.randn(2, 3, 8), torch.zeros(2, 3, dtype=torch.int64), torch.randn(2, 3)
+    with fwd.dual_level():
+        zd = fwd.make_dual(z, torch.ones_like(z))
+        for call in (lambda: m.token_logprobs(zd, y), lambda: m.token_logprobs_backward(zd, y, f, f, f),
+                     lambda: m.policy_loss(zd, y, f, f), lambda: m.preference_loss(zd, y)):
+            with pytest.raises(ValueError, match="forward-mode"):
+                call()
+        # the logits' own check, that they are on the GPU, comes later than this one
+        with pytest.raises(ValueError, match="CUDA"):
+            m.token_logprobs(zd.detach(), y)
+
+
+@pytest.mark.gpu
+def test_forward_mode_tangents_of_the_other_arguments_are_refused():
+    import torch.autograd.forward_ad as fwd
+
+    import mote_b200 as m
+    if not torch.cuda.is_available():
+        pytest.skip("needs a GPU")
+    dev = torch.device("cuda", 0)
+    z, y, f = torch.randn(2, 3, 8, device=dev), torch.zeros(2, 3, dtype=torch.int64, device=dev), torch.randn(2, 3, device=dev)
+    one = torch.ones((), device=dev)
+    with fwd.dual_level():
+        fd, s, d = fwd.make_dual(f, f), fwd.make_dual(f[:, 0].contiguous(), one.expand(2)), fwd.make_dual(one, one)
+        for call in (lambda: m.policy_loss(z, y, fd, f), lambda: m.policy_loss(z, y, f, fd), lambda: m.policy_loss(z, y, f, f, fd),
+                     lambda: m.policy_loss(z, y, f, f, weights=fd), lambda: m.token_logprobs_backward(z, y, f, f, fd),
+                     lambda: m.preference_loss(z, y, s), lambda: m.policy_loss(z, y, f, f, divisor=d)):
+            with pytest.raises(ValueError, match="forward-mode"):
+                call()
