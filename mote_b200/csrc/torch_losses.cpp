@@ -124,9 +124,6 @@ at::Tensor make(at::IntArrayRef sizes, at::ScalarType type, const at::Tensor& z)
 }
 at::Tensor scratch(size_t bytes, const at::Tensor& z) { return make({static_cast<int64_t>(bytes)}, at::kByte, z); }
 
-void checked(int rc, const char* what) {
-  if (rc != MOTEOPT_OK) refuse(lib_error, std::string(what) + " failed (" + std::to_string(rc) + "): " + api.last_error());
-}
 moteopt_stream_t stream_of(const at::Tensor& z) {
   return reinterpret_cast<moteopt_stream_t>(c10::cuda::getCurrentCUDAStream(z.get_device()).stream());
 }
@@ -148,7 +145,28 @@ PyObject* tuple(std::initializer_list<at::Tensor> ts) {
   return r;
 }
 
-// An entry point: its device current, nothing recorded for autograd, C++ errors as Python's
+// Other Python threads run while a call allocates and launches: it waits where the launch queue is full, on work that may itself
+// wait for one of them (a host function in a stream), or for memory.
+struct Threads {
+  PyThreadState* const state = PyEval_SaveThread();
+  ~Threads() { PyEval_RestoreThread(state); }
+};
+
+// `call` allocates and launches, the logits' device current; an error of the library is Python's
+template <typename F>
+void checked(const char* what, const at::Tensor& z, F call) {
+  int rc;
+  std::string why;
+  {
+    const Threads others;
+    const c10::cuda::CUDAGuard guard(z.device());
+    rc = call();
+    if (rc != MOTEOPT_OK) why = api.last_error();   // of this thread
+  }
+  if (rc != MOTEOPT_OK) refuse(lib_error, std::string(what) + " failed (" + std::to_string(rc) + "): " + why);
+}
+
+// An entry point: nothing recorded for autograd, C++ errors as Python's
 template <typename F>
 PyObject* entry(Py_ssize_t given, Py_ssize_t wanted, F body) {
   if (given != wanted) {
@@ -176,14 +194,16 @@ PyObject* token_logprobs(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const moteopt_logits L = logits_of(z);
     const moteopt_positions Y = targets_of(y, z);
     const double t = number(a[2]);
-    const c10::cuda::CUDAGuard guard(z.device());
-    const at::Tensor logp = make(y.sizes(), at::kFloat, z), lse = make(y.sizes(), at::kFloat, z);
-    const size_t bytes = api.logprobs_size(&L);
-    at::Tensor ws;
-    if (bytes > kHeader) ws = scratch(bytes, z);
-    checked(api.token_logprobs(&L, &Y, t, logp.data_ptr<float>(), lse.data_ptr<float>(),
-                               ws.defined() ? ws.data_ptr() : nullptr, ws.defined() ? bytes : 0, stream_of(z)),
-            "moteopt_token_logprobs");
+    at::Tensor logp, lse;
+    checked("moteopt_token_logprobs", z, [&] {
+      logp = make(y.sizes(), at::kFloat, z);
+      lse = make(y.sizes(), at::kFloat, z);
+      const size_t bytes = api.logprobs_size(&L);
+      at::Tensor ws;
+      if (bytes > kHeader) ws = scratch(bytes, z);
+      return api.token_logprobs(&L, &Y, t, logp.data_ptr<float>(), lse.data_ptr<float>(),
+                                ws.defined() ? ws.data_ptr() : nullptr, ws.defined() ? bytes : 0, stream_of(z));
+    });
     return tuple({logp, lse});
   });
 }
@@ -198,10 +218,11 @@ PyObject* token_logprobs_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const moteopt_positions P = positions_of(a[2], y, "logprobs"), S = positions_of(a[3], y, "lse");
     const moteopt_positions G = positions_of(a[4], y, "grad_logprobs", true);
     const double t = number(a[5]);
-    const c10::cuda::CUDAGuard guard(z.device());
-    const at::Tensor grad = make(z.sizes(), z.scalar_type(), z);
-    checked(api.token_logprobs_backward(&L, &Y, t, &P, &S, &G, grad.data_ptr(), stream_of(z)),
-            "moteopt_token_logprobs_backward");
+    at::Tensor grad;
+    checked("moteopt_token_logprobs_backward", z, [&] {
+      grad = make(z.sizes(), z.scalar_type(), z);
+      return api.token_logprobs_backward(&L, &Y, t, &P, &S, &G, grad.data_ptr(), stream_of(z));
+    });
     return wrap(grad);
   });
 }
@@ -228,15 +249,16 @@ PyObject* policy_loss(PyObject*, PyObject* const* a, Py_ssize_t n) {
     P.divisor_device = scalar_of(a[11], z);
     const bool with_grad = truth(a[12]);
     if (P.kl_coef != 0.0 && a[4] == Py_None) refuse(PyExc_ValueError, "policy_loss: kl_coef needs ref_logprobs");
-    const c10::cuda::CUDAGuard guard(z.device());
-    const size_t bytes = api.policy_size(&L);
-    const at::Tensor ws = scratch(bytes, z);
-    const at::Tensor sums = make({4}, at::kFloat, z), logp = make(y.sizes(), at::kFloat, z);
-    at::Tensor grad;
-    if (with_grad) grad = make(z.sizes(), z.scalar_type(), z);
-    checked(api.policy(&L, &Y, &P, t, sums.data_ptr<float>(), logp.data_ptr<float>(), with_grad ? grad.data_ptr() : nullptr,
-                       ws.data_ptr(), bytes, stream_of(z)),
-            "moteopt_policy_loss");
+    at::Tensor sums, logp, grad;
+    checked("moteopt_policy_loss", z, [&] {
+      const size_t bytes = api.policy_size(&L);
+      const at::Tensor ws = scratch(bytes, z);
+      sums = make({4}, at::kFloat, z);
+      logp = make(y.sizes(), at::kFloat, z);
+      if (with_grad) grad = make(z.sizes(), z.scalar_type(), z);
+      return api.policy(&L, &Y, &P, t, sums.data_ptr<float>(), logp.data_ptr<float>(), with_grad ? grad.data_ptr() : nullptr,
+                        ws.data_ptr(), bytes, stream_of(z));
+    });
     return tuple({element(sums, 0), element(sums, 1), element(sums, 2), element(sums, 3), logp, grad});
   });
 }
@@ -279,16 +301,17 @@ PyObject* preference_loss(PyObject*, PyObject* const* a, Py_ssize_t n) {
     P.divisor = number(a[8]);
     P.divisor_device = scalar_of(a[9], z);
     const bool with_grad = truth(a[10]);
-    const c10::cuda::CUDAGuard guard(z.device());
-    const size_t bytes = api.preference_size(&L, P.sequences);
-    const at::Tensor ws = scratch(bytes, z);
-    const at::Tensor loss = make({}, at::kFloat, z), rewards = make({P.sequences}, at::kFloat, z);
-    const at::Tensor logp = make({P.sequences}, at::kFloat, z);
-    at::Tensor grad;
-    if (with_grad) grad = make(z.sizes(), z.scalar_type(), z);
-    checked(api.preference(&L, &Y, &P, t, loss.data_ptr<float>(), rewards.data_ptr<float>(), logp.data_ptr<float>(),
-                           with_grad ? grad.data_ptr() : nullptr, ws.data_ptr(), bytes, stream_of(z)),
-            "moteopt_preference_loss");
+    at::Tensor loss, rewards, logp, grad;
+    checked("moteopt_preference_loss", z, [&] {
+      const size_t bytes = api.preference_size(&L, P.sequences);
+      const at::Tensor ws = scratch(bytes, z);
+      loss = make({}, at::kFloat, z);
+      rewards = make({P.sequences}, at::kFloat, z);
+      logp = make({P.sequences}, at::kFloat, z);
+      if (with_grad) grad = make(z.sizes(), z.scalar_type(), z);
+      return api.preference(&L, &Y, &P, t, loss.data_ptr<float>(), rewards.data_ptr<float>(), logp.data_ptr<float>(),
+                            with_grad ? grad.data_ptr() : nullptr, ws.data_ptr(), bytes, stream_of(z));
+    });
     return tuple({loss, rewards, logp, grad});
   });
 }
