@@ -46,6 +46,8 @@ std::string shape_of(const at::Tensor& t) {
 const at::Tensor& tensor(PyObject* o, const char* what) {
   if (!THPVariable_Check(o)) refuse(PyExc_TypeError, std::string(what) + " must be a tensor, got " + Py_TYPE(o)->tp_name);
   const at::Tensor& t = THPVariable_Unpack(o);
+  if (t.is_neg())   // its memory holds the values before the negation
+    refuse(PyExc_ValueError, std::string(what) + " is a view that negates when it is read: resolve_neg() it");
   if (t._fw_grad(0).defined())
     refuse(PyExc_ValueError, std::string(what) + " carries a forward-mode tangent, which the losses do not have: detach() it");
   return t;

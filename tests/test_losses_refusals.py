@@ -59,6 +59,32 @@ def test_forward_mode_tangents_are_refused():
             m.token_logprobs(zd.detach(), y)
 
 
+def test_views_that_negate_when_they_are_read_are_refused():
+    """The imaginary part of a conjugate: torch keeps the values and a flag."""
+    import mote_b200 as m
+    z, y = torch.randn(2, 3, 8, dtype=torch.complex64).conj().imag, torch.zeros(2, 3, dtype=torch.int64)
+    assert z.is_neg()
+    with pytest.raises(ValueError, match="resolve_neg"):
+        m.token_logprobs(z, y)
+    with pytest.raises(ValueError, match="CUDA"):
+        m.token_logprobs(z.resolve_neg(), y)
+
+
+@pytest.mark.gpu
+def test_views_that_negate_are_refused_from_every_argument():
+    import mote_b200 as m
+    if not torch.cuda.is_available():
+        pytest.skip("needs a GPU")
+    dev = torch.device("cuda", 0)
+    z, y, f = torch.randn(2, 3, 8, device=dev), torch.zeros(2, 3, dtype=torch.int64, device=dev), torch.zeros(2, 3, device=dev)
+    n = torch.ones(2, 3, dtype=torch.complex64, device=dev).conj().imag
+    for call in (lambda: m.policy_loss(z, y, n, f), lambda: m.policy_loss(z, y, f, n), lambda: m.policy_loss(z, y, f, f, n),
+                 lambda: m.policy_loss(z, y, f, f, weights=n[:, 0]), lambda: m.token_logprobs_backward(z, y, f, f, n),
+                 lambda: m.preference_loss(z, y, n[:, 0]), lambda: m.policy_loss(z, y, f, f, divisor=n[0, 0])):
+        with pytest.raises(ValueError, match="resolve_neg"):
+            call()
+
+
 @pytest.mark.gpu
 def test_forward_mode_tangents_of_the_other_arguments_are_refused():
     import torch.autograd.forward_ad as fwd
