@@ -302,10 +302,13 @@ constexpr int kSumBlocks = 128;
 struct PolicyLayout {
   size_t partials, sums, bytes;
 };
-PolicyLayout policy_layout(int64_t n) {
+PolicyLayout policy_layout(int dtype, int64_t n, int64_t vocab) {
+  // a row of partials for each block: of long rows one a position, of short ones at most one for a row a warp. Up to 128 KB are
+  // not counted out
+  const int64_t rows = short_rows(dtype, vocab) ? std::max(cdiv(n, kTileWarps), std::min<int64_t>(n, kSumShare)) : n;
   PolicyLayout L;
   L.partials = kHeaderBytes;
-  L.sums = align_up(L.partials + 32 * static_cast<size_t>(n), 256);   // at most one row of partials a position
+  L.sums = align_up(L.partials + 32 * static_cast<size_t>(rows), 256);
   L.bytes = L.sums + 32 * kSumBlocks;
   return L;
 }
@@ -426,7 +429,7 @@ int moteopt_token_logprobs_backward(const moteopt_logits* logits, const moteopt_
 
 size_t moteopt_policy_loss_workspace_size(const moteopt_logits* logits) {
   if (!shape_fits(logits)) return 0;
-  return policy_layout(logits->seqs * logits->tokens).bytes;
+  return policy_layout(logits->dtype, logits->seqs * logits->tokens, logits->vocab).bytes;
 }
 
 int moteopt_policy_loss(const moteopt_logits* logits, const moteopt_positions* targets, const moteopt_policy* policy,
@@ -446,7 +449,7 @@ int moteopt_policy_loss(const moteopt_logits* logits, const moteopt_positions* t
   MO_TRY(check_aligned(who, 4, {sums, logprobs, policy->advantages.data, policy->old_logprobs.data, policy->ref_logprobs.data,
                                 policy->weights.data, policy->divisor_device}));
   MO_TRY(check_aligned(who, esize(logits->dtype), {grad_logits}));
-  const PolicyLayout L = policy_layout(R.n);
+  const PolicyLayout L = policy_layout(logits->dtype, R.n, R.vocab);
   MO_TRY(check_ws(workspace, workspace_bytes, L.bytes));
   int sms = 0;
   MO_TRY(loss_setup(&sms));
