@@ -474,14 +474,14 @@ struct Running {
 #pragma unroll
     for (int k = 0; k < kN; ++k) t = vec_max<T>(t, v[k]);
     const float top = W::top(t), above = (top - m) * R.c_hi;
-    if (!(above <= limit)) {   // hardly ever, or always about a far m
+    if (!(above <= limit)) {   // hardly ever, or always about a far m, whose limit is a NaN (above itself may be -inf)
       if (above > kSlack) {
         const float by = rescale(m, top, R);
         s0 *= by;
         s1 *= by;
         m = top;
         ex = Ex(top, R);
-        limit = ex.far() ? kNegInf : kSlack;
+        limit = ex.far() ? NAN : kSlack;
       }
       if (ex.far()) {
 #pragma unroll
@@ -729,7 +729,7 @@ __device__ __forceinline__ void pair_loss(const PairArgs& A, uint32_t pair) {   
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
     const float c = sh_c[k];
-        if (kShort) {
+    if (kShort) {
 #pragma unroll 1
       for (int64_t i = b[k] + threadIdx.x; i < e[k]; i += kThreads) A.coef[i] = c;
     } else {

@@ -193,3 +193,33 @@ def test_the_preference_gradient_does_not_feel_where_the_logits_lie(dev, size, d
     rel = 4 * math.log(2.0) * 2.0 ** -20 + 16 * U
     tol = want.abs() * (rel + 0.1 * 2 * T * rel)
     assert_rounded(r.grad, want, tol, "grad")
+
+
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("V", [271, 2200, 6000, 50021, 300000])
+def test_logits_farther_apart_than_fp32(dev, V, dtype):  # noqa: F811
+    """A logit of 3e38 (1e36 and a temperature of 0.01) and the others ten times below it or at its negative: their difference
+    in exponents is no fp32 number. The large one in the first, a middle and the last line of a row."""
+    from mote_b200 import policy_loss, token_logprobs, token_logprobs_backward
+    sure, lost = [0, 1, 2, 3, 4], [5, 6, 7, 8]   # rows whose target is the large one, and another
+    for top, T in ((3e38, 1.0), (1e36, 0.01), (-1e35, 0.01)):
+        z = torch.empty(1, 9, V)
+        z[0] = top / 10 if top > 0 else top * 30
+        z[0, 3:6] = -abs(top) * 10 if top < 0 else -top
+        for r, j in enumerate((0, V // 2, V - 1) * 3):
+            z[0, r, j] = top
+        z = z.to(dtype)
+        y = torch.tensor([[0, V // 2, V - 1, 0, V // 2, V - 2, V // 3, 1, 0]])
+        r = token_logprobs(z.to(dev), y.to(dev), temperature=T)
+        assert not bool(r.logprobs[0, sure].any()), (top, r.logprobs)   # of probability 1
+        assert float(r.logprobs[0, lost].max()) <= -1e35, (top, r.logprobs)
+        one = torch.ones(1, 9, device=dev)
+        p = policy_loss(z.to(dev), y.to(dev), one, torch.zeros(1, 9, device=dev), temperature=T)
+        assert torch.equal(p.logprobs, r.logprobs) and not bool(p.grad.any())   # the ratio is 0 where it is not sure
+        d = token_logprobs_backward(z.to(dev), y.to(dev), r.logprobs, r.lse, one, temperature=T)
+        if T == 1.0:   # their lse is an fp32 number
+            want = torch.zeros(9, V)
+            for i in lost:
+                want[i, y[0, i]] = 1.0
+                want[i, (0, V // 2, V - 1)[i % 3]] = -1.0
+            assert torch.equal(d[0].float().cpu(), want)
