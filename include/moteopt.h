@@ -353,8 +353,8 @@ MOTEOPT_API int moteopt_selftest_grad_divide(const float* a, float d, float* out
 MOTEOPT_API int moteopt_selftest_wait_timeout(int mode, double limit_seconds, int* counter, int* status,
                                               unsigned long long* elapsed_ns, moteopt_stream_t stream);
 
-/* ---- losses on logits, for post-training (the reference trains on such losses in mote/train/dpo.py, kto.py and
- *      rlvr.py, with the clip and AdamW of this library's kind behind them: dpo.py:217, kto.py:151, rlvr.py:308).
+/* ---- losses on logits, for post-training: the usual ones of loops like the reference's, which end in a clip and AdamW of
+ *      this library's kind (mote/train/dpo.py:217, kto.py:151, rlvr.py:308).
  *
  * The logits are [seqs][tokens][vocab], fp32 or bf16, the last axis contiguous and the others with strides (in elements),
  * so a shifted view needs no copy; packed sequences are seqs = 1. `targets` are int64. For a position with logits z,
@@ -384,7 +384,8 @@ MOTEOPT_API int moteopt_token_logprobs(const moteopt_logits* logits, const moteo
                                        float* logprobs, float* lse, void* workspace, size_t workspace_bytes,
                                        moteopt_stream_t stream);
 /* grad_logits = grad_logprobs ([j == y] - exp(x_j - lse)) / temperature from the logprobs and lse that
- * moteopt_token_logprobs gave for these logits. A position whose grad_logprobs is 0 gets 0, whatever its logits hold. */
+ * moteopt_token_logprobs gave for these logits. A position whose grad_logprobs is 0 gets 0, whatever its logits hold. lse is
+ * fp32: where it is of size L, the probabilities are off by 6e-8 L. */
 MOTEOPT_API int moteopt_token_logprobs_backward(const moteopt_logits* logits, const moteopt_positions* targets,
                                                 double temperature, const moteopt_positions* logprobs,
                                                 const moteopt_positions* lse, const moteopt_positions* grad_logprobs,
@@ -416,7 +417,8 @@ typedef struct moteopt_preference {
   int64_t sequences;
   const int32_t* cu_seqlens;        /* NULL: sequence q is logits' seq q. Else (logits->seqs == 1) device, sequences + 1
                                        ascending row offsets, held to [0, tokens]; rows outside [first, last) do not
-                                       count */
+                                       count. Where they descend, a row of several sequences has the coefficient of
+                                       one of them */
   const float* ref_logprobs;        /* device [sequences], or NULL: 0 */
   double beta, label_smoothing;
   int average;

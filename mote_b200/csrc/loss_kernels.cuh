@@ -1,6 +1,6 @@
 // Losses on logits: token log-probabilities (forward and backward), the clipped policy loss with a KL term and the paired
-// preference loss, each with its gradient in the logits. The steps that train on them are the reference's post-training
-// loops (mote/train/dpo.py:217, kto.py:151, rlvr.py:308: clip and AdamW after such a loss).
+// preference loss, each with its gradient in the logits. Loops like the reference's train on them (mote/train/dpo.py:217,
+// kto.py:151, rlvr.py:308: clip and AdamW after such a loss).
 //
 // Per row (one position) with logits z, temperature T, x = z / T and target y:
 //   logp = x_y - lse(x),  dlogp/dz_j = ([j == y] - exp(x_j - lse)) / T
@@ -11,8 +11,9 @@
 // so that neither logp nor 1 - p_y cancels where the model is sure of its target (p_y -> 1). The exponentials and their sums
 // are fp32, a position's logp is kept in 64 bits, and the sums over positions are in 64 bits.
 //
-// All kernels are memory-bound in principle (2 or 4 bytes read per logit, as many written for a gradient); the exponential
-// is next: one ex2 per logit at 16 per clock and SM takes 0.73 of the time in which the copy bandwidth reads a bf16 logit.
+// By their bytes all kernels are memory-bound (2 or 4 read per logit, as many written for a gradient); the exponential is next:
+// one ex2 per logit at 16 per clock and SM takes 0.73 of the time in which the copy bandwidth reads a bf16 logit. Only the stream
+// and the gradient of long rows come near either.
 #pragma once
 
 #include <cfloat>
@@ -86,7 +87,8 @@ __device__ __forceinline__ F2 fma2(F2 x, F2 y, F2 z) {
 // exactly. c_hi has 12 bits, so that what the first multiply-add leaves to the second is not lost under half a unit of its
 // result (with one float for c, or a full one for c_hi, its rounding leans every exponent of a row the same way: 5e-8 of a sum,
 // and the sums of thousands of positions keep it). b is base + 16: ex2 is asked for values below -1 only, where its relative
-// error has the mean of -5.05e-8 that row_stat takes out. c_lo > 0 keeps -inf a -inf.
+// error has the mean of -5.05e-8 that row_stat takes out. So exponents are rounded between 16 and 32, twice, by 2^-20 at most: an
+// exponential is off by up to 1.3e-6, mostly by 2e-7. c_lo > 0 keeps -inf a -inf.
 //
 // Where |m c| >= 2^18 (a far m: a mask of -1e9, say), ref(m) is m / T itself and m is taken from z first: the difference is
 // exact where its exponential is not 0, and b is kAbove alone. A product with m there would leave half a unit of m c, which is
@@ -1234,9 +1236,9 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
 // it loaded itself; the blocks' parts meet in distributed shared memory; one thread forms the row's values, and all go over
 // the slice again for the gradient, by the lines of the output.
 //
-// What bounds it is the two exponentials of a logit and the arithmetic around them (4 x 1024 x 32768 bf16: 109 us, 0.75 of the
-// copy bandwidth's rate; the special-function units are busy for 0.64 of it). Blocks that stay, and ask for the next row's
-// lines while they store this one's gradient, took 115 us.
+// Nothing is full (4 x 1024 x 32768 bf16: 109 us, 0.75 of the copy bandwidth's rate; special-function units 0.63, issue slots
+// 0.53, DRAM 0.55): a block loads, exchanges, forms its values and stores in turn, and three of them share an SM. Blocks that
+// stay, and ask for the next row's lines while they store this one's gradient, took 115 us.
 // Exponentials again instead of kept ones: 32 fp32 exponentials a thread in registers left two blocks of 512 threads an SM,
 // whose chain of load, cluster exchange and row values then stands between them (8192 rows of 131072: 1497 us).
 struct SliceArgs {

@@ -1,19 +1,21 @@
-"""Losses on logits for post-training, with their gradients: what the reference's preference and policy loops
-(mote/train/dpo.py, kto.py, rlvr.py) compute between the model and the clip + AdamW step (dpo.py:217, kto.py:151,
-rlvr.py:308) that `fused_step` replaces.
+"""Losses on logits for post-training, with their gradients: what stands between a model and the clip + AdamW step that
+`fused_step` replaces in loops like the reference's (mote/train/dpo.py:217, kto.py:151, rlvr.py:308).
 
     r = policy_loss(logits, targets, advantages, old_logprobs, ref_logprobs, kl_coef=0.04)
     logits.backward(r.grad)
     fused_step(opt, max_norm=1.0, grad_divisor=r.count)      # the losses are sums: divided here, over any micro-batches
 
 The calls read logits and write their gradient in the logits' type; nothing is recorded for autograd, so the gradient is
-handed on with `logits.backward(grad)` (a step that is captured into a CUDA graph captures that too).
+handed on with `logits.backward(grad)` (a step that is captured into a CUDA graph captures that too). Tensors with a
+forward-mode tangent are refused.
 
 Logits are [S, T, V] (S sequences of T positions) or [N, V] (packed positions), fp32 or bf16, on the GPU. The last axis has
 to be contiguous; the others may be strided (`logits[:, :-1]` needs no copy). A position whose target is negative does not
 count: it is not read, its log-probability and its gradient are 0, whatever its logits hold. A target of V or more makes its
 position NaN. `targets` is int64, one shape with the logits' leading axes; the label of a position stands at that position
 (shift the targets, or the logits, by one for next-token prediction).
+
+`temperature` divides the logits as torch divides fp32 by a number: a product with its fp32 reciprocal.
 
 Two calls on the same inputs give the same bits. Scratch memory is allocated per call on the current stream. The argument
 checks and allocations are in C++ (csrc/torch_losses.cpp, mote_b200/_torch_losses.so).
@@ -91,8 +93,8 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, *, temperature: 
 def token_logprobs_backward(logits: torch.Tensor, targets: torch.Tensor, logprobs: torch.Tensor, lse: torch.Tensor,
                             grad_logprobs: torch.Tensor, *, temperature: float = 1.0) -> torch.Tensor:
     """The gradient in the logits of sum(grad_logprobs * logprobs), from what token_logprobs gave for the same logits,
-    targets and temperature: grad ([j == y] - softmax_j) / temperature. Positions whose grad_logprobs is 0 get 0, whatever
-    their logits hold. `grad_logprobs` is the targets' shape, or [S] for [S, T] targets."""
+    targets and temperature: grad ([j == y] - exp(x_j - lse)) / temperature. Positions whose grad_logprobs is 0 get 0, whatever
+    their logits hold. lse is fp32: where it is of size L, the probabilities are off by 6e-8 L. `grad_logprobs` is the targets' shape, or [S] for [S, T] targets."""
     return _torch.token_logprobs_backward(logits, targets, logprobs, lse, grad_logprobs, temperature)
 
 
@@ -100,7 +102,7 @@ def policy_loss(logits: torch.Tensor, targets: torch.Tensor, advantages: torch.T
                 ref_logprobs: Optional[torch.Tensor] = None, *, weights: Optional[torch.Tensor] = None,
                 clip_low: float = 0.2, clip_high: float = 0.2, kl_coef: float = 0.0, temperature: float = 1.0,
                 divisor: Divisor = None, grad: bool = True) -> PolicyLoss:
-    """The clipped policy loss with a KL term, and its gradient in the logits (rlvr.py's loop). Per counted position:
+    """The clipped policy loss with a KL term, and its gradient in the logits (for a loop like rlvr.py). Per counted position:
 
         r = exp(logp - old),  d = ref - logp
         loss += w (-min(r A, clip(r, 1 - clip_low, 1 + clip_high) A) + kl_coef (exp(d) - d - 1)) / divisor
@@ -119,10 +121,11 @@ def preference_loss(logits: torch.Tensor, targets: torch.Tensor, ref_logprobs: O
                     cu_seqlens: Optional[torch.Tensor] = None, beta: float = 0.1, label_smoothing: float = 0.0,
                     average: bool = False, temperature: float = 1.0, divisor: Divisor = None,
                     grad: bool = True) -> PreferenceLoss:
-    """The paired preference loss, and its gradient in the logits (dpo.py's loop). The sequences are the chosen ones, then
-    the rejected ones in the same order: [S, T, V] logits with S even, or [N, V] with `cu_seqlens` (int32, S + 1 ascending
-    row offsets on the device, held to [0, N]; rows outside them do not count). With s a sequence's summed log-probability (its mean with
-    `average`; 0 where no position counts) and ref_logprobs [S] the reference model's (none: 0):
+    """The paired preference loss, and its gradient in the logits (for a loop like dpo.py). The sequences are the chosen ones,
+    then the rejected ones in the same order: [S, T, V] logits with S even, or [N, V] with `cu_seqlens` (int32, S + 1 ascending
+    row offsets on the device, held to [0, N]; rows outside them do not count; where offsets descend, a row of several
+    sequences has the coefficient of one of them). With s a sequence's summed log-probability (its mean with `average`; 0 where
+    no position counts) and ref_logprobs [S] the reference model's (none: 0):
 
         u = beta ((s_i - ref_i) - (s_j - ref_j)),  j = i + S / 2
         loss = sum_i (-(1 - label_smoothing) log sigmoid(u) - label_smoothing log sigmoid(-u)) / divisor
