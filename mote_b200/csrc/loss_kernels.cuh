@@ -351,7 +351,7 @@ __device__ __forceinline__ RowLoss policy_row_loss(double logp, const Policy& P,
 
 // The policy loss of a row: its sums' terms, and its gradient's factors: 2^up f exp(x_j - ref(m)), gy at the target. A slope
 // beyond 2^96 stays in 64 bits to the factors, and what is left above 2^64 goes into the exponents (Ex): products with small
-// probabilities are finite then, and those with a probability of 0 are 0.
+// probabilities are finite then, and those with a probability of 0 (one below 2^-126 counts as 0) are 0.
 struct PolicyRow {
   double part[4];
   float f, gy, up;
