@@ -598,6 +598,13 @@ struct Kept {
   int pairs;
   float* loss;
 };
+// A factor near fp32's end, whose product with kFix would overflow: its power of two goes into the exponents (Ex)
+__device__ __forceinline__ void lift(float& f, float& up) {
+  if (fabsf(f) >= 0x1p96f) {
+    f *= 0x1p-64f;
+    up += 64.f;
+  }
+}
 // exp(x_j - lse) = exp(x_j - ref(m)) exp(ref(m) - lse) with m = lse T
 struct KeptRow {
   float m, f, gy, up;   // d_j = 2^up exp(x_j - ref(m)) f, gy at the target
@@ -619,6 +626,7 @@ __device__ __forceinline__ KeptRow kept_row(const Kept& K, const Rows& R, uint32
     r.f = -g;
     r.up = static_cast<float>((r.m * R.inv_t - lse) * kLog2e);
   }
+  lift(r.f, r.up);
   r.gy = -expm1f(lp) * g;
   return r;
 }
@@ -821,7 +829,8 @@ __device__ __forceinline__ void tile_rows(const TileArgs& A, unsigned char* sm, 
   using W = Word<T>;
   constexpr uint32_t kPer = 16 / sizeof(T);
   constexpr int kAtOnce = 32 / kG;
-  __shared__ float4 sh_row[kTileWarps * kTileRows];   // (m, s, target logit, counts), then (m, f, gy, up; -inf where the row's gradient is 0)
+  // a row's (m, s, target logit, counts), then (m, f, gy, up; -inf where its gradient is 0)
+  __shared__ float4 sh_row[kTileWarps * kTileRows];
   const Rows& R = A.R;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = lane / kG;
   const uint32_t gl = lane % kG;
@@ -1000,7 +1009,9 @@ __device__ __forceinline__ void tile_rows(const TileArgs& A, unsigned char* sm, 
       if (lane < rows) {
         const float coef = __ldcg(A.coef + first + lane), g = static_cast<float>(coef * R.inv_t);
         const float4 v = own[lane];
-        own[lane] = make_float4(v.x, -g * v.y, g * v.z, coef != 0.f ? v.w : kNegInf);
+        float f = -g * v.y, up = v.w;
+        lift(f, up);
+        own[lane] = make_float4(v.x, f, g * v.z, coef != 0.f ? up : kNegInf);
       }
       __syncwarp();
     }

@@ -223,3 +223,30 @@ def test_logits_farther_apart_than_fp32(dev, V, dtype):  # noqa: F811
                 want[i, y[0, i]] = 1.0
                 want[i, (0, V // 2, V - 1)[i % 3]] = -1.0
             assert torch.equal(d[0].float().cpu(), want)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("size", [(2, 6, 271), (2, 600, 60), (2, 6, 2200), (2, 6, 6000), (2, 3, 50021)], ids=str)
+def test_coefficients_near_the_end_of_fp32(dev, size, dtype):  # noqa: F811
+    """A gradient of 1e37 that reaches the log-probabilities, a beta of 1e37 whose pair's preference is wrong: their products
+    with probabilities are fp32 numbers, 0 in columns of probability 0."""
+    from mote_b200 import preference_loss, token_logprobs, token_logprobs_backward
+    S, T, V = size
+    z, y, _ = cpu_case(S, T, V, dtype, V, prompt=0.0)
+    y = y % (V // 2)
+    z[..., V // 2 + 3:] = -math.inf
+    r = token_logprobs(z.to(dev), y.to(dev))
+    lse = ref.row_values(z, y, 1.0)[1]
+    g = torch.full((S, T), 1e37)
+    want, tol = ref.gradient(z, y, g.double(), 1.0, y >= 0)
+    tol = tol + want.abs() * 4 * U * (lse.abs() + 1)[..., None]
+    d = token_logprobs_backward(z.to(dev), y.to(dev), r.logprobs, r.lse, g.to(dev))
+    assert_rounded(d, want, tol, "backward")
+    assert not bool(d[..., V // 2 + 3:].any())
+    wrong = torch.tensor([1e3, -1e3], device=dev)   # u = beta (s_0 - s_1 - 2000): -beta sigmoid(-u) is -beta
+    q = preference_loss(z.to(dev), y.to(dev), wrong, beta=1e37)
+    sums = r.logprobs.double().sum(-1)
+    assert float(sums[0] - sums[1]) < 1900
+    sign = torch.tensor([-1.0, 1.0]).view(2, 1, 1)
+    assert_rounded(q.grad, sign * want, tol, "preference")
+    assert not bool(q.grad[..., V // 2 + 3:].any())
